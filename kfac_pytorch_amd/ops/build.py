@@ -12,6 +12,8 @@ import importlib.machinery
 import os
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 OPS_DIR = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(OPS_DIR, "csrc")
@@ -37,13 +39,26 @@ def _sources(name: str = EXT_NAME):
             if f.endswith(".hip")]
 
 
+def _headers(name: str = EXT_NAME):
+    src_dir = os.path.join(OPS_DIR, EXTENSIONS[name][0])
+    return [os.path.join(src_dir, f) for f in sorted(os.listdir(src_dir))
+            if f.endswith(".h")]
+
+
+# packed fp32 instructions (v_pk_add/mul/fma_f32) are kept out: some of their
+# forms have given wrong results on this card
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang",
+                  "-packed-fp32-ops"]
+
+
 def needs_build(name: str = EXT_NAME) -> bool:
     so = ext_path(name)
     if not os.path.exists(so):
         return True
     so_mtime = os.path.getmtime(so)
     return any(os.path.getmtime(s) > so_mtime
-               for s in _sources(name) + [os.path.abspath(__file__)])
+               for s in _sources(name) + _headers(name)
+               + [os.path.abspath(__file__)])
 
 
 def build_all(verbose: bool = True, force: bool = False):
@@ -64,34 +79,47 @@ def build(verbose: bool = True, force: bool = False,
     import sysconfig
     py_include = sysconfig.get_paths()["include"]
 
-    cmd = [
-        os.path.join(ce.ROCM_HOME or "/opt/rocm", "bin", "hipcc"),
-        f"--offload-arch={GFX_ARCH}",
-        "-O3", "-std=c++17", "-shared", "-fPIC",
+    hipcc = [os.path.join(ce.ROCM_HOME or "/opt/rocm", "bin", "hipcc"),
+             f"--offload-arch={GFX_ARCH}"]
+    flags = [
+        "-O3", "-std=c++17", "-fPIC",
         f"-DTORCH_EXTENSION_NAME={name}",
         "-DTORCH_API_INCLUDE_EXTENSION_H",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-    ]
-    cmd += ce.COMMON_HIP_FLAGS + ce.COMMON_HIPCC_FLAGS
+    ] + NO_PACKED_FP32
+    flags += ce.COMMON_HIP_FLAGS + ce.COMMON_HIPCC_FLAGS
     for inc in ce.include_paths("cuda"):
-        cmd.append(f"-I{inc}")
-    cmd.append(f"-I{py_include}")
-    cmd += _sources(name)
+        flags.append(f"-I{inc}")
+    flags.append(f"-I{py_include}")
+    link = ["-shared", "-fPIC"]
     for lp in ce.library_paths("cuda"):
-        cmd.append(f"-L{lp}")
-    cmd += ["-ltorch", "-ltorch_hip", "-lc10", "-lc10_hip", "-ltorch_python",
-            "-lamdhip64"] + EXTENSIONS[name][1] + ["-o", so]
+        link.append(f"-L{lp}")
+    link += ["-ltorch", "-ltorch_hip", "-lc10", "-lc10_hip",
+             "-ltorch_python", "-lamdhip64"] + EXTENSIONS[name][1]
 
     if verbose:
         print(f"[kfac build] hipcc -> {os.path.basename(so)} "
               f"({GFX_ARCH})", flush=True)
-    try:
-        subprocess.run(cmd, check=True, capture_output=True, text=True)
-    except subprocess.CalledProcessError as e:
-        sys.stderr.write(e.stdout or "")
-        sys.stderr.write(e.stderr or "")
-        raise RuntimeError(
-            f"hipcc build of {name} failed (see output above)") from e
+
+    def run(cmd):
+        try:
+            subprocess.run(cmd, check=True, capture_output=True, text=True)
+        except subprocess.CalledProcessError as e:
+            sys.stderr.write(e.stdout or "")
+            sys.stderr.write(e.stderr or "")
+            raise RuntimeError(
+                f"hipcc build of {name} failed (see output above)") from e
+
+    # a file each at once: most of a compile is torch's headers
+    with tempfile.TemporaryDirectory() as tmp, \
+            ThreadPoolExecutor(max_workers=4) as pool:
+        sources = _sources(name)
+        objs = [os.path.join(tmp, os.path.basename(s) + ".o")
+                for s in sources]
+        list(pool.map(lambda so_: run(hipcc + flags + ["-c", so_[0], "-o",
+                                                       so_[1]]),
+                      zip(sources, objs)))
+        run(hipcc + objs + link + ["-o", so])
     return so
 
 

@@ -30,7 +30,7 @@ setup(
     description="MI355X-native distributed K-FAC for PyTorch-ROCm",
     packages=find_packages(include=["kfac_pytorch_amd",
                                     "kfac_pytorch_amd.*"]),
-    package_data={"kfac_pytorch_amd.ops": ["*.so", "csrc/*.hip",
+    package_data={"kfac_pytorch_amd.ops": ["*.so", "csrc/*.hip", "csrc/*.h",
                                            "csrc_rccl/*.hip",
                                            "csrc_solver/*.hip"]},
     cmdclass={"build_ext": HipBuildExt},
