@@ -167,3 +167,23 @@ def has_jacobi_eigh(m: int) -> bool:
         return False
     return (hasattr(mod, "jacobi_eigh_batched")
             and m <= int(mod.jacobi_eigh_max_dim()))
+
+
+# -- cross entropy of a vocabulary projection ---------------------------------
+def vocab_loss_forward(hidden, weight, target, bias, ignore_index: int,
+                       eps: float, reduction: str):
+    """(loss of every row, total or None, log-sum-exp of the kept rows, the
+    kept rows' numbers) -- the last two are what the backward pass needs."""
+    return _load().vocab_loss_forward(hidden, weight, target, bias,
+                                      ignore_index, eps, reduction == "sum",
+                                      reduction == "mean")
+
+
+def vocab_loss_backward(up, hidden, weight, bias, lse, ints, eps: float,
+                        reduction: str, need_x: bool, need_w: bool,
+                        need_b: bool):
+    """(d hidden, d weight, d bias); None for those not asked for."""
+    return _load().vocab_loss_backward(up, hidden, weight, bias, lse, ints,
+                                       eps, reduction == "none",
+                                       reduction == "mean", need_x, need_w,
+                                       need_b)

@@ -424,6 +424,16 @@ int jacobi_eigh_max_dim();
 std::vector<torch::Tensor> jacobi_eigh_batched(
     std::vector<torch::Tensor> mats);
 
+// defined in vocab_loss_entry.hip
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>
+vocab_loss_forward(torch::Tensor hidden, torch::Tensor weight,
+                   torch::Tensor target, std::optional<torch::Tensor> bias,
+                   int64_t ignore_index, double eps, bool sum, bool mean);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> vocab_loss_backward(
+    torch::Tensor up, torch::Tensor hidden, torch::Tensor weight,
+    std::optional<torch::Tensor> bias, torch::Tensor lse, torch::Tensor ints,
+    double eps, bool each, bool mean, bool need_x, bool need_w, bool need_b);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "MI355X-native HIP kernels for distributed K-FAC";
   m.def("eigen_scale_", &eigen_scale_entry,
@@ -437,4 +447,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "batched LDS-resident Jacobi symmetric eigensolver (packed W, V)");
   m.def("jacobi_eigh_max_dim", &jacobi_eigh_max_dim,
         "largest dim the Jacobi kernel handles");
+  m.def("vocab_loss_forward", &vocab_loss_forward,
+        "cross entropy of a vocabulary projection, no logits in memory");
+  m.def("vocab_loss_backward", &vocab_loss_backward,
+        "gradients of vocab_loss_forward");
 }

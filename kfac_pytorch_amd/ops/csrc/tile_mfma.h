@@ -1,0 +1,274 @@
+// The matrix-product loop that the vocabulary-loss kernels share.
+//
+// C[m, n] = sum_k A(m, k) B(n, k), fp32 accumulation, one BM x BN tile of C
+// per workgroup.  An operand lies in memory either k-inner (row m, k
+// contiguous) or k-outer (row k, m contiguous).  Both kinds are staged by
+// 16-byte loads that go from memory straight to LDS, 128 bytes of k for each
+// of the tile's rows, in two buffers: the loads of the next slice of k are in
+// flight while the matrix cores work on this one.
+//
+// Loads straight to LDS write lane i's 16 bytes at base + 16 i, so a layout
+// without bank conflicts is made by choosing which chunk each lane fetches:
+//   k-inner: row r keeps its 16-byte chunk c at slot c ^ (r & 7); the 16 rows
+//     of a fragment's chunk then fall on all bank groups.
+//   k-outer, 16 bits: fragments are read by the transposing LDS read, whose 64
+//     lanes touch 32 bytes of each of 16 k-rows; the 32-byte column is xored
+//     with the 4 bits of k that tell those 16 rows apart.
+//   k-outer, 32 bits: fragments are read word by word, 64 bytes of each of 4
+//     k-rows; the 64-byte column is xored with the 2 bits of k.
+//
+// Rows past the end of an operand, and k past its end, are turned into
+// out-of-range buffer offsets, for which the hardware returns zeros.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace tile {
+
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using s16x4 = __attribute__((ext_vector_type(4))) short;
+using s16x8 = __attribute__((ext_vector_type(8))) short;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using lds_void = __attribute__((address_space(3))) void;
+using lds_s16x4 = __attribute__((address_space(3))) s16x4;
+
+constexpr uint32_t OUT_OF_RANGE = 0x7ffffff0u;
+constexpr long MAX_RECORDS = 0x7fffff00l;
+
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p,
+                                                           long bytes) {
+  const long n = bytes < 0 ? 0 : (bytes > MAX_RECORDS ? MAX_RECORDS : bytes);
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n,
+                                           0x00020000);
+}
+
+// one 16-byte fragment piece: 8 values of 16 bits, or 4 of 32
+union Frag {
+  s16x8 h;
+  f32x4 f;
+  s16x4 q[2];
+  float w[4];
+};
+
+template <class T>
+__device__ __forceinline__ f32x4 mma(const Frag& a, const Frag& b, f32x4 c);
+
+template <>
+__device__ __forceinline__ f32x4 mma<__bf16>(const Frag& a, const Frag& b,
+                                             f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+      __builtin_bit_cast(bf16x8, a.h), __builtin_bit_cast(bf16x8, b.h), c, 0,
+      0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma<_Float16>(const Frag& a, const Frag& b,
+                                               f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+      __builtin_bit_cast(f16x8, a.h), __builtin_bit_cast(f16x8, b.h), c, 0, 0,
+      0);
+}
+// lane group l >> 4 holds 4 consecutive k of its row; the instruction takes
+// one k of each group, and any pairing of k will do that both operands share
+template <>
+__device__ __forceinline__ f32x4 mma<float>(const Frag& a, const Frag& b,
+                                            f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.f[j], b.f[j], c, 0, 0, 0);
+  }
+  return c;
+}
+
+// A tile shape: BM x BN of C by WM x WN waves.
+template <int BM_, int BN_, int WM_, int WN_>
+struct Shape {
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int NW = WM * WN, THREADS = NW * 64;
+  static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
+  static constexpr int LDS = 2 * (BM + BN) * 128;
+};
+
+// One operand of a tile: R rows (of C's rows or columns).
+template <class T, bool KOUTER, int R, int NW>
+struct Operand {
+  static constexpr int SZ = sizeof(T);
+  static constexpr int E = 16 / SZ;       // values in a chunk
+  static constexpr int BK = 128 / SZ;     // k values of a slice
+  static constexpr int BYTES = R * 128;
+  static constexpr int LOADS = R / 8 / NW;
+  static constexpr int NC = R * SZ / 16;  // chunks of a k-outer row
+  static_assert(R % (8 * NW) == 0, "whole loads for every wave");
+
+  const char* base;
+  long ld_bytes;
+  uint32_t off[LOADS];
+  int extent;  // rows of the operand from this tile's first on
+  int kend;
+
+  __device__ __forceinline__ void init(const T* p, long ld, int r0, int rows,
+                                       int kend_, int wave, int lane) {
+    ld_bytes = ld * SZ;
+    extent = rows - r0;
+    kend = kend_;
+    if constexpr (KOUTER) {
+      base = reinterpret_cast<const char*>(p) + (long)r0 * SZ;
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int at = (j * NW + wave) * 64 + lane;
+        const int k = at / NC;
+        const int c = (at % NC) ^ swizzle(k);
+        off[j] = (uint32_t)(k * ld_bytes + c * 16);
+      }
+    } else {
+      base = reinterpret_cast<const char*>(p) + (long)r0 * ld_bytes;
+      const int c = (lane & 7) ^ (lane >> 3);
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        const int r = (j * NW + wave) * 8 + (lane >> 3);
+        off[j] = (uint32_t)(r * ld_bytes + c * 16);
+      }
+    }
+  }
+
+  __device__ __forceinline__ static int swizzle(int k) {
+    if constexpr (SZ == 2) {
+      return (((k & 3) | (((k >> 3) & 3) << 2)) << 1) & (NC - 1);
+    } else {
+      return (((k >> 2) & 3) << 2) & (NC - 1);
+    }
+  }
+
+  // start the loads of the slice at k0 into `lds`
+  __device__ __forceinline__ void load(char* lds, int k0, int wave,
+                                       int lane) const {
+    if constexpr (KOUTER) {
+      const __amdgpu_buffer_rsrc_t r =
+          make_rsrc(base + (long)k0 * ld_bytes,
+                    (long)(kend - k0 - 1) * ld_bytes + (long)extent * SZ);
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (lds_void*)(lds + (j * NW + wave) * 1024), 16, off[j], 0, 0,
+            0);
+      }
+    } else {
+      const int rows = extent < R ? extent : R;
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(
+          base, (long)(rows - 1) * ld_bytes + (long)kend * SZ);
+      const int c = (lane & 7) ^ (lane >> 3);
+      const bool past = k0 + c * E >= kend;
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j) {
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            r, (lds_void*)(lds + (j * NW + wave) * 1024), 16,
+            past ? OUT_OF_RANGE : off[j], k0 * SZ, 0, 0);
+      }
+    }
+  }
+
+  // the fragment of rows row0 .. row0+15, half `ks` of the slice
+  __device__ __forceinline__ static Frag read(const char* lds, int row0,
+                                              int ks, int lane) {
+    Frag v;
+    const int i = lane & 15, g = lane >> 4;
+    if constexpr (!KOUTER) {
+      const int c = (ks * 4 + g) ^ (i & 7);
+      v.h = *reinterpret_cast<const s16x8*>(lds + (row0 + i) * 128 + c * 16);
+    } else if constexpr (SZ == 2) {
+      const int k = ks * 32 + g * 8 + (i >> 2);
+      const int c = ((row0 >> 3) + ((i >> 1) & 1)) ^ swizzle(k);
+      const char* p = lds + k * (R * 2) + c * 16 + (i & 1) * 8;
+      v.q[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)p);
+      v.q[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_s16x4*)(p + 4 * (R * 2)));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = ks * 16 + g * 4 + j;
+        const int c = ((row0 + i) >> 2) ^ swizzle(k);
+        v.w[j] = *reinterpret_cast<const float*>(lds + k * (R * 4) + c * 16 +
+                                                 (i & 3) * 4);
+      }
+    }
+    return v;
+  }
+};
+
+// acc += the product over k in [kbeg, kend); kbeg is a multiple of BK.  A
+// k-inner operand needs whole chunks up to kend; rows of a k-outer one from
+// `krows` on are taken for zeros.  `smem` is S::LDS bytes.  Every wave of the workgroup calls it with the same
+// arguments; on return all of them are done with smem.
+template <class T, bool KA, bool KB, class S>
+__device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
+                                        const T* B, long ldb, int n0, int N,
+                                        int kbeg, int kend, int krows,
+                                        char* smem,
+                                        f32x4 (&acc)[S::MI][S::NI]) {
+  using OA = Operand<T, KA, S::BM, S::NW>;
+  using OB = Operand<T, KB, S::BN, S::NW>;
+  constexpr int BK = OA::BK;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = (wave / S::WN) * (S::MI * 16);
+  const int wn = (wave % S::WN) * (S::NI * 16);
+  OA a;
+  OB b;
+  a.init(A, lda, m0, M, KA ? krows : kend, wave, lane);
+  b.init(B, ldb, n0, N, KB ? krows : kend, wave, lane);
+
+  char* cur = smem;
+  char* nxt = smem + S::LDS / 2;
+  if (kbeg < kend) {
+    a.load(cur, kbeg, wave, lane);
+    b.load(cur + OA::BYTES, kbeg, wave, lane);
+  }
+  for (int k0 = kbeg; k0 < kend; k0 += BK) {
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (k0 + BK < kend) {
+      a.load(nxt, k0 + BK, wave, lane);
+      b.load(nxt + OA::BYTES, k0 + BK, wave, lane);
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      Frag fb[S::NI];
+#pragma unroll
+      for (int ni = 0; ni < S::NI; ++ni) {
+        fb[ni] = OB::read(cur + OA::BYTES, wn + ni * 16, ks, lane);
+      }
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) {
+        const Frag fa = OA::read(cur, wm + mi * 16, ks, lane);
+#pragma unroll
+        for (int ni = 0; ni < S::NI; ++ni) {
+          acc[mi][ni] = mma<T>(fa, fb[ni], acc[mi][ni]);
+        }
+      }
+    }
+    char* t = cur;
+    cur = nxt;
+    nxt = t;
+  }
+  __syncthreads();
+}
+
+// Which tile a workgroup takes.  Workgroups go to the 8 XCDs in turn; each
+// XCD has an L2 of its own, so each gets one run of neighbouring tiles, and a
+// run walks 8 tiles of m for each tile of n before the next n.
+__device__ __forceinline__ void pick(int id, int mt, int nt, int* m, int* n) {
+  const int total = mt * nt;
+  const int q = total >> 3, r = total & 7;
+  const int x = id & 7, y = id >> 3;
+  const int p = x * q + (x < r ? x : r) + y;
+  const int group = p / (8 * nt);
+  const int first = group * 8;
+  const int wide = mt - first < 8 ? mt - first : 8;
+  const int in = p - first * nt;
+  *m = first + in % wide;
+  *n = in / wide;
+}
+
+}  // namespace tile

@@ -1,0 +1,159 @@
+"""Cross entropy of a vocabulary projection, without the logits in memory.
+
+``linear_cross_entropy(hidden, weight, target, bias)`` is
+``F.cross_entropy(F.linear(hidden, weight, bias), target)``: the output layer
+and the loss of a language model in one operator.  K-FAC leaves that layer out
+(``exclude_vocabulary_size``), so nothing needs its input and output as
+tensors of their own.
+
+    z[n, v] = sum_d hidden[n, d] weight[v, d] + bias[v]
+    loss[n] = log sum_v exp z[n, v] - (1 - eps) z[n, target[n]]
+              - eps / V sum_v z[n, v]
+
+On the GPU, hand-written MFMA kernels (``csrc/vocab_loss.hip``) make the logits
+tile by tile in registers; the backward pass makes them once more, piece by
+piece of the vocabulary, in the inputs' type.  Sums, losses and the log-sum-exp
+are fp32.  On the CPU the plain expression above runs.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn.functional as F
+
+__all__ = ["linear_cross_entropy"]
+
+_REDUCTIONS = ("mean", "sum", "none")
+_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+class _VocabLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, bias, target, ignore_index, eps,
+                reduction):
+        from kfac_pytorch_amd.ops import _ext
+        loss, total, lse, ints = _ext.vocab_loss_forward(
+            hidden, weight, target, bias, ignore_index, eps, reduction)
+        ctx.save_for_backward(hidden, weight, bias, lse, ints)
+        ctx.eps = eps
+        ctx.reduction = reduction
+        return loss if reduction == "none" else total
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, up):
+        from kfac_pytorch_amd.ops import _ext
+        hidden, weight, bias, lse, ints = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        dx, dw, db = _ext.vocab_loss_backward(
+            up.contiguous(), hidden, weight, bias, lse, ints, ctx.eps,
+            ctx.reduction, need[0], need[1], need[2] and bias is not None)
+        return dx, dw, db, None, None, None, None
+
+
+def _check(hidden, weight, target, bias, label_smoothing, reduction):
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be one of "
+                         f"{_REDUCTIONS}, got {reduction!r}")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError("linear_cross_entropy: label_smoothing must be in "
+                         f"[0, 1], got {label_smoothing}")
+    if hidden.dim() < 1 or weight.dim() != 2 \
+            or hidden.size(-1) != weight.size(1):
+        raise ValueError("linear_cross_entropy: hidden (..., d) and weight "
+                         f"(V, d) expected, got {tuple(hidden.shape)} and "
+                         f"{tuple(weight.shape)}")
+    if target.shape != hidden.shape[:-1]:
+        raise ValueError("linear_cross_entropy: target must have the shape "
+                         f"{tuple(hidden.shape[:-1])}, got "
+                         f"{tuple(target.shape)}")
+    if bias is not None and bias.shape != weight.shape[:1]:
+        raise ValueError("linear_cross_entropy: bias must have the shape "
+                         f"{tuple(weight.shape[:1])}, got "
+                         f"{tuple(bias.shape)}")
+    if target.dtype not in (torch.int64, torch.int32):
+        raise TypeError("linear_cross_entropy: target must be int64 or "
+                        f"int32, got {target.dtype}")
+    if weight.size(0) == 0 or weight.size(1) == 0:
+        raise ValueError("linear_cross_entropy: weight is empty")
+    for name, t in (("weight", weight), ("target", target), ("bias", bias)):
+        if t is not None and t.device != hidden.device:
+            raise ValueError(f"linear_cross_entropy: {name} is on "
+                             f"{t.device}, hidden on {hidden.device}")
+
+
+def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
+                         target: torch.Tensor,
+                         bias: Optional[torch.Tensor] = None, *,
+                         ignore_index: int = -100,
+                         label_smoothing: float = 0.0,
+                         reduction: str = "mean") -> torch.Tensor:
+    """Cross entropy of ``F.linear(hidden, weight, bias)`` against ``target``.
+
+    Args:
+      hidden: (..., d), bf16, fp16 or fp32, any strides.
+      weight: (V, d), the type of ``hidden``.
+      target: (...), int64 or int32; rows with ``ignore_index`` count for
+        nothing, whatever their hidden states hold, and get zero gradients.
+      bias: (V,), or None.
+      label_smoothing: as in ``F.cross_entropy``: the target keeps
+        ``1 - eps``, and ``eps`` is spread over the whole vocabulary.
+      reduction: ``"mean"`` over the rows that count (NaN if none does, with
+        zero gradients), ``"sum"``, or ``"none"`` (ignored rows are 0).
+
+    Returns fp32 (a scalar, or one loss for each row).  Under autocast the
+    floating arguments are cast as ``F.linear`` casts them.  A target outside
+    the vocabulary raises on the CPU; on the GPU, where raising would mean to
+    wait for the device, that row's loss and the gradients become NaN.
+    Gradients can be taken once (no double backward).
+    """
+    _check(hidden, weight, target, bias, label_smoothing, reduction)
+    kind = hidden.device.type
+    if torch.is_autocast_enabled(kind):
+        t = torch.get_autocast_dtype(kind)
+        hidden, weight = hidden.to(t), weight.to(t)
+        bias = bias.to(t) if bias is not None else None
+    if hidden.dtype != weight.dtype or (
+            bias is not None and bias.dtype != weight.dtype):
+        raise TypeError("linear_cross_entropy: hidden, weight and bias must "
+                        f"have one dtype, got {hidden.dtype}, {weight.dtype}"
+                        + (f", {bias.dtype}" if bias is not None else ""))
+
+    if not hidden.is_cuda:
+        wide = (lambda a: a if a is None or a.dtype == torch.float64
+                else a.float())
+        with torch.autocast(kind, enabled=False):
+            z = F.linear(wide(hidden), wide(weight), wide(bias))
+            loss = F.cross_entropy(
+                z.reshape(-1, z.size(-1)), target.reshape(-1).long(),
+                ignore_index=ignore_index, label_smoothing=label_smoothing,
+                reduction=reduction)
+        return loss.view(target.shape) if reduction == "none" else loss
+
+    if hidden.dtype not in _TYPES:
+        raise TypeError("linear_cross_entropy: bf16, fp16 or fp32 expected "
+                        f"on the GPU, got {hidden.dtype}")
+    rows = hidden.reshape(-1, hidden.size(-1))
+    if rows.size(0) == 0:
+        # F.cross_entropy's values, with a graph to hidden, weight and bias
+        zero = rows.sum() + weight[:0].sum()
+        zero = zero + (bias[:0].sum() if bias is not None else 0.0)
+        if reduction == "none":
+            return zero.float() + torch.empty(
+                target.shape, device=hidden.device)
+        return zero.float() / 0.0 if reduction == "mean" else zero.float()
+    flat = target.reshape(-1).contiguous()
+    if torch.is_grad_enabled() and (
+            rows.requires_grad or weight.requires_grad
+            or (bias is not None and bias.requires_grad)):
+        loss = _VocabLoss.apply(rows, weight, bias, flat, int(ignore_index),
+                                float(label_smoothing), reduction)
+    else:
+        from kfac_pytorch_amd.ops import _ext
+        loss, total, _, _ = _ext.vocab_loss_forward(
+            rows, weight, flat, bias, int(ignore_index),
+            float(label_smoothing), reduction)
+        loss = loss if reduction == "none" else total
+    return loss.view(target.shape) if reduction == "none" else loss

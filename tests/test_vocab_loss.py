@@ -1,0 +1,450 @@
+"""linear_cross_entropy against the formula in float64.
+
+Tolerances.  u is half a step of a type relative to the value (bf16 2^-8,
+fp16 2^-11, fp32 2^-24).  With S = sum_d |x||w| + |b|:
+
+* a logit's fp32 sum over d terms is off by at most about (d + 2) 2^-24 S, and
+  a loss is a difference and a log-sum of logits: two logits' error, plus the
+  exponentials' (a few 2^-23) and the rounding of the loss itself.
+* g = c (p - y) is p times (1 + that error), rounded once to the inputs' type
+  (fp32: not at all); a gradient is a sum of products of g, off by
+  (u + logit error + terms 2^-24) sum |g||w|, plus u of its own rounding.
+"""
+
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from kfac_pytorch_amd import ops
+
+IGNORE = -100
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11,
+        torch.float32: 2.0 ** -24}
+needs_gpu = pytest.mark.skipif(not torch.cuda.is_available(),
+                               reason="needs GPU")
+
+
+def inputs(rows, dim, vocab, dtype, bias, ignored=0.0, seed=0,
+           device="cuda", ints=torch.int64):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, dim, generator=g).to(dtype)
+    w = (torch.randn(vocab, dim, generator=g) * 2 / math.sqrt(dim)).to(dtype)
+    b = torch.randn(vocab, generator=g).to(dtype) if bias else None
+    t = torch.randint(vocab, (rows,), generator=g)
+    drop = torch.rand(rows, generator=g) < ignored
+    t = t.masked_fill(drop, IGNORE).to(ints)
+    put = (lambda a: None if a is None else a.to(device))
+    return put(x), put(w), put(b), put(t)
+
+
+def formula(x, w, b, t, eps, up):
+    """float64: losses, gradients of sum(up * loss), and the bounds' sums."""
+    x, w = x.double().cpu(), w.double().cpu()
+    b = torch.zeros(w.size(0), dtype=torch.float64) if b is None \
+        else b.double().cpu()
+    t = t.long().cpu()
+    keep = t != IGNORE
+    xs = torch.where(keep[:, None], x, torch.zeros(()).double())
+    z = xs @ w.t() + b
+    size = (xs.abs() @ w.abs().t() + b.abs()).amax(1)
+    y = torch.full_like(z, eps / w.size(0))
+    y[torch.arange(len(t)), t.clamp(min=0)] += 1 - eps
+    lse = torch.logsumexp(z, 1)
+    loss = torch.where(keep, lse - (y * z).sum(1), torch.zeros(()).double())
+    g = (z - lse[:, None]).exp() - y
+    g = torch.where(keep[:, None], g * up.double().cpu()[:, None],
+                    torch.zeros(()).double())
+    return {"loss": loss, "size": size, "lse": lse,
+            "dx": g @ w, "dw": g.t() @ xs, "db": g.sum(0),
+            "sx": g.abs() @ w.abs(), "sw": g.abs().t() @ xs.abs(),
+            "sb": g.abs().sum(0), "g": g, "keep": keep,
+            "c": torch.where(keep, up.double().cpu().abs(),
+                             torch.zeros(()).double()),
+            "share": eps / w.size(0)}
+
+
+def logit_error(ref, dim):
+    return (dim + 8) * 2.0 ** -24 * float(ref["size"].max())
+
+
+def check(name, got, want, bound):
+    off = (got.double().cpu() - want).abs()
+    assert torch.isfinite(got.double()).all(), name
+    worst = (off - bound).max()
+    assert worst <= 0, f"{name}: {float(worst)} past the bound, off by up " \
+                       f"to {float(off.max())}"
+
+
+def check_all(ref, loss, grads, x, w, b, dtype, rows, lift=0.0):
+    dim, vocab = x.size(1), w.size(0)
+    u, e = HALF[dtype], 2 * logit_error(ref, dim)
+    if loss is not None:
+        check("loss", loss, ref["loss"],
+              e + 16 * 2.0 ** -24 * (ref["lse"].abs() + 1)
+              + 2.0 ** -23 * ref["size"])
+    if grads is None:
+        return
+    # the smallest steps of fp16 and of exp's flush to zero
+    tiny = 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -120
+    round_g = 0.0 if dtype == torch.float32 else u
+    # p = exp(z - lse) is off by the logits' error times p; off the target p
+    # is at most |g| / c + eps / V, at the target at most 1
+    gabs = ref["g"].abs()
+    rel = round_g + 8 * 2.0 ** -24
+    wa, xa = w.double().cpu().abs(), x.double().cpu().abs()
+    xa = torch.where(ref["keep"][:, None], xa, torch.zeros(()).double())
+    p_err = e * (gabs + ref["share"] * ref["c"][:, None])
+    at_target = e * ref["c"]
+    sx = rel * ref["sx"] + p_err @ wa + (2 * at_target)[:, None] * wa.amax(0)
+    sw = rel * ref["sw"] + p_err.t() @ xa \
+        + 2 * at_target.max() * xa.amax(0)
+    terms = 2.0 ** -24
+    check("dx", grads[0], ref["dx"], sx + (vocab + 8) * terms * ref["sx"]
+          + u * ref["dx"].abs() + sx * u + tiny)
+    check("dw", grads[1], ref["dw"], sw + (rows + 8) * terms * ref["sw"]
+          + u * ref["dw"].abs() + sw * u + tiny)
+    if b is not None:
+        sb = 8 * 2.0 ** -24 * ref["sb"] + p_err.sum(0) + 2 * at_target.max()
+        check("db", grads[2], ref["db"], sb + (rows + 8) * terms * ref["sb"]
+              + u * ref["db"].abs() + sb * u + tiny)
+
+
+def run(x, w, b, t, eps=0.0, reduction="mean", up=None):
+    leaves = [a.detach().requires_grad_() for a in (x, w, b) if a is not None]
+    loss = ops.linear_cross_entropy(
+        leaves[0], leaves[1], t, bias=leaves[2] if b is not None else None,
+        label_smoothing=eps, reduction=reduction)
+    grads = torch.autograd.grad(loss, leaves, grad_outputs=up)
+    return loss.detach(), grads
+
+
+SIZES = [
+    (1, 8, 2), (1, 64, 1000), (3, 1, 5), (17, 33, 129), (128, 64, 128),
+    (129, 72, 257), (35, 256, 3331), (300, 136, 1003), (513, 40, 511),
+]
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("dtype", list(HALF), ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("rows,dim,vocab", SIZES)
+@pytest.mark.parametrize("bias", [False, True])
+def test_each_row(rows, dim, vocab, dtype, bias):
+    x, w, b, t = inputs(rows, dim, vocab, dtype, bias, 0.2, rows + dim)
+    up = torch.linspace(-1.5, 2.0, rows, device="cuda")
+    loss, grads = run(x, w, b, t, reduction="none", up=up)
+    ref = formula(x, w, b, t, 0.0, up)
+    assert loss.dtype == torch.float32 and loss.shape == t.shape
+    assert [g.dtype for g in grads] == [dtype] * len(grads)
+    check_all(ref, loss, grads, x, w, b, dtype, rows)
+    assert not grads[0][t == IGNORE].any() and not loss[t == IGNORE].any()
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("dtype", list(HALF), ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("eps", [0.0, 0.1, 1.0])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_reduced(dtype, eps, reduction):
+    rows, dim, vocab = 200, 96, 700
+    x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.3, 5)
+    kept = int((t != IGNORE).sum())
+    up = torch.tensor(3.0, device="cuda")
+    loss, grads = run(x, w, b, t, eps, reduction, up)
+    each = 3.0 / (kept if reduction == "mean" else 1)
+    ref = formula(x, w, b, t, eps, torch.full((rows,), each))
+    total = ref["loss"].sum() / (kept if reduction == "mean" else 1)
+    per = 2 * logit_error(ref, dim) + 2.0 ** -20 * float(ref["lse"].max() + 1)
+    check("loss", loss, total,
+          per * (1 if reduction == "mean" else kept)
+          + 2.0 ** -23 * abs(float(total)))
+    check_all(ref, None, grads, x, w, b, dtype, rows)
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("rows,dim,vocab,dtype", [
+    (2100, 264, 8200, torch.bfloat16),   # more than 256 wide tiles
+    (2100, 260, 8200, torch.bfloat16),   # and rows that need packing
+    (2100, 264, 8200, torch.float32),
+    (40, 64, 33278, torch.float16),      # a long vocabulary, few rows
+])
+def test_wide_tiles(rows, dim, vocab, dtype):
+    x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.1, 9)
+    up = torch.rand(rows, device="cuda")
+    loss, grads = run(x, w, b, t, 0.05, "none", up)
+    check_all(formula(x, w, b, t, 0.05, up), loss, grads, x, w, b, dtype,
+              rows)
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_ignored_rows_may_hold_anything():
+    x, w, b, t = inputs(130, 64, 300, torch.bfloat16, True, 0.4, 3)
+    want = run(x, w, b, t)
+    dirty = x.clone()
+    gone = (t == IGNORE).nonzero().squeeze(1)
+    dirty[gone[0::3]] = float("nan")
+    dirty[gone[1::3]] = float("inf")
+    dirty[gone[2::3]] = torch.finfo(torch.bfloat16).min
+    got = run(dirty, w, b, t)
+    assert torch.equal(got[0], want[0])
+    for a, c in zip(got[1], want[1]):
+        assert torch.equal(a, c)
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_no_row_counts(reduction):
+    x, w, b, _ = inputs(70, 64, 300, torch.bfloat16, True)
+    t = torch.full((70,), IGNORE, device="cuda")
+    up = torch.ones(70, device="cuda") if reduction == "none" else None
+    loss, grads = run(x, w, b, t, 0.0, reduction, up)
+    if reduction == "mean":
+        assert torch.isnan(loss)
+    else:
+        assert not loss.any()
+    for g in grads:
+        assert not g.any()
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("low", [float("-inf"), "min"])
+def test_entries_masked_by_the_bias(low):
+    """A bias of -inf, or of the type's lowest value, takes entries out."""
+    for dtype in HALF:
+        x, w, b, t = inputs(50, 64, 600, dtype, True, 0.1, 4)
+        out = torch.arange(600, device="cuda") % 3 == 1
+        t = torch.where((t >= 0) & (t % 3 == 1), t - 1, t)
+        out[256:384] = True              # all of one tile
+        t = torch.where((t >= 256) & (t < 384), 0, t)
+        value = torch.finfo(dtype).min if low == "min" else low
+        b = b.masked_fill(out, value)
+        up = torch.ones(50, device="cuda")
+        loss, grads = run(x, w, b, t, 0.0, "none", up)
+        kept = ~out
+        small = (torch.cumsum(kept, 0) - 1)[t.clamp(min=0)]
+        small = torch.where(t == IGNORE, t, small)
+        ref = formula(x, w[kept], b[kept], small, 0.0, up)
+        check_all(ref, loss, [grads[0], grads[1][kept], grads[2][kept]],
+                  x, w[kept], b[kept], dtype, 50)
+        assert not grads[1][out].any() and not grads[2][out].any()
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_infinite_and_nan_logits():
+    x, w, b, t = inputs(6, 32, 200, torch.float32, True)
+    t = torch.tensor([3, 3, 3, 3, 3, 3], device="cuda")
+    x[1, 0] = float("nan")
+    x[2, 0] = float("inf")               # logits of both signs: NaN
+    b[7] = float("-inf")
+    loss = ops.linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    want = F.cross_entropy(x @ w.t() + b, t, reduction="none")
+    assert torch.equal(torch.isnan(loss), torch.isnan(want))
+    t[4] = 7                             # a target that cannot be
+    loss = ops.linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    assert loss[4] == float("inf") and torch.isfinite(loss[[0, 3, 5]]).all()
+    b[:] = float("-inf")
+    loss = ops.linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    assert torch.isnan(loss).all()
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("bad", [300, -1, 2 ** 40, -2 ** 40])
+def test_target_outside_the_vocabulary(bad):
+    x, w, b, t = inputs(20, 64, 300, torch.bfloat16, True)
+    t[5] = bad
+    loss = ops.linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    assert torch.isnan(loss[5])
+    assert torch.isfinite(loss[torch.arange(20) != 5]).all()
+    total, grads = run(x, w, b, t)
+    assert torch.isnan(total) and torch.isnan(grads[0][5]).all()
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_layouts():
+    """Strided, offset, transposed and expanded operands; int32 targets."""
+    dtype = torch.bfloat16
+    x, w, b, t = inputs(60, 72, 500, dtype, True, 0.1, 6)
+    want = run(x, w, b, t)
+    big = torch.zeros(60, 200, device="cuda", dtype=dtype)
+    big[:, 3:75] = x
+    wt = w.t().contiguous().t()
+    off = torch.zeros(500 * 72 + 3, device="cuda", dtype=dtype)[3:]
+    off = off.view(500, 72).copy_(w)
+    pad = torch.full((500, 90), float("nan"), device="cuda", dtype=dtype)
+    pad[:, :72] = w
+    half = torch.zeros(1000, device="cuda", dtype=dtype)[::2].copy_(b)
+    for xx in (big[:, 3:75], x.t().contiguous().t()):
+        for ww in (wt, off, pad[:, :72]):
+            got = run(xx, ww, half, t.int())
+            assert torch.equal(got[0], want[0])
+            for a, c in zip(got[1], want[1]):
+                assert torch.equal(a, c)
+    row = x[:1].expand(60, 72)
+    got = run(row, w, b, t)
+    ref = run(row.contiguous(), w, b, t)
+    assert torch.equal(got[0], ref[0])
+    cube = x.view(5, 12, 72)
+    one = ops.linear_cross_entropy(cube, w, t.view(5, 12), bias=b,
+                                   reduction="none")
+    two = ops.linear_cross_entropy(x, w, t, bias=b, reduction="none")
+    assert one.shape == (5, 12) and torch.equal(one.view(-1), two)
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_which_gradients():
+    x, w, b, t = inputs(40, 64, 300, torch.bfloat16, True, 0.1, 8)
+    full = run(x, w, b, t)[1]
+    for k in range(3):
+        leaves = [a.clone() for a in (x, w, b)]
+        leaves[k].requires_grad_()
+        loss = ops.linear_cross_entropy(leaves[0], leaves[1], t,
+                                        bias=leaves[2])
+        got, = torch.autograd.grad(loss, [leaves[k]])
+        assert torch.equal(got, full[k])
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_gradient_against_differences():
+    x, w, b, t = inputs(12, 16, 40, torch.float32, True, 0.2, 2)
+    _, grads = run(x, w, b, t, 0.1, "sum")
+    g = torch.Generator().manual_seed(1)
+    for k, a in enumerate((x, w, b)):
+        step = torch.randn(a.shape, generator=g).double()
+        args = [v.double().cpu() for v in (x, w, b)]
+        side = []
+        for s in (1e-4, -1e-4):
+            moved = list(args)
+            moved[k] = args[k] + s * step
+            z = moved[0] @ moved[1].t() + moved[2]
+            side.append(F.cross_entropy(z, t.cpu(), ignore_index=IGNORE,
+                                        label_smoothing=0.1,
+                                        reduction="sum"))
+        slope = (side[0] - side[1]) / 2e-4
+        got = (grads[k].double().cpu() * step).sum()
+        # third derivatives of a log-sum-exp are at most about |x|^3 <= 1e3
+        # along the step: 1e-8 / 6 of that; fp32 sums: 1e-5 of the terms
+        bound = 1e-5 + 1e-5 * (grads[k].double().cpu() * step).abs().sum()
+        assert abs(got - slope) <= bound
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_autocast_and_shared_weight():
+    """bf16 under autocast; one weight as embedding and as projection."""
+    torch.manual_seed(0)
+    emb = torch.nn.Embedding(90, 32, device="cuda")
+    t = torch.randint(90, (3, 7), device="cuda")
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        loss = ops.linear_cross_entropy(emb(t), emb.weight, t)
+    assert loss.dtype == torch.float32
+    loss.backward()
+    wide = emb.weight.detach().bfloat16()
+    x = wide[t.reshape(-1)]
+    ref = formula(x, wide, None, t.reshape(-1), 0.0, torch.full((21,), 1 / 21))
+    want = ref["dw"].index_add(0, t.reshape(-1).cpu(), ref["dx"])
+    bound = 2.0 ** -6 * (ref["sw"] + ref["dw"].abs()).index_add(
+        0, t.reshape(-1).cpu(), ref["sx"] + ref["dx"].abs()) + 1e-6
+    check("shared", emb.weight.grad, want, bound)
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_repeats_streams_and_graph():
+    """The same bits every time: again, on another stream, and replayed."""
+    x, w, b, t = inputs(300, 64, 1100, torch.bfloat16, True, 0.2, 11)
+    want = run(x, w, b, t, 0.1)
+    again = run(x, w, b, t, 0.1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = run(x, w, b, t, 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    sx, st = torch.zeros_like(x), torch.zeros_like(t)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(sx, w, b, st, 0.1)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        kept = run(sx, w, b, st, 0.1)
+    second = inputs(300, 64, 1100, torch.bfloat16, True, 0.5, 12)
+    for xx, tt in ((x, t), (second[0], second[3]), (x, t)):
+        sx.copy_(xx)
+        st.copy_(tt)
+        graph.replay()
+        torch.cuda.synchronize()
+        eager = run(xx, w, b, tt, 0.1)
+        for a, c in zip((kept[0], *kept[1]), (eager[0], *eager[1])):
+            assert torch.equal(a, c)
+    for got in (again, other):
+        for a, c in zip((got[0], *got[1]), (want[0], *want[1])):
+            assert torch.equal(a, c)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(
+    "cuda", marks=[pytest.mark.gpu, needs_gpu])])
+def test_refusals(device):
+    x, w, b, t = inputs(6, 16, 20, torch.float32, True, device=device)
+    call = ops.linear_cross_entropy
+    for args, kw in [
+            ((x, w, t), {"reduction": "avg"}),
+            ((x, w, t), {"label_smoothing": 1.5}),
+            ((x, w[:, :8], t), {}), ((x, w[0], t), {}),
+            ((x, w, t[:3]), {}), ((x, w, t), {"bias": b[:3]}),
+            ((x, w[:0], t), {})]:
+        with pytest.raises(ValueError):
+            call(*args, **kw)
+    with pytest.raises(TypeError):
+        call(x, w, t.float())
+    with pytest.raises(TypeError):
+        call(x, w.bfloat16(), t)
+    with pytest.raises(TypeError):
+        call(x, w, t, bias=b.bfloat16())
+    if device == "cuda":
+        with pytest.raises(ValueError):
+            call(x, w.cpu(), t)
+        with pytest.raises(TypeError):
+            call(x.double(), w.double(), t)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(
+    "cuda", marks=[pytest.mark.gpu, needs_gpu])])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_no_rows_at_all(device, reduction):
+    x = torch.empty(0, 16, device=device, requires_grad=True)
+    w = torch.randn(20, 16, device=device, requires_grad=True)
+    t = torch.empty(0, dtype=torch.int64, device=device)
+    loss = ops.linear_cross_entropy(x, w, t, reduction=reduction)
+    want = F.cross_entropy(x @ w.t(), t, reduction=reduction)
+    assert loss.shape == want.shape
+    assert torch.equal(torch.isnan(loss), torch.isnan(want))
+    if reduction != "mean":
+        loss.sum().backward()
+        assert not w.grad.any()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("eps", [0.0, 0.1])
+def test_cpu(reduction, eps):
+    x, w, b, t = inputs(30, 24, 70, torch.float32, True, 0.3, 1, "cpu")
+    up = torch.rand(30) if reduction == "none" else None
+    loss, grads = run(x, w, b, t, eps, reduction, up)
+    kept = int((t != IGNORE).sum())
+    each = up if up is not None else torch.full(
+        (30,), 1.0 / kept if reduction == "mean" else 1.0)
+    ref = formula(x, w, b, t, eps, each)
+    check_all(ref, loss if reduction == "none" else None, grads, x, w, b,
+              torch.float32, 30)
+    with pytest.raises(IndexError):
+        ops.linear_cross_entropy(x, w, torch.full_like(t, 70))
