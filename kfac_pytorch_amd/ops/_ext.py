@@ -187,3 +187,15 @@ def vocab_loss_backward(up, hidden, weight, bias, lse, ints, eps: float,
                                        eps, reduction == "none",
                                        reduction == "mean", need_x, need_w,
                                        need_b)
+
+
+# -- one norm or inner product over many tensors ------------------------------
+def grad_norm(tensors, out, max_norm: float, kind: int) -> torch.Tensor:
+    """[norm, factor], fp32 on the GPU; ``out`` (a list, or None) gets the
+    tensors times the factor.  kind: 0 for p = 2, 1 for p = 1, 2 for inf."""
+    return _load().grad_norm(tensors, out, float(max_norm), kind)
+
+
+def trust_region(updates, grads, out, lr: float, kl: float) -> torch.Tensor:
+    """nu, fp32 on the GPU; ``out`` gets the updates times nu."""
+    return _load().trust_region(updates, grads, out, float(lr), float(kl))

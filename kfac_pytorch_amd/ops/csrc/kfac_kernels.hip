@@ -434,6 +434,15 @@ std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> vocab_loss_backward(
     std::optional<torch::Tensor> bias, torch::Tensor lse, torch::Tensor ints,
     double eps, bool each, bool mean, bool need_x, bool need_w, bool need_b);
 
+// defined in grad_scale.hip
+torch::Tensor grad_norm(std::vector<torch::Tensor> tensors,
+                        std::optional<std::vector<torch::Tensor>> out,
+                        double max_norm, int64_t kind);
+torch::Tensor trust_region(std::vector<torch::Tensor> updates,
+                           std::vector<torch::Tensor> grads,
+                           std::vector<torch::Tensor> out, double lr,
+                           double kl);
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "MI355X-native HIP kernels for distributed K-FAC";
   m.def("eigen_scale_", &eigen_scale_entry,
@@ -451,4 +460,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "cross entropy of a vocabulary projection, no logits in memory");
   m.def("vocab_loss_backward", &vocab_loss_backward,
         "gradients of vocab_loss_forward");
+  m.def("grad_norm", &grad_norm,
+        "norm over many tensors, and their rescale by it");
+  m.def("trust_region", &trust_region,
+        "inner product over many tensors, and the updates' rescale by it");
 }

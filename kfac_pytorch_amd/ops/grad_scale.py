@@ -1,0 +1,195 @@
+"""Rescaling a whole model's gradients by one number that they give.
+
+* ``global_norm`` / ``clip_by_global_norm`` / ``clip_grad_norm_``: the norm
+  over all tensors and clipping by it, as ``torch.nn.utils.clip_grad_norm_``.
+* ``kl_clip``: K-FAC's trust region,
+  ``nu = min(1, sqrt(kl_clip / |lr^2 sum_i <update_i, grad_i>|))``
+  (reference: kfac/kfac_preconditioner_inv.py:188-217).
+
+On the GPU two passes over the data, a few launches whatever the number of
+tensors (``csrc/grad_scale.hip``), and no wait for the device: norms and
+factors stay there.  On the CPU the plain expressions run.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
+
+import torch
+
+__all__ = ["global_norm", "clip_by_global_norm", "clip_grad_norm_",
+           "kl_clip"]
+
+_KINDS = {2.0: 0, 1.0: 1, math.inf: 2}
+_TYPES = (torch.float32, torch.bfloat16, torch.float16)
+Tensors = Union[torch.Tensor, Iterable[torch.Tensor]]
+
+
+def _as_list(tensors: Tensors) -> List[torch.Tensor]:
+    if isinstance(tensors, torch.Tensor):
+        return [tensors]
+    return list(tensors)
+
+
+def _check_lists(name: str, *lists: Sequence[torch.Tensor]) -> None:
+    first = lists[0]
+    for other in lists[1:]:
+        if len(other) != len(first):
+            raise ValueError(f"{name}: lists of {len(first)} and "
+                             f"{len(other)} tensors")
+        for a, b in zip(first, other):
+            if a.shape != b.shape:
+                raise ValueError(f"{name}: shapes {tuple(a.shape)} and "
+                                 f"{tuple(b.shape)} differ")
+    device = first[0].device
+    for group in lists:
+        for t in group:
+            if t.device != device:
+                raise ValueError(f"{name}: tensors on {device} and "
+                                 f"{t.device}")
+            if not t.dtype.is_floating_point or t.layout != torch.strided:
+                raise TypeError(f"{name}: dense floating tensors expected, "
+                                f"got {t.dtype}, {t.layout}")
+            if t.is_cuda and t.dtype not in _TYPES:
+                raise TypeError(f"{name}: fp32, bf16 or fp16 expected on the "
+                                f"GPU, got {t.dtype}")
+
+
+def _check_outputs(name: str, out: Sequence[torch.Tensor]) -> None:
+    """Each output is written by its own workgroups: none may be there
+    twice."""
+    seen = [t.data_ptr() for t in out if t.numel()]
+    if len(set(seen)) != len(seen):
+        raise ValueError(f"{name}: the same tensor is to be written twice")
+
+
+def _kind(name: str, norm_type: float) -> int:
+    try:
+        return _KINDS[float(norm_type)]
+    except KeyError:
+        raise ValueError(f"{name}: norm_type must be 1, 2 or inf, got "
+                         f"{norm_type}") from None
+
+
+def _cpu_norm(tensors, norm_type: float) -> torch.Tensor:
+    parts = [torch.linalg.vector_norm(t.detach().double(), norm_type)
+             for t in tensors if t.numel()]
+    if not parts:
+        return torch.zeros(())
+    return torch.linalg.vector_norm(torch.stack(parts), norm_type).float()
+
+
+@torch.no_grad()
+def global_norm(tensors: Tensors, norm_type: float = 2.0) -> torch.Tensor:
+    """``(sum |t|^p)^(1/p)`` over all values of all tensors; p = 1, 2 or inf.
+
+    fp32, a scalar on the tensors' device (0 on the CPU for no tensors).
+    Sums are in double, so no square overflows or vanishes.
+    """
+    tensors = _as_list(tensors)
+    kind = _kind("global_norm", norm_type)
+    if not tensors:
+        return torch.zeros(())
+    _check_lists("global_norm", tensors)
+    if not tensors[0].is_cuda:
+        return _cpu_norm(tensors, float(norm_type))
+    from kfac_pytorch_amd.ops import _ext
+    return _ext.grad_norm(tensors, None, math.inf, kind)[0]
+
+
+@torch.no_grad()
+def clip_by_global_norm(
+        tensors: Tensors, max_norm: float, norm_type: float = 2.0,
+        out: Optional[Sequence[torch.Tensor]] = None,
+) -> Tuple[List[torch.Tensor], torch.Tensor]:
+    """The tensors times ``min(1, max_norm / (norm + 1e-6))``, and the norm.
+
+    ``out``: tensors to write, of the same shapes (any of the types); the
+    inputs themselves clip in place, and are then left untouched where the
+    factor is 1.  New tensors by default.  A norm that is not finite gives
+    what the expression gives (0 or NaN times the values).
+    """
+    tensors = _as_list(tensors)
+    kind = _kind("clip_by_global_norm", norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"clip_by_global_norm: max_norm must not be "
+                         f"negative, got {max_norm}")
+    if out is None:
+        out = [torch.empty_like(t) for t in tensors]
+    out = _as_list(out)
+    if not tensors:
+        if out:
+            raise ValueError("clip_by_global_norm: out without tensors")
+        return out, torch.zeros(())
+    _check_lists("clip_by_global_norm", tensors, out)
+    _check_outputs("clip_by_global_norm", out)
+    if not tensors[0].is_cuda:
+        norm = _cpu_norm(tensors, float(norm_type))
+        factor = (max_norm / (norm.double() + 1e-6)).clamp(max=1.0).float()
+        for t, o in zip(tensors, out):
+            o.copy_(t * factor.to(t.dtype) if t.dtype == torch.float64
+                    else t.float() * factor)
+        return out, norm
+    from kfac_pytorch_amd.ops import _ext
+    return out, _ext.grad_norm(tensors, out, max_norm, kind)[0]
+
+
+def clip_grad_norm_(parameters: Tensors, max_norm: float,
+                    norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False) -> torch.Tensor:
+    """Clip the gradients of ``parameters`` in place; returns their norm.
+
+    ``torch.nn.utils.clip_grad_norm_`` for one device, with an fp32 norm and
+    without a wait for the device (``error_if_nonfinite`` does wait, and
+    raises before anything is written).
+    """
+    # a parameter given twice counts once
+    grads = list({id(p): p.grad for p in _as_list(parameters)
+                  if p.grad is not None}.values())
+    if error_if_nonfinite:
+        norm = global_norm(grads, norm_type)
+        if not math.isfinite(float(norm)):
+            raise RuntimeError(f"clip_grad_norm_: the gradients' norm is "
+                               f"{float(norm)}")
+    return clip_by_global_norm([g.detach() for g in grads], max_norm,
+                               norm_type, out=[g.detach() for g in grads])[1]
+
+
+@torch.no_grad()
+def kl_clip(updates: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], *,
+            lr: float, kl_clip: float,
+            out: Optional[Sequence[torch.Tensor]] = None,
+            ) -> Tuple[List[torch.Tensor], torch.Tensor]:
+    """The updates times ``nu = min(1, sqrt(kl_clip / |lr^2 <u, g>|))``.
+
+    ``<u, g>`` is the inner product over all tensors, summed in double.
+    ``out``: tensors to write, of the same shapes (any of the types), which
+    may be the updates or the gradients themselves.  New tensors like the
+    gradients by default.  Returns them and nu (fp32, on the device).
+    """
+    updates, grads = _as_list(updates), _as_list(grads)
+    lr, kl = float(lr), float(kl_clip)
+    if not kl > 0:
+        raise ValueError(f"kl_clip: kl_clip must be positive, got {kl}")
+    if out is None:
+        out = [torch.empty_like(g) for g in grads]
+    out = _as_list(out)
+    if not updates:
+        if grads or out:
+            raise ValueError("kl_clip: gradients without updates")
+        return out, torch.ones(())
+    _check_lists("kl_clip", updates, grads, out)
+    _check_outputs("kl_clip", out)
+    if not updates[0].is_cuda:
+        total = sum((u.double() * g.double()).sum()
+                    for u, g in zip(updates, grads)) * lr ** 2
+        nu = (kl / total.abs().clamp_min(1e-30)).sqrt().clamp(max=1.0)
+        nu = nu.float()
+        for u, o in zip(updates, out):
+            o.copy_(u * nu.to(u.dtype) if u.dtype == torch.float64
+                    else u.float() * nu)
+        return out, nu
+    from kfac_pytorch_amd.ops import _ext
+    return out, _ext.trust_region(updates, grads, out, lr, kl)
