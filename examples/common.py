@@ -26,6 +26,8 @@ REPO_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 if REPO_ROOT not in sys.path:
     sys.path.insert(0, REPO_ROOT)
 
+from kfac_pytorch_amd.ops import clip_grad_norm_  # noqa: E402
+
 logger = logging.getLogger("kfac_examples")
 
 
@@ -38,6 +40,9 @@ def add_common_args(p: argparse.ArgumentParser):
     g.add_argument("--base-lr", type=float, default=0.1)
     g.add_argument("--momentum", type=float, default=0.9)
     g.add_argument("--weight-decay", type=float, default=5e-4)
+    g.add_argument("--clip-grad", type=float, default=0.0,
+                   help="clip the gradients' global norm before the "
+                        "preconditioner (0: off)")
     g.add_argument("--warmup-epochs", type=float, default=5)
     g.add_argument("--lr-decay", type=int, nargs="*", default=[35, 75, 90])
     g.add_argument("--checkpoint-format", default=None,
@@ -145,6 +150,8 @@ def train_loop(model, ddp_model, optimizer, preconditioner, criterion,
         else:
             loss = criterion(ddp_model(data), target)
         loss.backward()  # DDP allreduce overlaps here (COMM phase)
+        if args.clip_grad:
+            clip_grad_norm_(model.parameters(), args.clip_grad)
         timers.stop()
 
         if preconditioner is not None:

@@ -84,6 +84,8 @@ def main():
                 loss = (F.cross_entropy(s_logits, starts) +
                         F.cross_entropy(e_logits, ends)) / 2
             loss.backward()
+            if args.clip_grad:
+                common.clip_grad_norm_(model.parameters(), args.clip_grad)
             if precond is not None:
                 precond.step()
             optimizer.step()

@@ -90,6 +90,8 @@ def main():
                     else:
                         loss = F.cross_entropy(ddp_model(x), y)
                     (loss / args.batches_per_allreduce).backward()
+            if args.clip_grad:
+                common.clip_grad_norm_(model.parameters(), args.clip_grad)
             if precond is not None:
                 precond.step()
             optimizer.step()

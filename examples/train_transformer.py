@@ -25,6 +25,9 @@ def main():
     p.add_argument("--layers", type=int, default=6)
     p.add_argument("--optimizer", default="sgd", choices=["sgd", "adam"])
     p.add_argument("--label-smoothing", type=float, default=0.1)
+    p.add_argument("--fused-loss", action="store_true",
+                   help="loss from the generator's weights without the "
+                        "logits in memory")
     common.add_common_args(p)
     p.set_defaults(batch_size=128, base_lr=0.1, damping=0.003)
     args = p.parse_args()
@@ -84,9 +87,13 @@ def main():
             out.append((src, trg))
         return out
 
-    def criterion(logits, trg_out):
+    def loss_of(src, trg):
+        if args.fused_loss:
+            return ddp_model(src, trg[:, :-1], targets=trg[:, 1:],
+                             smoothing=args.label_smoothing)
+        logits = ddp_model(src, trg[:, :-1])
         return crit(logits.reshape(-1, args.vocab_size),
-                    trg_out.reshape(-1))
+                    trg[:, 1:].reshape(-1))
 
     import time
     for epoch in range(args.epochs):
@@ -98,12 +105,12 @@ def main():
             optimizer.zero_grad(set_to_none=False)
             if args.dtype == "bf16" and use_cuda:
                 with torch.autocast("cuda", dtype=torch.bfloat16):
-                    logits = ddp_model(src, trg[:, :-1])
-                    loss = criterion(logits, trg[:, 1:])
+                    loss = loss_of(src, trg)
             else:
-                logits = ddp_model(src, trg[:, :-1])
-                loss = criterion(logits, trg[:, 1:])
+                loss = loss_of(src, trg)
             loss.backward()
+            if args.clip_grad:
+                common.clip_grad_norm_(model.parameters(), args.clip_grad)
             if precond is not None:
                 precond.step()
             optimizer.step()

@@ -50,6 +50,9 @@ def parse_args():
                         "vocab projections too)")
     p.add_argument("--include-vocab", dest="exclude_vocab",
                    action="store_false")
+    p.add_argument("--fused-loss", action="store_true",
+                   help="loss from the decoder's weights without the logits "
+                        "in memory (needs --exclude-vocab with K-FAC)")
     p.set_defaults(batch_size=20, base_lr=20.0 / 20, damping=0.003)
     return p.parse_args()
 
@@ -116,9 +119,19 @@ def main():
             logits = out[0] if isinstance(out, tuple) else out
             return self.ce(logits.reshape(-1, vocab), target.reshape(-1))
 
+    criterion = LMLoss()
+    forward = ddp
+    if args.fused_loss:
+        # the model takes the targets and returns its loss
+        def forward(batch):
+            return ddp(batch[0], targets=batch[1])
+
+        def criterion(out, target):
+            return out[0]
+
     for epoch in range(args.epochs):
         loss, iter_times = train_loop(
-            model, ddp, optimizer, pre, LMLoss(),
+            model, forward, optimizer, pre, criterion,
             TokenBatches(args.iters_per_epoch), args, rank, use_cuda)
         if rank == 0 and not args.speed:
             print(f"epoch {epoch}: loss={loss:.4f}")

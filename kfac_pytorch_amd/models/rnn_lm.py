@@ -11,6 +11,8 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
+from kfac_pytorch_amd.ops.vocab_loss import projection_loss
+
 __all__ = ["LSTMLanguageModel"]
 
 
@@ -29,7 +31,13 @@ class LSTMLanguageModel(nn.Module):
             self.decoder.weight = self.embed.weight
         self.vocab_size = vocab_size
 
-    def forward(self, x, hidden=None):
+    def forward(self, x, hidden=None, targets=None):
+        """Logits and the LSTM's state; with ``targets`` (token numbers, the
+        shape of ``x``) the mean cross entropy instead of the logits, which
+        are then never in memory (``ops.linear_cross_entropy``)."""
         emb = self.drop(self.embed(x))
         out, hidden = self.lstm(emb, hidden)
-        return self.decoder(self.drop(out)), hidden
+        out = self.drop(out)
+        if targets is not None:
+            return projection_loss(self.decoder, out, targets), hidden
+        return self.decoder(out), hidden

@@ -18,6 +18,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from kfac_pytorch_amd.ops.vocab_loss import projection_loss
+
 __all__ = ["Seq2SeqTransformer", "make_transformer"]
 
 
@@ -60,7 +62,12 @@ class Seq2SeqTransformer(nn.Module):
 
     def forward(self, src: torch.Tensor, trg: torch.Tensor,
                 src_pad_mask: Optional[torch.Tensor] = None,
-                trg_pad_mask: Optional[torch.Tensor] = None):
+                trg_pad_mask: Optional[torch.Tensor] = None,
+                targets: Optional[torch.Tensor] = None,
+                smoothing: float = 0.0, ignore_index: int = -100):
+        """Logits; with ``targets`` (token numbers, the shape of ``trg``)
+        the mean loss instead, without the logits in memory.  ``smoothing``
+        is ``utils.LabelSmoothLoss``'s (spread over the other tokens)."""
         causal = nn.Transformer.generate_square_subsequent_mask(
             trg.size(1), device=trg.device)
         h = self.transformer(
@@ -69,6 +76,13 @@ class Seq2SeqTransformer(nn.Module):
             tgt_mask=causal,
             src_key_padding_mask=src_pad_mask,
             tgt_key_padding_mask=trg_pad_mask)
+        if targets is not None:
+            # spread over the V - 1 others: s / (V - 1) for each is eps / V
+            v = self.trg_vocab
+            eps = smoothing * v / (v - 1.0) if smoothing else 0.0
+            return projection_loss(self.generator, h, targets,
+                                   ignore_index=ignore_index,
+                                   label_smoothing=eps)
         return self.generator(h)
 
     @torch.no_grad()

@@ -23,7 +23,7 @@ from typing import Optional
 import torch
 import torch.nn.functional as F
 
-__all__ = ["linear_cross_entropy"]
+__all__ = ["linear_cross_entropy", "projection_loss"]
 
 _REDUCTIONS = ("mean", "sum", "none")
 _TYPES = (torch.bfloat16, torch.float16, torch.float32)
@@ -157,3 +157,22 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
             float(label_smoothing), reduction)
         loss = loss if reduction == "none" else total
     return loss.view(target.shape) if reduction == "none" else loss
+
+
+def projection_loss(layer: torch.nn.Linear, hidden: torch.Tensor,
+                    target: torch.Tensor, **kw) -> torch.Tensor:
+    """``linear_cross_entropy`` with an output layer's weight and bias.
+
+    The layer itself is not called, so nothing that hangs on its calls may
+    be left waiting: a layer with hooks (K-FAC's, of a preconditioner that
+    does not leave the vocabulary projection out) is refused.
+    """
+    if (layer._forward_pre_hooks or layer._forward_hooks
+            or layer._backward_hooks or layer._backward_pre_hooks):
+        raise RuntimeError(
+            "the vocabulary projection carries hooks, which a loss without "
+            "logits does not run; leave the layer out of K-FAC "
+            f"(exclude_vocabulary_size={layer.out_features}) or take the "
+            "loss from the logits")
+    return linear_cross_entropy(hidden, layer.weight, target,
+                                bias=layer.bias, **kw)

@@ -510,21 +510,30 @@ class KFACBase(optim.Optimizer):
         """Copy preconditioned grads into .grad and apply the kl-clip
         rescale nu = min(1, sqrt(kl_clip/|sum(v*g*lr^2)|))
         (reference: kfac/kfac_preconditioner_inv.py:188-217) with no
-        host-device sync: vg_sum stays a device scalar."""
+        host-device sync: nu stays a device scalar.  On the GPU two passes
+        over all layers at once (ops.kl_clip); otherwise layer by layer."""
         use_clip = self.kl_clip is not None
-        vg_sum = None
         grads: List[torch.Tensor] = []
+        updates: List[torch.Tensor] = []
         for module in self.modules:
-            v = self._reshape_preconditioned_grad(
-                module, self.m_precon_grad[module])
             params = [module.weight] + (
                 [module.bias] if module.bias is not None else [])
-            for p, vi in zip(params, v):
-                if use_clip:
-                    contrib = (vi * p.grad.data).sum() * (self.lr ** 2)
-                    vg_sum = contrib if vg_sum is None else vg_sum + contrib
-                p.grad.data.copy_(vi)
-                grads.append(p.grad.data)
+            grads += [p.grad.data for p in params]
+            updates += self._reshape_preconditioned_grad(
+                module, self.m_precon_grad[module])
+        if (use_clip and grads and not self.exclude_communicate_inverse
+                and self._one_pass_update(grads, updates)):
+            from kfac_pytorch_amd.ops.grad_scale import kl_clip
+            kl_clip(updates, grads, lr=self.lr, kl_clip=self.kl_clip,
+                    out=grads)
+            return
+
+        vg_sum = None
+        for g, v in zip(grads, updates):
+            if use_clip:
+                contrib = (v * g).sum() * (self.lr ** 2)
+                vg_sum = contrib if vg_sum is None else vg_sum + contrib
+            g.copy_(v)
 
         if use_clip and vg_sum is not None:
             if self.exclude_communicate_inverse:
@@ -533,6 +542,18 @@ class KFACBase(optim.Optimizer):
                 (self.kl_clip / vg_sum.abs().clamp_min(1e-30)).sqrt(),
                 max=1.0)
             torch._foreach_mul_(grads, nu)
+
+    @staticmethod
+    def _one_pass_update(grads, updates) -> bool:
+        """Whether the many-tensor kernels take the update: all of it on one
+        GPU in fp32, and no gradient there twice (two hooked layers that
+        share a weight are updated one after the other)."""
+        device = grads[0].device
+        return (device.type == "cuda"
+                and all(t.device == device and t.dtype == torch.float32
+                        and t.layout == torch.strided
+                        for t in grads + updates)
+                and len({g.data_ptr() for g in grads}) == len(grads))
 
     # ------------------------------------------------------------------ step
     def _phase(self, name: str):
