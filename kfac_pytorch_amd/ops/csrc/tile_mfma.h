@@ -38,11 +38,39 @@ using lds_s16x4 = __attribute__((address_space(3))) s16x4;
 constexpr uint32_t OUT_OF_RANGE = 0x7ffffff0u;
 constexpr long MAX_RECORDS = 0x7fffff00l;
 
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p,
-                                                           long bytes) {
+// A raw buffer of `bytes` bytes from p on.
+using Rsrc = __attribute__((ext_vector_type(4))) int;
+__device__ __forceinline__ Rsrc make_rsrc(const void* p, long bytes) {
   const long n = bytes < 0 ? 0 : (bytes > MAX_RECORDS ? MAX_RECORDS : bytes);
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)n,
-                                           0x00020000);
+  const uint64_t at = reinterpret_cast<uint64_t>(p);
+  return Rsrc{(int)(uint32_t)at, (int)(uint32_t)(at >> 32) & 0xffff, (int)n,
+              0x00020000};
+}
+
+// Starts a load of 16 bytes a lane from buffer r at offset off + uniform,
+// straight to LDS at `to` + 16 * lane.  Written as assembly because the
+// compiler takes the builtin's write to LDS for an alias of every later LDS
+// read and waits for it there; what orders the two here are the explicit wait
+// and the barrier in product().  It has no register to return.
+__device__ __forceinline__ void load_to_lds(Rsrc r, char* to, uint32_t off,
+                                            uint32_t uniform) {
+  const uint32_t at = (uint32_t)(uintptr_t)(lds_void*)to;
+  asm volatile(
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, %3 offen lds"
+      :
+      : "s"(at), "v"(off), "s"(r), "s"(uniform)
+      : "m0", "memory");
+}
+
+// all loads to LDS of this wave have arrived, all its LDS reads too, and the
+// other waves are as far
+__device__ __forceinline__ void arrive() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+  __builtin_amdgcn_sched_barrier(0);
 }
 
 // one 16-byte fragment piece: 8 values of 16 bits, or 4 of 32
@@ -82,6 +110,23 @@ __device__ __forceinline__ f32x4 mma<float>(const Frag& a, const Frag& b,
   return c;
 }
 
+template <class T>
+constexpr int MMAS = sizeof(T) == 2 ? 1 : 4;  // instructions of one mma()
+
+// Asks the scheduler to start with a matrix instruction (its operands have
+// been read long before) and to put the LDS reads singly between the next
+// ones, so that the last has arrived when the block ends.
+template <int MATRIX, int READS>
+__device__ __forceinline__ void spread() {
+  constexpr int EACH = MATRIX / 4 * 3 / READS > 0 ? MATRIX / 4 * 3 / READS : 1;
+#pragma unroll
+  for (int i = 0; i < READS; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);  // matrix
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);     // LDS read
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, MATRIX, 0);
+}
+
 // A tile shape: BM x BN of C by WM x WN waves.
 template <int BM_, int BN_, int WM_, int WN_>
 struct Shape {
@@ -100,6 +145,7 @@ struct Operand {
   static constexpr int BYTES = R * 128;
   static constexpr int LOADS = R / 8 / NW;
   static constexpr int NC = R * SZ / 16;  // chunks of a k-outer row
+  static constexpr int READS = KOUTER ? (SZ == 2 ? 2 : 4) : 1;  // a fragment
   static_assert(R % (8 * NW) == 0, "whole loads for every wave");
 
   const char* base;
@@ -107,6 +153,9 @@ struct Operand {
   uint32_t off[LOADS];
   int extent;  // rows of the operand from this tile's first on
   int kend;
+  const char* at;  // k-outer: where the next slice starts, and
+  long left;       // the bytes from there on
+  Rsrc rsrc;
 
   __device__ __forceinline__ void init(const T* p, long ld, int r0, int rows,
                                        int kend_, int wave, int lane) {
@@ -141,31 +190,37 @@ struct Operand {
     }
   }
 
-  // start the loads of the slice at k0 into `lds`
-  __device__ __forceinline__ void load(char* lds, int k0, int wave,
-                                       int lane) const {
+  // Which buffer the next slice is loaded from: a k-outer operand's starts at
+  // that slice's first row, so offsets within it stay small.
+  __device__ __forceinline__ void start(int kbeg) {
     if constexpr (KOUTER) {
-      const __amdgpu_buffer_rsrc_t r =
-          make_rsrc(base + (long)k0 * ld_bytes,
-                    (long)(kend - k0 - 1) * ld_bytes + (long)extent * SZ);
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            r, (lds_void*)(lds + (j * NW + wave) * 1024), 16, off[j], 0, 0,
-            0);
-      }
+      at = base + (long)kbeg * ld_bytes;
+      left = (long)(kend - kbeg - 1) * ld_bytes + (long)extent * SZ;
+      rsrc = make_rsrc(at, left);
     } else {
       const int rows = extent < R ? extent : R;
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(
-          base, (long)(rows - 1) * ld_bytes + (long)kend * SZ);
+      rsrc = make_rsrc(base, (long)(rows - 1) * ld_bytes + (long)kend * SZ);
+    }
+  }
+
+  __device__ __forceinline__ void next() {
+    if constexpr (KOUTER) {
+      at += BK * ld_bytes;
+      left -= BK * ld_bytes;
+      rsrc = make_rsrc(at, left);
+    }
+  }
+
+  // start load j of the slice at k0 into `lds`
+  __device__ __forceinline__ void load(char* lds, int k0, int j, int wave,
+                                       int lane) const {
+    char* to = lds + (j * NW + wave) * 1024;
+    if constexpr (KOUTER) {
+      load_to_lds(rsrc, to, off[j], 0);
+    } else {
       const int c = (lane & 7) ^ (lane >> 3);
-      const bool past = k0 + c * E >= kend;
-#pragma unroll
-      for (int j = 0; j < LOADS; ++j) {
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(
-            r, (lds_void*)(lds + (j * NW + wave) * 1024), 16,
-            past ? OUT_OF_RANGE : off[j], k0 * SZ, 0, 0);
-      }
+      load_to_lds(rsrc, to, k0 + c * E >= kend ? OUT_OF_RANGE : off[j],
+                  k0 * SZ);
     }
   }
 
@@ -197,16 +252,15 @@ struct Operand {
   }
 };
 
-// acc += the product over k in [kbeg, kend); kbeg is a multiple of BK.  A
+// acc (f32x4 [S::MI][S::NI]) += the product over k in [kbeg, kend); kbeg is a multiple of BK.  A
 // k-inner operand needs whole chunks up to kend; rows of a k-outer one from
 // `krows` on are taken for zeros.  `smem` is S::LDS bytes.  Every wave of the workgroup calls it with the same
 // arguments; on return all of them are done with smem.
-template <class T, bool KA, bool KB, class S>
+template <class T, bool KA, bool KB, class S, class Acc>
 __device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
                                         const T* B, long ldb, int n0, int N,
                                         int kbeg, int kend, int krows,
-                                        char* smem,
-                                        f32x4 (&acc)[S::MI][S::NI]) {
+                                        char* smem, Acc& acc) {
   using OA = Operand<T, KA, S::BM, S::NW>;
   using OB = Operand<T, KB, S::BN, S::NW>;
   constexpr int BK = OA::BK;
@@ -219,40 +273,70 @@ __device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
   a.init(A, lda, m0, M, KA ? krows : kend, wave, lane);
   b.init(B, ldb, n0, N, KB ? krows : kend, wave, lane);
 
+  // Two slices are in LDS or on their way there, and two halves of a slice
+  // in registers: the matrix cores work on one half while the other is read.
+  // Loads and reads past the last slice are harmless (zeros, unused), which
+  // keeps the loop free of branches.
   char* cur = smem;
   char* nxt = smem + S::LDS / 2;
-  if (kbeg < kend) {
-    a.load(cur, kbeg, wave, lane);
-    b.load(cur + OA::BYTES, kbeg, wave, lane);
-  }
-  for (int k0 = kbeg; k0 < kend; k0 += BK) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();
-    if (k0 + BK < kend) {
-      a.load(nxt, k0 + BK, wave, lane);
-      b.load(nxt + OA::BYTES, k0 + BK, wave, lane);
+  Frag fa[2][S::MI], fb[2][S::NI];
+  constexpr int FRAGS = S::MI + S::NI, LOADS = OA::LOADS + OB::LOADS;
+  // one fragment of half ks; those of B first, the first products need them
+  auto read = [&](const char* lds, int ks, int to, int i) {
+    if (i < S::NI) {
+      fb[to][i] = OB::read(lds + OA::BYTES, wn + i * 16, ks, lane);
+    } else {
+      fa[to][i - S::NI] = OA::read(lds, wm + (i - S::NI) * 16, ks, lane);
     }
+  };
+  auto multiply = [&](int from) {
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      Frag fb[S::NI];
+    for (int mi = 0; mi < S::MI; ++mi) {
 #pragma unroll
       for (int ni = 0; ni < S::NI; ++ni) {
-        fb[ni] = OB::read(cur + OA::BYTES, wn + ni * 16, ks, lane);
-      }
-#pragma unroll
-      for (int mi = 0; mi < S::MI; ++mi) {
-        const Frag fa = OA::read(cur, wm + mi * 16, ks, lane);
-#pragma unroll
-        for (int ni = 0; ni < S::NI; ++ni) {
-          acc[mi][ni] = mma<T>(fa, fb[ni], acc[mi][ni]);
-        }
+        acc[mi][ni] = mma<T>(fa[from][mi], fb[from][ni], acc[mi][ni]);
       }
     }
+  };
+  auto load = [&](char* lds, int k0, int j) {
+    if (j < OA::LOADS) {
+      a.load(lds, k0, j, wave, lane);
+    } else {
+      b.load(lds + OA::BYTES, k0, j - OA::LOADS, wave, lane);
+    }
+  };
+  a.start(kbeg);
+  b.start(kbeg);
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) load(cur, kbeg, j);
+  a.next();
+  b.next();
+  arrive();
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) load(nxt, kbeg + BK, j);
+#pragma unroll
+  for (int i = 0; i < FRAGS; ++i) read(cur, 0, 0, i);
+  for (int k0 = kbeg; k0 < kend; k0 += BK) {
+#pragma unroll
+    for (int i = 0; i < FRAGS; ++i) read(cur, 1, 1, i);
+    a.next();
+    b.next();
+    multiply(0);
+    spread<S::MI * S::NI * MMAS<T>, S::MI * OA::READS + S::NI * OB::READS>();
+    arrive();  // cur is in registers, nxt is in LDS
+    // the compiler keeps reads and loads, both of LDS, in this order
+#pragma unroll
+    for (int i = 0; i < (FRAGS > LOADS ? FRAGS : LOADS); ++i) {
+      if (i < FRAGS) read(nxt, 0, 0, i);
+      if (i < LOADS) load(cur, k0 + 2 * BK, i);
+    }
+    multiply(1);
+    spread<S::MI * S::NI * MMAS<T>, S::MI * OA::READS + S::NI * OB::READS>();
     char* t = cur;
     cur = nxt;
     nxt = t;
   }
-  __syncthreads();
+  arrive();
 }
 
 // Which tile a workgroup takes.  Workgroups go to the 8 XCDs in turn; each
