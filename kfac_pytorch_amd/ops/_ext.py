@@ -171,22 +171,29 @@ def has_jacobi_eigh(m: int) -> bool:
 
 # -- cross entropy of a vocabulary projection ---------------------------------
 def vocab_loss_forward(hidden, weight, target, bias, ignore_index: int,
-                       eps: float, reduction: str):
-    """(loss of every row, total or None, log-sum-exp of the kept rows, the
-    kept rows' numbers) -- the last two are what the backward pass needs."""
+                       eps: float, reduction: str,
+                       need=(False, False, False)):
+    """(loss of every row, total or None, state, ints, kept).  state and ints
+    are what ``vocab_loss_backward`` needs, kept what ``vocab_loss_finish``
+    does (empty: there is nothing to finish)."""
     return _load().vocab_loss_forward(hidden, weight, target, bias,
                                       ignore_index, eps, reduction == "sum",
-                                      reduction == "mean")
+                                      reduction == "mean", *need)
 
 
-def vocab_loss_backward(up, hidden, weight, bias, lse, ints, eps: float,
-                        reduction: str, need_x: bool, need_w: bool,
-                        need_b: bool):
-    """(d hidden, d weight, d bias); None for those not asked for."""
-    return _load().vocab_loss_backward(up, hidden, weight, bias, lse, ints,
+def vocab_loss_finish(up, hidden, weight, ints, kept):
+    """(d hidden, d weight, d bias) from what the forward pass kept, which is
+    used up; None for those not asked for."""
+    return _load().vocab_loss_finish(up, hidden, weight, ints, kept)
+
+
+def vocab_loss_backward(up, hidden, weight, bias, state, ints, eps: float,
+                        reduction: str, need):
+    """(d hidden, d weight, d bias), the logits made again; None for those
+    not asked for."""
+    return _load().vocab_loss_backward(up, hidden, weight, bias, state, ints,
                                        eps, reduction == "none",
-                                       reduction == "mean", need_x, need_w,
-                                       need_b)
+                                       reduction == "mean", *need)
 
 
 # -- one norm or inner product over many tensors ------------------------------

@@ -425,14 +425,20 @@ std::vector<torch::Tensor> jacobi_eigh_batched(
     std::vector<torch::Tensor> mats);
 
 // defined in vocab_loss_entry.hip
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor,
+           std::vector<std::optional<torch::Tensor>>>
 vocab_loss_forward(torch::Tensor hidden, torch::Tensor weight,
                    torch::Tensor target, std::optional<torch::Tensor> bias,
-                   int64_t ignore_index, double eps, bool sum, bool mean);
+                   int64_t ignore_index, double eps, bool sum, bool mean,
+                   bool need_x, bool need_w, bool need_b);
+std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> vocab_loss_finish(
+    torch::Tensor up, torch::Tensor hidden, torch::Tensor weight,
+    torch::Tensor ints, std::vector<std::optional<torch::Tensor>> kept);
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> vocab_loss_backward(
     torch::Tensor up, torch::Tensor hidden, torch::Tensor weight,
-    std::optional<torch::Tensor> bias, torch::Tensor lse, torch::Tensor ints,
-    double eps, bool each, bool mean, bool need_x, bool need_w, bool need_b);
+    std::optional<torch::Tensor> bias, torch::Tensor state,
+    torch::Tensor ints, double eps, bool each, bool mean, bool need_x,
+    bool need_w, bool need_b);
 
 // defined in grad_scale.hip
 torch::Tensor grad_norm(std::vector<torch::Tensor> tensors,
@@ -459,7 +465,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("vocab_loss_forward", &vocab_loss_forward,
         "cross entropy of a vocabulary projection, no logits in memory");
   m.def("vocab_loss_backward", &vocab_loss_backward,
-        "gradients of vocab_loss_forward");
+        "gradients of vocab_loss_forward, from its operands");
+  m.def("vocab_loss_finish", &vocab_loss_finish,
+        "gradients that vocab_loss_forward kept, times the upstream factor");
   m.def("grad_norm", &grad_norm,
         "norm over many tensors, and their rescale by it");
   m.def("trust_region", &trust_region,

@@ -22,36 +22,37 @@ inline void check(hipError_t e) {
 
 // How a call of given sizes is cut up.
 struct Plan {
-  bool wide;
-  int edge, tiles, row_tiles, dx_splits, dw_splits;
-  long piece;
+  bool wide;              // tiles of 256 x 256, else of 128 x 128
+  int edge, band, bands;  // of a tile; entries of a band, bands of a row
+  long piece;             // entries of the vocabulary at a time
+  int part, parts;        // tokens of a part of the bias gradient's sum
+  int dx_splits, dw_splits;
 };
 
-Plan plan(long rows, long vocab, int ldim, int size);
+// keep: the whole vocabulary's powers are kept for the gradients
+Plan plan(long rows, long vocab, int ldim, int size, bool keep);
 
-struct Forward {
+long padded(long n);  // to whole 16-byte chunks of every type
+
+struct Operands {
   Plan plan;
   const void *w, *x, *bias;
   long ldw, rows, vocab;
   int ldx;  // packed x: kept rows by ldx values, zeros past the hidden size
-  float eps;
-  const int *pos, *tgt, *count;
-  float *pmax, *psum, *pz, *ztgt, *lse, *loss;
-};
-
-struct Backward {
-  Plan plan;
-  const void *w, *x, *bias;
-  long ldw, rows, vocab, piece;
-  int ldx, dim;
+  int dim;
   float eps;
   const int *pos, *idx, *tgt, *count;
-  const float* lse;
-  const float* up;  // upstream gradient: one value, or one for each row
-  bool each, mean;
-  int dx_splits, dw_splits;
+};
+
+struct Sums {
+  float *pmax, *psum, *pz;             // [row][band]
+  float *rowm, *rowi, *ztgt, *loss;    // [row]
+};
+
+struct Grads {
   float *coef, *scale, *pbias, *dx_slabs, *dw_slabs;
   void *grad, *dx, *dw, *db;
+  int part;
 };
 
 void scan(const void* target, bool wide_ints, long rows, long ignore,
@@ -60,9 +61,19 @@ void scan(const void* target, bool wide_ints, long rows, long ignore,
 void pack(Type t, const void* in, long ld, long step, long rows, int cols,
           const int* idx, const int* count, void* out, int ldo,
           hipStream_t s);
-void forward(Type t, const Forward& f, hipStream_t s);
+// grad: where the powers go, or null
+void forward(Type t, const Operands& o, const Sums& f, void* grad,
+             hipStream_t s);
 void total(const float* loss, long rows, const int* count, bool mean,
            float* out, hipStream_t s);
-void backward(Type t, const Backward& b, hipStream_t s);
+// up: one value, one for each row (`each`), or null for 1
+void coefficients(Type t, const Operands& o, const float* up, bool each,
+                  bool mean, const Grads& b, hipStream_t s);
+void gradients_kept(Type t, const Operands& o, const Sums& f, const Grads& b,
+                    hipStream_t s);
+void finish_kept(Type t, const Operands& o, const Grads& b, const float* up,
+                 hipStream_t s);
+void gradients_again(Type t, const Operands& o, const Sums& f, const Grads& b,
+                     hipStream_t s);
 
 }  // namespace vocab_loss

@@ -7,11 +7,25 @@
 //   g[n, v]  = c_n (exp(z[n, v] - lse[n]) - (1 - eps) [v = t_n] - eps / V)
 //   dx = g w,   dw = g^T x,   db = sum_n g,    c_n = d(total) / d(loss[n])
 //
-// Forward: a workgroup makes one tile of z in registers and leaves, for each
-// of its rows n, the tile's maximum, the sum of exp(z - maximum) and (with
-// smoothed labels) the sum of z; a wave per row joins the tiles.  Backward:
-// piece by piece of the vocabulary, z is made once more, turned into g in
-// registers and written in the inputs' type, then multiplied with w and x.
+// A workgroup makes one tile of z in registers.  Of each band of its rows it
+// leaves, for every token n, a reference (the band's largest z in units of
+// log 2, rounded to a whole number, so that exp2(z log2(e) - reference) takes
+// one fused multiply-add and the reference carries no error), the sum of those
+// powers and, with smoothed labels, the sum of z; a wave per row joins them.
+//
+// Gradients, either of two ways:
+//   kept: the forward pass writes the powers themselves, in the inputs' type;
+//     once the sums are joined a pass over them makes g, and g is multiplied
+//     with w and x: 3 products in all.  They exist during the call only; what
+//     is kept for the backward pass are the gradients for an upstream factor
+//     of 1.
+//   again: the backward pass makes z once more, piece by piece of the
+//     vocabulary: 4 products, and a piece's g at a time.  For losses of single
+//     rows, whose factors come with the backward pass, and where the powers
+//     would take too much memory.
+// g is rounded to the inputs' type once (kept: twice) before the products, as
+// it would be by a layer that computes in that type.  The target's own entry
+// is always made from fp32: there p - 1 cancels.
 //
 // Rows that the loss leaves out (ignore_index) are dropped before the first
 // product: x is packed to the kept rows, so padding costs nothing and what it
@@ -29,14 +43,8 @@ using tile::f32x4;
 using tile::Shape;
 
 constexpr float LOG2E = 1.44269504088896340736f;
-constexpr float LN2 = 0.69314718055994530942f;
 
 // ------------------------------------------------------------ small helpers
-template <class T>
-__device__ __forceinline__ float to_float(T v) {
-  return (float)v;
-}
-
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll
   for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
@@ -49,11 +57,23 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
-// a maximum to subtract: -inf (nothing seen, or all of it -inf) gives 0, so
-// that exp(-inf - 0) is 0 and a NaN still shows in the sum
+// a reference to subtract: -inf (nothing seen, or all of it -inf) gives 0, so
+// that exp2(-inf - 0) is 0 and a NaN still shows in the sum
 __device__ __forceinline__ float safe(float m) {
   return m == -INFINITY ? 0.f : m;
 }
+
+// exp(z) / 2^m for a whole m
+__device__ __forceinline__ float power(float z, float m) {
+  return __builtin_amdgcn_exp2f(fmaf(z, LOG2E, -m));
+}
+
+// Powers are at most 2^0.5; fp16 gets them times 2^15, so that those down to
+// 2^-29 of the largest keep all their bits.
+template <class T>
+constexpr float LIFT = 1.f;
+template <>
+constexpr float LIFT<_Float16> = 32768.f;
 
 // ------------------------------------------------------- kept rows, one block
 // pos[n]: the row's place among the kept ones, or -1; idx, tgt: the kept rows'
@@ -130,105 +150,263 @@ __global__ void pack_kernel(const T* __restrict__ in, long ld, long step,
 // -------------------------------------------------------------- logits tiles
 // Rows of the tile are vocabulary entries, columns are tokens: a lane then
 // holds 4 neighbouring entries of one token, which it can write at once, and
-// a token's sums stay within a column.
-template <class T, class S>
-__global__ __launch_bounds__(S::THREADS) void stats_kernel(
-    const T* __restrict__ w, long ldw, const T* __restrict__ x, long ldx,
-    const T* __restrict__ bias, int vocab, int dim, const int* count, int mt,
-    int nt, const int* __restrict__ tgt, int smooth,
-    float* __restrict__ pmax, float* __restrict__ psum,
-    float* __restrict__ pz, float* __restrict__ ztgt) {
+// a token's sums stay within a column.  A wave's rows are one band.
+struct Logits {
+  long ldw;
+  int ldx, v0, vocab;  // the piece [v0, v0 + vocab) of the entries
+  int mt, nt;
+  const int *count, *tgt;
+  // sums, KEEP
+  float *pmax, *psum, *pz, *ztgt;  // [row][band]; pz null without smoothing
+  int bands;
+  // g, KEEP
+  long ldg;
+  // g
+  const float *rowm, *rowi, *coef;
+  float eps, share;
+  float* pbias;        // [tile of tokens][entry of all]
+  long all;
+};
+
+enum Mode { SUMS, KEEP, AGAIN };
+
+template <class T, class S, int MODE>
+__global__ __launch_bounds__(S::THREADS) void logits_kernel(
+    const T* __restrict__ w, const T* __restrict__ x,
+    const T* __restrict__ bias, T* __restrict__ grad, const Logits p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   int tm, tn;
-  tile::pick(blockIdx.x, mt, nt, &tm, &tn);
-  const int rows = *count;
+  tile::pick(blockIdx.x, p.mt, p.nt, &tm, &tn);
+  const int rows = *p.count;
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   if (n0 >= rows) return;
-  f32x4 acc[S::MI][S::NI] = {};
-  tile::product<T, false, false, S>(w, ldw, m0, vocab, x, ldx, n0, rows, 0,
-                                    dim, dim, smem, acc);
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i = lane & 15, g = lane >> 4;
   const int wrow = (wave / S::WN) * (S::MI * 16);
   const int wcol = (wave % S::WN) * (S::NI * 16);
-  float mx[S::NI], sm[S::NI], zs[S::NI];
+  const int vbase = m0 + wrow + g * 4;  // + 16 mi + r
+  const int nbase = n0 + wcol + i;      // + 16 ni
+
+  f32x4 acc[S::MI][S::NI];
+#pragma unroll
+  for (int mi = 0; mi < S::MI; ++mi) {
+    f32x4 b = {};
+    if (bias) {
+      const int v = vbase + mi * 16;
+      T t[4] = {};
+      if (v + 4 <= p.vocab) {
+        __builtin_memcpy(t, bias + p.v0 + v, sizeof(t));
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (v + r < p.vocab) t[r] = bias[p.v0 + v + r];
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) b[r] = (float)t[r];
+    }
+#pragma unroll
+    for (int ni = 0; ni < S::NI; ++ni) acc[mi][ni] = b;
+  }
+  tile::product<T, false, false, S>(w + (long)p.v0 * p.ldw, p.ldw, m0,
+                                    p.vocab, x, p.ldx, n0, rows, 0, p.ldx,
+                                    p.ldx, smem, acc);
+
+  // where a token's target is among this lane's entries: 16 mi + r, or none
   int t[S::NI];
 #pragma unroll
   for (int ni = 0; ni < S::NI; ++ni) {
-    const int n = n0 + wcol + ni * 16 + i;
-    t[ni] = n < rows ? tgt[n] : BAD;
-    mx[ni] = -INFINITY;
-    sm[ni] = 0.f;
-    zs[ni] = 0.f;
-  }
-#pragma unroll
-  for (int mi = 0; mi < S::MI; ++mi) {
-    const int v = m0 + wrow + mi * 16 + g * 4;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const bool in = v + r < vocab;
-      const float b = bias && in ? to_float(bias[v + r]) : 0.f;
-#pragma unroll
-      for (int ni = 0; ni < S::NI; ++ni) {
-        const float z = acc[mi][ni][r] + b;
-        if (v + r == t[ni] && in) ztgt[n0 + wcol + ni * 16 + i] = z;
-        zs[ni] += in ? z : 0.f;
-        acc[mi][ni][r] = in ? z : -INFINITY;
-        mx[ni] = fmaxf(mx[ni], acc[mi][ni][r]);
-      }
+    const int n = nbase + ni * 16;
+    t[ni] = n < rows ? p.tgt[n] - p.v0 - vbase : -1;
+    if ((unsigned)t[ni] >= (unsigned)(S::MI * 16) || (t[ni] & 15) > 3 ||
+        vbase + t[ni] >= p.vocab) {
+      t[ni] = -1;
     }
   }
-  float* red = reinterpret_cast<float*>(smem);
+  const bool whole = m0 + S::BM <= p.vocab;
+
+  if constexpr (MODE != AGAIN) {
+    float zs[S::NI];
 #pragma unroll
-  for (int ni = 0; ni < S::NI; ++ni) {
-    mx[ni] = fmaxf(mx[ni], __shfl_xor(mx[ni], 16));
-    mx[ni] = fmaxf(mx[ni], __shfl_xor(mx[ni], 32));
-    const float m = safe(mx[ni]);
+    for (int ni = 0; ni < S::NI; ++ni) {
+      zs[ni] = 0.f;
+      if (t[ni] >= 0) {
+#pragma unroll
+        for (int k = 0; k < S::MI * 4; ++k) {
+          if (t[ni] == (k >> 2) * 16 + (k & 3)) {
+            p.ztgt[nbase + ni * 16] = acc[k >> 2][ni][k & 3];
+          }
+        }
+      }
+    }
+    if (p.pz) {
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const bool in = whole || vbase + mi * 16 + r < p.vocab;
+#pragma unroll
+          for (int ni = 0; ni < S::NI; ++ni) {
+            zs[ni] += in ? acc[mi][ni][r] : 0.f;
+          }
+        }
+      }
+    }
+    if (!whole) {
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (vbase + mi * 16 + r >= p.vocab) {
+#pragma unroll
+            for (int ni = 0; ni < S::NI; ++ni) acc[mi][ni][r] = -INFINITY;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int ni = 0; ni < S::NI; ++ni) {
+      float m = -INFINITY;
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) m = fmaxf(m, acc[mi][ni][r]);
+      }
+      m = fmaxf(m, __shfl_xor(m, 16));
+      m = fmaxf(m, __shfl_xor(m, 32));
+      m = rintf(m * LOG2E);
+      const float ref = safe(m);
+      const int n = nbase + ni * 16;
+      float s = 0.f;
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) {
+        T out[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float e = power(acc[mi][ni][r], ref);
+          s += e;
+          out[r] = (T)(e * LIFT<T>);
+        }
+        if constexpr (MODE == KEEP) {
+          const int v = vbase + mi * 16;
+          if (n < rows && v < p.ldg) {
+            __builtin_memcpy(grad + (long)n * p.ldg + v, out, sizeof(out));
+          }
+        }
+      }
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+      float z = zs[ni];
+      if (p.pz) {
+        z += __shfl_xor(z, 16);
+        z += __shfl_xor(z, 32);
+      }
+      if (g == 0 && n < rows) {
+        const long at = (long)n * p.bands + tm * S::WM + wave / S::WN;
+        p.pmax[at] = m;
+        p.psum[at] = s;
+        if (p.pz) p.pz[at] = z;
+      }
+    }
+  } else {
+    float m[S::NI], k[S::NI], c[S::NI];
+#pragma unroll
+    for (int ni = 0; ni < S::NI; ++ni) {
+      const int n = nbase + ni * 16;
+      const bool in = n < rows;
+      c[ni] = in ? p.coef[n] : 0.f;
+      m[ni] = in ? p.rowm[n] : 0.f;
+      k[ni] = in ? p.rowi[n] * c[ni] : 0.f;
+    }
 #pragma unroll
     for (int mi = 0; mi < S::MI; ++mi) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        sm[ni] += __builtin_amdgcn_exp2f((acc[mi][ni][r] - m) * LOG2E);
+      for (int ni = 0; ni < S::NI; ++ni) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          acc[mi][ni][r] = fmaf(power(acc[mi][ni][r], m[ni]), k[ni],
+                                -p.share * c[ni]);
+        }
       }
     }
-    sm[ni] += __shfl_xor(sm[ni], 16);
-    sm[ni] += __shfl_xor(sm[ni], 32);
-    zs[ni] += __shfl_xor(zs[ni], 16);
-    zs[ni] += __shfl_xor(zs[ni], 32);
-    if (g == 0) {
-      float* p = red + ((wave / S::WN) * S::BN + wcol + ni * 16 + i) * 3;
-      p[0] = mx[ni];
-      p[1] = sm[ni];
-      p[2] = zs[ni];
-    }
-  }
-  __syncthreads();
-  for (int c = threadIdx.x; c < S::BN; c += S::THREADS) {
-    if (n0 + c >= rows) continue;
-    float m = -INFINITY, s = 0.f, z = 0.f;
 #pragma unroll
-    for (int k = 0; k < S::WM; ++k) m = fmaxf(m, red[(k * S::BN + c) * 3]);
+    for (int ni = 0; ni < S::NI; ++ni) {
+      if (t[ni] >= 0) {
 #pragma unroll
-    for (int k = 0; k < S::WM; ++k) {
-      const float* p = red + (k * S::BN + c) * 3;
-      s += p[1] * __builtin_amdgcn_exp2f((safe(p[0]) - safe(m)) * LOG2E);
-      z += p[2];
+        for (int q = 0; q < S::MI * 4; ++q) {
+          if (t[ni] == (q >> 2) * 16 + (q & 3)) {
+            acc[q >> 2][ni][q & 3] -= (1.f - p.eps) * c[ni];
+          }
+        }
+      }
     }
-    const long at = (long)(n0 + c) * mt + tm;
-    pmax[at] = m;
-    psum[at] = s;
-    if (smooth) pz[at] = z;
+    if (!whole) {
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (vbase + mi * 16 + r >= p.vocab) {
+#pragma unroll
+            for (int ni = 0; ni < S::NI; ++ni) acc[mi][ni][r] = 0.f;
+          }
+        }
+      }
+    }
+    float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int mi = 0; mi < S::MI; ++mi) {
+      const int v = vbase + mi * 16;
+#pragma unroll
+      for (int ni = 0; ni < S::NI; ++ni) {
+        const int n = nbase + ni * 16;
+        T out[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) out[r] = (T)acc[mi][ni][r];
+        if (n < rows && v < p.ldg) {
+          __builtin_memcpy(grad + (long)n * p.ldg + v, out, sizeof(out));
+        }
+      }
+      if (p.pbias) {  // summed before the rounding
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float s = 0.f;
+#pragma unroll
+          for (int ni = 0; ni < S::NI; ++ni) {
+            s += nbase + ni * 16 < rows ? acc[mi][ni][r] : 0.f;
+          }
+          s += __shfl_xor(s, 1);
+          s += __shfl_xor(s, 2);
+          s += __shfl_xor(s, 4);
+          s += __shfl_xor(s, 8);
+          if (i == 0) {
+            red[(wave % S::WN) * S::BM + wrow + mi * 16 + g * 4 + r] = s;
+          }
+        }
+      }
+    }
+    if (p.pbias) {
+      __syncthreads();
+      for (int q = threadIdx.x; q < S::BM; q += S::THREADS) {
+        if (m0 + q >= p.vocab) continue;
+        float s = 0.f;
+#pragma unroll
+        for (int j = 0; j < S::WN; ++j) s += red[j * S::BM + q];
+        p.pbias[(long)tn * p.all + p.v0 + m0 + q] = s;
+      }
+    }
   }
 }
 
-// one wave per row of the call: joins the tiles' sums
+// One wave per row of the call: joins the bands.  rowm is the row's whole
+// reference and rowi the inverse of its sum, p = power(z, rowm) rowi.
 __global__ __launch_bounds__(256) void join_kernel(
     const float* __restrict__ pmax, const float* __restrict__ psum,
     const float* __restrict__ pz, const float* __restrict__ ztgt,
     const int* __restrict__ pos, const int* __restrict__ tgt, long rows,
-    int mt, float eps, float share, float* __restrict__ lse,
-    float* __restrict__ loss) {
+    int bands, float eps, float share, float* __restrict__ rowm,
+    float* __restrict__ rowi, float* __restrict__ loss) {
   const int lane = threadIdx.x & 63;
   const long n = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (n >= rows) return;
@@ -237,25 +415,75 @@ __global__ __launch_bounds__(256) void join_kernel(
     if (lane == 0) loss[n] = 0.f;
     return;
   }
-  const long at = (long)p * mt;
+  const long at = (long)p * bands;
   float m = -INFINITY;
-  for (int k = lane; k < mt; k += 64) m = fmaxf(m, pmax[at + k]);
-  m = wave_max(m);
-  const float base = safe(m);
+  for (int k = lane; k < bands; k += 64) m = fmaxf(m, pmax[at + k]);
+  m = safe(wave_max(m));
   float s = 0.f, z = 0.f;
-  for (int k = lane; k < mt; k += 64) {
-    s += psum[at + k] *
-         __builtin_amdgcn_exp2f((safe(pmax[at + k]) - base) * LOG2E);
-    if (eps != 0.f) z += pz[at + k];
+  for (int k = lane; k < bands; k += 64) {
+    s = fmaf(psum[at + k], __builtin_amdgcn_exp2f(safe(pmax[at + k]) - m), s);
+    if (pz) z += pz[at + k];
   }
   s = wave_sum(s);
   z = wave_sum(z);
   if (lane == 0) {
-    const float l = base + __builtin_amdgcn_logf(s) * LN2;
-    lse[p] = l;
-    float v = l - (1.f - eps) * ztgt[p];
-    if (eps != 0.f) v -= share * z;
-    loss[n] = tgt[p] == BAD ? NAN : v;
+    rowm[p] = m;
+    rowi[p] = 1.f / s;
+    // the powers are of the rounded log2(e): dividing by it undoes that
+    double v = ((double)m + log2((double)s)) / (double)LOG2E -
+               (1.0 - (double)eps) * (double)ztgt[p];
+    if (pz) v -= (double)share * (double)z;
+    loss[n] = tgt[p] == BAD ? NAN : (float)v;
+  }
+}
+
+// ------------------------------------------------- g from the kept powers
+// In place: g = c (power 2^(band - row) / sum - eps / V), the target's entry
+// anew from its z.  A workgroup takes PROWS tokens, a lane one 16-byte chunk
+// of each of them, and sums the bias gradient down the rows in passing.
+constexpr int PROWS = 64;
+
+template <class T>
+__global__ __launch_bounds__(256) void probs_kernel(
+    T* __restrict__ grad, long ldg, int vocab, const int* __restrict__ count,
+    const int* __restrict__ tgt, const float* __restrict__ pmax, int bands,
+    int band, const float* __restrict__ rowm, const float* __restrict__ rowi,
+    const float* __restrict__ ztgt, const float* __restrict__ coef, float eps,
+    float share, float* __restrict__ pbias) {
+  constexpr int E = 16 / sizeof(T);
+  const int rows = *count;
+  const int n0 = blockIdx.x * PROWS;
+  const int v = (blockIdx.y * 256 + threadIdx.x) * E;
+  if (n0 >= rows || v >= ldg) return;
+  const int n1 = rows - n0 < PROWS ? rows : n0 + PROWS;
+  const int mine = v / band;
+  float sum[E] = {};
+#pragma unroll 4
+  for (int n = n0; n < n1; ++n) {
+    struct alignas(16) Chunk {
+      T v[E];
+    };
+    Chunk* at = reinterpret_cast<Chunk*>(grad + (long)n * ldg + v);
+    Chunk t = *at;
+    const float c = coef[n], m = rowm[n], i = rowi[n];
+    const float k = __builtin_amdgcn_exp2f(safe(pmax[(long)n * bands + mine]) -
+                                           m) * i * c * (1.f / LIFT<T>);
+    const int hit = tgt[n] - v;
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      float d = fmaf((float)t.v[j], k, -share * c);
+      if (hit == j) d = (power(ztgt[n], m) * i - share - (1.f - eps)) * c;
+      d = v + j < vocab ? d : 0.f;
+      sum[j] += d;
+      t.v[j] = (T)d;
+    }
+    *at = t;
+  }
+  if (pbias) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) {
+      if (v + j < vocab) pbias[(long)blockIdx.x * vocab + v + j] = sum[j];
+    }
   }
 }
 
@@ -279,7 +507,7 @@ __global__ __launch_bounds__(1024) void total_kernel(
 
 // ---------------------------------------------------------- row coefficients
 // coef[i] = d(total)/d(loss of kept row i) times a power of two, scale[0];
-// scale[1] is its inverse.  fp16 holds g to 6e-8 only, and c_n = 1/rows times
+// scale[1] is its inverse.  Without `up` the upstream factor is 1.  fp16 holds g to 6e-8 only, and c_n = 1/rows times
 // a small probability is soon below that: there the largest |c_n| is brought
 // to [2^14, 2^15) (|g| <= |c_n|, and the type ends at 65504) and the products
 // are scaled back in fp32.
@@ -291,7 +519,8 @@ __global__ __launch_bounds__(1024) void coef_kernel(
   __shared__ float part[16];
   __shared__ float shared_scale;
   const int rows = *count;
-  const float one = each ? 1.f : (mean ? *up / (float)rows : *up);
+  const float first = up && !each ? *up : 1.f;
+  const float one = mean ? first / (float)rows : first;
   float top = 0.f;
   if (lift) {
     if (each) {
@@ -325,106 +554,23 @@ __global__ __launch_bounds__(1024) void coef_kernel(
   }
 }
 
-// ------------------------------------------------------------ gradient tiles
-// g[n, v - v0] for a piece [v0, v0 + piece) of the vocabulary; entries from
-// the piece's end to ldg are zeros.  The bias gradient's part of a tile is
-// summed before the rounding.
-template <class T, class S>
-__global__ __launch_bounds__(S::THREADS) void grad_kernel(
-    const T* __restrict__ w, long ldw, const T* __restrict__ x, long ldx,
-    const T* __restrict__ bias, int v0, int piece, int dim, const int* count,
-    int mt, int nt, const int* __restrict__ tgt,
-    const float* __restrict__ lse, const float* __restrict__ coef, float eps,
-    float share, T* __restrict__ grad, long ldg, float* __restrict__ pbias,
-    long vocab) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  int tm, tn;
-  tile::pick(blockIdx.x, mt, nt, &tm, &tn);
-  const int rows = *count;
-  const int m0 = tm * S::BM, n0 = tn * S::BN;
-  if (n0 >= rows) return;
-  f32x4 acc[S::MI][S::NI] = {};
-  tile::product<T, false, false, S>(w + (long)v0 * ldw, ldw, m0, piece, x,
-                                    ldx, n0, rows, 0, dim, dim, smem, acc);
-
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int i = lane & 15, g = lane >> 4;
-  const int wrow = (wave / S::WN) * (S::MI * 16);
-  const int wcol = (wave % S::WN) * (S::NI * 16);
-  float l[S::NI], c[S::NI];
-  int t[S::NI];
-#pragma unroll
-  for (int ni = 0; ni < S::NI; ++ni) {
-    const int n = n0 + wcol + ni * 16 + i;
-    const bool in = n < rows;
-    l[ni] = in ? lse[n] : 0.f;
-    c[ni] = in ? coef[n] : 0.f;
-    t[ni] = in ? tgt[n] - v0 : BAD;
-  }
-  float* red = reinterpret_cast<float*>(smem);
-#pragma unroll
-  for (int mi = 0; mi < S::MI; ++mi) {
-    const int vl = wrow + mi * 16 + g * 4;  // within the tile
-    const int v = m0 + vl;                  // within the piece
-    float b[4], sb[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      b[r] = bias && v + r < piece ? to_float(bias[v0 + v + r]) : 0.f;
-    }
-#pragma unroll
-    for (int ni = 0; ni < S::NI; ++ni) {
-      const int n = n0 + wcol + ni * 16 + i;
-      T out[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const float p =
-            __builtin_amdgcn_exp2f((acc[mi][ni][r] + b[r] - l[ni]) * LOG2E);
-        float d = p - share;
-        if (v + r == t[ni]) d -= 1.f - eps;
-        d *= c[ni];
-        d = v + r < piece ? d : 0.f;
-        sb[r] += n < rows ? d : 0.f;
-        out[r] = (T)d;
-      }
-      if (n < rows && v < ldg) {
-        __builtin_memcpy(grad + (long)n * ldg + v, out, 4 * sizeof(T));
-      }
-    }
-    if (pbias) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float s = sb[r];
-        s += __shfl_xor(s, 1);
-        s += __shfl_xor(s, 2);
-        s += __shfl_xor(s, 4);
-        s += __shfl_xor(s, 8);
-        if (i == 0) red[(wave % S::WN) * S::BM + vl + r] = s;
-      }
-    }
-  }
-  if (pbias) {
-    __syncthreads();
-    for (int k = threadIdx.x; k < S::BM; k += S::THREADS) {
-      if (m0 + k >= piece) continue;
-      float s = 0.f;
-#pragma unroll
-      for (int j = 0; j < S::WN; ++j) s += red[j * S::BM + k];
-      pbias[(long)tn * vocab + v0 + m0 + k] = s;
-    }
-  }
+// what the products are multiplied by at the end
+__device__ __forceinline__ float factor(const float* scale, const float* up) {
+  return scale[1] * (up ? *up : 1.f);
 }
 
 template <class T>
 __global__ void bias_kernel(const float* __restrict__ pbias, long vocab,
-                            int bn, const int* __restrict__ count,
+                            int part, const int* __restrict__ count,
                             const float* __restrict__ scale,
+                            const float* __restrict__ up,
                             T* __restrict__ out) {
   const long v = (long)blockIdx.x * blockDim.x + threadIdx.x;
   if (v >= vocab) return;
-  const int parts = (*count + bn - 1) / bn;
+  const int parts = (*count + part - 1) / part;  // of `part` tokens
   float s = 0.f;
   for (int k = 0; k < parts; ++k) s += pbias[(long)k * vocab + v];
-  out[v] = (T)(s * scale[1]);
+  out[v] = (T)(s * factor(scale, up));
 }
 
 // ------------------------------------------------------------- dx += g w
@@ -464,25 +610,63 @@ __global__ __launch_bounds__(S::THREADS) void dx_kernel(
   }
 }
 
-// dx of every row of the call: the slabs' sum, or zeros for a row left out
+// Adds slabs of fp32 rows (ldim values, a multiple of 4) into rows of `dim`
+// values of T.  pos: which slab row a row takes, none (zeros) for -1.
 template <class T>
-__global__ void dx_out_kernel(const float* __restrict__ slabs, long slab,
-                              int splits, int ldim, int dim, long rows,
-                              const int* __restrict__ pos,
-                              const float* __restrict__ scale,
-                              T* __restrict__ out) {
-  const float inv = scale[1];
-  const long total = rows * dim;
+__global__ __launch_bounds__(256) void add_kernel(
+    const float* __restrict__ slabs, long slab, int splits, int ldim, int dim,
+    long rows, const int* __restrict__ pos, const float* __restrict__ scale,
+    const float* __restrict__ up, T* __restrict__ out) {
+  const float f = factor(scale, up);
+  const int groups = (dim + 3) / 4;
+  const long total = rows * groups;
   for (long k = (long)blockIdx.x * blockDim.x + threadIdx.x; k < total;
        k += (long)gridDim.x * blockDim.x) {
-    const long n = k / dim;
-    const int d = (int)(k - n * dim);
-    const int p = pos[n];
-    float s = 0.f;
+    const long n = k / groups;
+    const int d = (int)(k - n * groups) * 4;
+    const long p = pos ? pos[n] : n;
+    f32x4 s = {};
     if (p >= 0) {
-      for (int j = 0; j < splits; ++j) s += slabs[j * slab + (long)p * ldim + d];
+      const float* at = slabs + p * ldim + d;
+#pragma unroll 8
+      for (int j = 0; j < splits; ++j) {
+        s += *reinterpret_cast<const f32x4*>(at + j * slab);
+      }
     }
-    out[k] = (T)(s * inv);
+    T o[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = (T)(s[r] * f);
+    if (d + 4 <= dim) {
+      __builtin_memcpy(out + n * dim + d, o, sizeof(o));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (d + r < dim) out[n * dim + d + r] = o[r];
+      }
+    }
+  }
+}
+
+// out *= up, where that changes anything; out is 16-byte aligned
+template <class T>
+__global__ __launch_bounds__(256) void times_kernel(
+    T* __restrict__ out, long n, const float* __restrict__ up) {
+  const float f = *up;
+  if (f == 1.f) return;
+  constexpr int E = 16 / sizeof(T);
+  struct alignas(16) Chunk {
+    T v[E];
+  };
+  for (long k = (long)blockIdx.x * blockDim.x + threadIdx.x; k * E < n;
+       k += (long)gridDim.x * blockDim.x) {
+    if ((k + 1) * E <= n) {
+      Chunk c = reinterpret_cast<Chunk*>(out)[k];
+#pragma unroll
+      for (int j = 0; j < E; ++j) c.v[j] = (T)((float)c.v[j] * f);
+      reinterpret_cast<Chunk*>(out)[k] = c;
+    } else {
+      for (long j = k * E; j < n; ++j) out[j] = (T)((float)out[j] * f);
+    }
   }
 }
 
@@ -533,23 +717,6 @@ __global__ __launch_bounds__(S::THREADS) void dw_kernel(
   }
 }
 
-template <class T>
-__global__ void dw_out_kernel(const float* __restrict__ slabs, long slab,
-                              int splits, int ldim, int dim, long entries,
-                              const float* __restrict__ scale,
-                              T* __restrict__ out) {
-  const float inv = scale[1];
-  const long total = entries * dim;
-  for (long k = (long)blockIdx.x * blockDim.x + threadIdx.x; k < total;
-       k += (long)gridDim.x * blockDim.x) {
-    const long v = k / dim;
-    const int d = (int)(k - v * dim);
-    float s = 0.f;
-    for (int j = 0; j < splits; ++j) s += slabs[j * slab + v * ldim + d];
-    out[k] = (T)(s * inv);
-  }
-}
-
 int blocks_for(long work) {
   return (int)std::min<long>(std::max<long>((work + 255) / 256, 1), 8192);
 }
@@ -557,7 +724,7 @@ int blocks_for(long work) {
 int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 using Wide = Shape<256, 256, 2, 4>;
-using Mid = Shape<128, 128, 2, 2>;
+using Mid = Shape<128, 128, 2, 4>;
 
 template <class F>
 void with_lds(F* kernel, int bytes) {
@@ -568,71 +735,117 @@ void with_lds(F* kernel, int bytes) {
 
 template <class T>
 struct Run {
-  template <class S>
-  static void stats(const Forward& f, hipStream_t s) {
-    const int mt = ceil_div(f.vocab, S::BM), nt = ceil_div(f.rows, S::BN);
-    with_lds(stats_kernel<T, S>, S::LDS);
-    stats_kernel<T, S><<<mt * nt, S::THREADS, S::LDS, s>>>(
-        (const T*)f.w, f.ldw, (const T*)f.x, f.ldx, (const T*)f.bias,
-        (int)f.vocab, f.ldx, f.count, mt, nt, f.tgt, f.eps != 0.f, f.pmax,
-        f.psum, f.pz, f.ztgt);
-    check(hipGetLastError());
-    join_kernel<<<ceil_div(f.rows, 4), 256, 0, s>>>(
-        f.pmax, f.psum, f.pz, f.ztgt, f.pos, f.tgt, f.rows, mt, f.eps,
-        f.eps / (float)f.vocab, f.lse, f.loss);
+  template <class S, int MODE>
+  static void logits(const Operands& o, Logits p, T* grad, hipStream_t s) {
+    p.ldw = o.ldw;
+    p.ldx = o.ldx;
+    p.mt = ceil_div(p.vocab, S::BM);
+    p.nt = ceil_div(o.rows, S::BN);
+    p.count = o.count;
+    p.tgt = o.tgt;
+    with_lds(logits_kernel<T, S, MODE>, S::LDS);
+    logits_kernel<T, S, MODE><<<p.mt * p.nt, S::THREADS, S::LDS, s>>>(
+        (const T*)o.w, (const T*)o.x, (const T*)o.bias, grad, p);
     check(hipGetLastError());
   }
 
   template <class S>
-  static void pieces(const Backward& b, hipStream_t s) {
-    const int dim = b.ldx;
-    const int nt = ceil_div(b.rows, S::BN), md = ceil_div(dim, S::BM);
-    const long slab = b.rows * dim;
-    with_lds(grad_kernel<T, S>, S::LDS);
-    with_lds(dx_kernel<T, S>, S::LDS);
-    with_lds(dw_kernel<T, S>, S::LDS);
-    for (long v0 = 0; v0 < b.vocab; v0 += b.piece) {
-      const int piece = (int)std::min(b.piece, b.vocab - v0);
-      const long ldg = (piece + 7) / 8 * 8;
-      const int mt = ceil_div(piece, S::BM);
-      grad_kernel<T, S><<<mt * nt, S::THREADS, S::LDS, s>>>(
-          (const T*)b.w, b.ldw, (const T*)b.x, b.ldx, (const T*)b.bias,
-          (int)v0, piece, dim, b.count, mt, nt, b.tgt, b.lse, b.coef, b.eps,
-          b.eps / (float)b.vocab, (T*)b.grad, ldg, b.pbias, b.vocab);
-      check(hipGetLastError());
-      if (b.dx) {
-        const int run = ceil_div(ceil_div(ldg, b.dx_splits), 64) * 64;
-        dx_kernel<T, S><<<md * nt * b.dx_splits, S::THREADS, S::LDS, s>>>(
-            (const T*)b.w + v0 * b.ldw, b.ldw, (const T*)b.grad, ldg, piece,
-            dim, b.count, md, nt, run, v0 == 0, b.dx_slabs, slab);
-        check(hipGetLastError());
-      }
-      if (b.dw) {
-        const int vt = ceil_div(piece, S::BN);
-        const int run = ceil_div(ceil_div(b.rows, b.dw_splits), 64) * 64;
-        T* out = (T*)b.dw + v0 * b.dim;
-        const long part = (long)piece * dim;
-        dw_kernel<T, S><<<md * vt * b.dw_splits, S::THREADS, S::LDS, s>>>(
-            (const T*)b.x, b.ldx, (const T*)b.grad, ldg, piece, b.dim, dim,
-            b.count, md, vt, run, b.scale, out,
-            b.dw_splits > 1 ? b.dw_slabs : nullptr, part);
-        check(hipGetLastError());
-        if (b.dw_splits > 1) {
-          dw_out_kernel<T><<<blocks_for((long)piece * b.dim), 256, 0, s>>>(
-              b.dw_slabs, part, b.dw_splits, dim, b.dim, piece, b.scale, out);
-          check(hipGetLastError());
-        }
-      }
+  static void forward(const Operands& o, const Sums& f, T* grad,
+                      hipStream_t s) {
+    Logits p{};
+    p.vocab = (int)o.vocab;
+    p.pmax = f.pmax;
+    p.psum = f.psum;
+    p.pz = o.eps != 0.f ? f.pz : nullptr;
+    p.ztgt = f.ztgt;
+    p.bands = o.plan.bands;
+    if (grad) {
+      p.ldg = padded(o.vocab);
+      logits<S, KEEP>(o, p, grad, s);
+    } else {
+      logits<S, SUMS>(o, p, nullptr, s);
     }
+    join_kernel<<<ceil_div(o.rows, 4), 256, 0, s>>>(
+        f.pmax, f.psum, p.pz, f.ztgt, o.pos, o.tgt, o.rows, p.bands, o.eps,
+        o.eps / (float)o.vocab, f.rowm, f.rowi, f.loss);
+    check(hipGetLastError());
+  }
+
+  static void probs(const Operands& o, const Sums& f, const Grads& b,
+                    hipStream_t s) {
+    const long ldg = padded(o.vocab);
+    const dim3 grid(ceil_div(o.rows, PROWS),
+                    ceil_div(ldg * sizeof(T) / 16, 256));
+    probs_kernel<T><<<grid, 256, 0, s>>>(
+        (T*)b.grad, ldg, (int)o.vocab, o.count, o.tgt, f.pmax, o.plan.bands,
+        o.plan.band, f.rowm, f.rowi, f.ztgt, b.coef, o.eps,
+        o.eps / (float)o.vocab, b.pbias);
+    check(hipGetLastError());
+  }
+
+  template <class S>
+  static void again(const Operands& o, const Sums& f, const Grads& b,
+                    long v0, int piece, hipStream_t s) {
+    Logits p{};
+    p.v0 = (int)v0;
+    p.vocab = piece;
+    p.ldg = padded(piece);
+    p.rowm = f.rowm;
+    p.rowi = f.rowi;
+    p.coef = b.coef;
+    p.eps = o.eps;
+    p.share = o.eps / (float)o.vocab;
+    p.pbias = b.pbias;
+    p.all = o.vocab;
+    logits<S, AGAIN>(o, p, (T*)b.grad, s);
+  }
+
+  template <class S>
+  static void products(const Operands& o, const Grads& b, long v0, int piece,
+                       hipStream_t s) {
+    const int ldim = o.ldx, md = ceil_div(ldim, S::BM);
+    const long ldg = padded(piece);
+    if (b.dx_slabs) {
+      const int nt = ceil_div(o.rows, S::BN), splits = o.plan.dx_splits;
+      const int run = ceil_div(ceil_div(ldg, splits), 64) * 64;
+      with_lds(dx_kernel<T, S>, S::LDS);
+      dx_kernel<T, S><<<md * nt * splits, S::THREADS, S::LDS, s>>>(
+          (const T*)o.w + v0 * o.ldw, o.ldw, (const T*)b.grad, ldg, piece,
+          ldim, o.count, md, nt, run, v0 == 0, b.dx_slabs, o.rows * ldim);
+      check(hipGetLastError());
+    }
+    if (b.dw || b.dw_slabs) {
+      const int vt = ceil_div(piece, S::BN), splits = o.plan.dw_splits;
+      const int run = ceil_div(ceil_div(o.rows, splits), 64) * 64;
+      with_lds(dw_kernel<T, S>, S::LDS);
+      dw_kernel<T, S><<<md * vt * splits, S::THREADS, S::LDS, s>>>(
+          (const T*)o.x, o.ldx, (const T*)b.grad, ldg, piece, o.dim, ldim,
+          o.count, md, vt, run, b.scale, (T*)b.dw + v0 * o.dim, b.dw_slabs,
+          (long)piece * ldim);
+      check(hipGetLastError());
+    }
+  }
+
+  // rows [v0, v0 + piece) of dw from its slabs
+  static void end_dw(const Operands& o, const Grads& b, long v0, int piece,
+                     const float* up, hipStream_t s) {
+    add_kernel<T><<<blocks_for((long)piece * ((o.dim + 3) / 4)), 256, 0, s>>>(
+        b.dw_slabs, (long)piece * o.ldx, o.plan.dw_splits, o.ldx, o.dim,
+        piece, nullptr, b.scale, up, (T*)b.dw + v0 * o.dim);
+    check(hipGetLastError());
+  }
+
+  static void end(const Operands& o, const Grads& b, const float* up,
+                  hipStream_t s) {
     if (b.dx) {
-      dx_out_kernel<T><<<blocks_for(b.rows * b.dim), 256, 0, s>>>(
-          b.dx_slabs, slab, b.dx_splits, dim, b.dim, b.rows, b.pos, b.scale,
-          (T*)b.dx);
+      add_kernel<T><<<blocks_for(o.rows * ((o.dim + 3) / 4)), 256, 0, s>>>(
+          b.dx_slabs, o.rows * o.ldx, o.plan.dx_splits, o.ldx, o.dim, o.rows,
+          o.pos, b.scale, up, (T*)b.dx);
       check(hipGetLastError());
     }
     if (b.db) {
-      bias_kernel<T><<<ceil_div(b.vocab, 256), 256, 0, s>>>(
-          b.pbias, b.vocab, S::BN, b.count, b.scale, (T*)b.db);
+      bias_kernel<T><<<ceil_div(o.vocab, 256), 256, 0, s>>>(
+          b.pbias, o.vocab, b.part, o.count, b.scale, up, (T*)b.db);
       check(hipGetLastError());
     }
   }
@@ -655,19 +868,24 @@ bool wide(long m, long n) {
 
 }  // namespace
 
-Plan plan(long rows, long vocab, int ldim, int size) {
+long padded(long n) { return (n + 7) / 8 * 8; }
+
+Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   Plan p;
   p.wide = wide(vocab, rows);
   p.edge = p.wide ? 256 : 128;
-  p.tiles = ceil_div(vocab, p.edge);
-  p.row_tiles = ceil_div(rows, p.edge);
+  p.band = p.wide ? 128 : 64;
+  p.bands = ceil_div(vocab, p.edge) * (p.edge / p.band);
   // a piece of the vocabulary: 256 MB of g at most, which the card's last
   // cache then holds between the three products; offsets within a tile of g
   // stay below 2^31 for rows of up to a million entries
   const long most = std::min<long>(
       std::max<long>((256l << 20) / (rows * size), p.edge), 1l << 20);
-  p.piece = std::min(vocab, most / p.edge * p.edge);
-  const long dx_tiles = (long)ceil_div(ldim, p.edge) * p.row_tiles;
+  p.piece = keep ? vocab : std::min(vocab, most / p.edge * p.edge);
+  p.parts = keep ? ceil_div(rows, PROWS) : ceil_div(rows, p.edge);
+  p.part = keep ? PROWS : p.edge;
+  const long dx_tiles =
+      (long)ceil_div(ldim, p.edge) * ceil_div(rows, p.edge);
   const long dw_tiles =
       (long)ceil_div(ldim, p.edge) * ceil_div(p.piece, p.edge);
   const long want = p.wide ? 256 : 512;
@@ -706,13 +924,14 @@ void pack(Type t, const void* in, long ld, long step, long rows, int cols,
   });
 }
 
-void forward(Type t, const Forward& f, hipStream_t s) {
-  by_type(t, [&](auto* p) {
-    using T = std::remove_pointer_t<decltype(p)>;
-    if (f.plan.wide) {
-      Run<T>::template stats<Wide>(f, s);
+void forward(Type t, const Operands& o, const Sums& f, void* grad,
+             hipStream_t s) {
+  by_type(t, [&](auto* q) {
+    using T = std::remove_pointer_t<decltype(q)>;
+    if (o.plan.wide) {
+      Run<T>::template forward<Wide>(o, f, (T*)grad, s);
     } else {
-      Run<T>::template stats<Mid>(f, s);
+      Run<T>::template forward<Mid>(o, f, (T*)grad, s);
     }
   });
 }
@@ -723,17 +942,59 @@ void total(const float* loss, long rows, const int* count, bool mean,
   check(hipGetLastError());
 }
 
-void backward(Type t, const Backward& b, hipStream_t s) {
-  coef_kernel<<<1, 1024, 0, s>>>(b.up, b.each, b.mean, b.idx, b.tgt, b.count,
+void coefficients(Type t, const Operands& o, const float* up, bool each,
+                  bool mean, const Grads& b, hipStream_t s) {
+  coef_kernel<<<1, 1024, 0, s>>>(up, each, mean, o.idx, o.tgt, o.count,
                                  t == Type::fp16, b.coef, b.scale);
   check(hipGetLastError());
-  by_type(t, [&](auto* p) {
-    using T = std::remove_pointer_t<decltype(p)>;
-    if (b.plan.wide) {
-      Run<T>::template pieces<Wide>(b, s);
+}
+
+void gradients_kept(Type t, const Operands& o, const Sums& f, const Grads& b,
+                    hipStream_t s) {
+  by_type(t, [&](auto* q) {
+    using T = std::remove_pointer_t<decltype(q)>;
+    Run<T>::probs(o, f, b, s);
+    if (o.plan.wide) {
+      Run<T>::template products<Wide>(o, b, 0, (int)o.vocab, s);
     } else {
-      Run<T>::template pieces<Mid>(b, s);
+      Run<T>::template products<Mid>(o, b, 0, (int)o.vocab, s);
     }
+  });
+}
+
+void finish_kept(Type t, const Operands& o, const Grads& b, const float* up,
+                 hipStream_t s) {
+  by_type(t, [&](auto* q) {
+    using T = std::remove_pointer_t<decltype(q)>;
+    Run<T>::end(o, b, up, s);
+    if (b.dw && b.dw_slabs) {
+      Run<T>::end_dw(o, b, 0, (int)o.vocab, up, s);
+    } else if (b.dw) {
+      const long n = o.vocab * o.dim;
+      times_kernel<T><<<blocks_for(n / 8), 256, 0, s>>>((T*)b.dw, n, up);
+      check(hipGetLastError());
+    }
+  });
+}
+
+void gradients_again(Type t, const Operands& o, const Sums& f, const Grads& b,
+                     hipStream_t s) {
+  by_type(t, [&](auto* q) {
+    using T = std::remove_pointer_t<decltype(q)>;
+    for (long v0 = 0; v0 < o.vocab; v0 += o.plan.piece) {
+      const int piece = (int)std::min(o.plan.piece, o.vocab - v0);
+      if (o.plan.wide) {
+        Run<T>::template again<Wide>(o, f, b, v0, piece, s);
+        Run<T>::template products<Wide>(o, b, v0, piece, s);
+      } else {
+        Run<T>::template again<Mid>(o, f, b, v0, piece, s);
+        Run<T>::template products<Mid>(o, b, v0, piece, s);
+      }
+      if (b.dw && b.dw_slabs) {
+        Run<T>::end_dw(o, b, v0, piece, nullptr, s);
+      }
+    }
+    Run<T>::end(o, b, nullptr, s);
   });
 }
 

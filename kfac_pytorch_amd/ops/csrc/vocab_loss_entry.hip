@@ -36,8 +36,6 @@ struct Ints {
   }
 };
 
-int padded(long dim) { return (int)((dim + 7) / 8 * 8); }
-
 // Whether the kernels can load the weight's rows as they lie; otherwise they
 // are packed once into rows of whole 16-byte chunks.
 bool direct(const Tensor& w) {
@@ -48,36 +46,82 @@ bool direct(const Tensor& w) {
          reinterpret_cast<uintptr_t>(w.data_ptr()) % 16 == 0;
 }
 
-struct Operands {
-  Tensor x, w, b;  // packed kept rows; weight; contiguous bias
-  long ldw;
+// The operands as the kernels take them, and what owns them.
+struct Call {
+  vocab_loss::Operands o{};
+  Tensor x, w, b;
+  Type type;
+  int size;
 };
 
-Operands operands(Type type, const Tensor& hidden, const Tensor& weight,
-                  const std::optional<Tensor>& bias, const Ints& ints,
-                  hipStream_t stream) {
-  Operands o;
-  const int ld = padded(hidden.size(1));
-  o.x = at::empty({hidden.size(0), ld}, hidden.options());
-  vocab_loss::pack(type, hidden.data_ptr(), hidden.stride(0),
-                   hidden.stride(1), hidden.size(0), (int)hidden.size(1),
-                   ints.idx, ints.count, o.x.data_ptr(), ld, stream);
-  if (direct(weight)) {
-    o.w = weight;
-    o.ldw = weight.stride(0);
-  } else {
-    o.w = at::empty({weight.size(0), ld}, weight.options());
-    vocab_loss::pack(type, weight.data_ptr(), weight.stride(0),
-                     weight.stride(1), weight.size(0), (int)weight.size(1),
-                     nullptr, nullptr, o.w.data_ptr(), ld, stream);
-    o.ldw = ld;
-  }
-  if (bias) o.b = bias->contiguous();
-  return o;
+Call make_call(const Tensor& hidden, const Tensor& weight,
+               const std::optional<Tensor>& bias, const Tensor& ints_t,
+               double eps, bool keep) {
+  Call c;
+  c.type = type_of(hidden);
+  c.size = (int)hidden.element_size();
+  auto& o = c.o;
+  o.rows = hidden.size(0);
+  o.vocab = weight.size(0);
+  o.dim = (int)hidden.size(1);
+  o.ldx = (int)vocab_loss::padded(o.dim);
+  o.eps = (float)eps;
+  o.plan = vocab_loss::plan(o.rows, o.vocab, o.ldx, c.size, keep);
+  const Ints ints(ints_t, o.rows);
+  o.pos = ints.pos;
+  o.idx = ints.idx;
+  o.tgt = ints.tgt;
+  o.count = ints.count;
+  return c;
 }
 
-const void* data_or_null(const Tensor& t) {
-  return t.defined() ? t.data_ptr() : nullptr;
+void pack(Call* c, const Tensor& hidden, const Tensor& weight,
+          const std::optional<Tensor>& bias, hipStream_t stream) {
+  auto& o = c->o;
+  c->x = at::empty({o.rows, o.ldx}, hidden.options());
+  vocab_loss::pack(c->type, hidden.data_ptr(), hidden.stride(0),
+                   hidden.stride(1), o.rows, o.dim, o.idx, o.count,
+                   c->x.data_ptr(), o.ldx, stream);
+  o.x = c->x.data_ptr();
+  if (direct(weight)) {
+    c->w = weight;
+    o.ldw = weight.stride(0);
+  } else {
+    c->w = at::empty({o.vocab, o.ldx}, weight.options());
+    vocab_loss::pack(c->type, weight.data_ptr(), weight.stride(0),
+                     weight.stride(1), o.vocab, o.dim, nullptr, nullptr,
+                     c->w.data_ptr(), o.ldx, stream);
+    o.ldw = o.ldx;
+  }
+  o.w = c->w.data_ptr();
+  if (bias) {
+    c->b = bias->contiguous();
+    o.bias = c->b.data_ptr();
+  }
+}
+
+float* floats(const Tensor& t) {
+  return t.defined() ? t.data_ptr<float>() : nullptr;
+}
+
+void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// The powers of a whole call are kept up to this many bytes (while the call
+// lasts); beyond, the backward pass makes the logits again.  Kept, 8192 x
+// 128000 x 4096 in bf16 takes 2 GiB and a quarter less time.
+constexpr long MOST_KEPT = 4l << 30;
+
+bool keeps(long rows, long vocab, int size) {
+  const long row = vocab_loss::padded(vocab) * size;
+  return row < (1l << 22) && rows * row <= MOST_KEPT;
+}
+
+vocab_loss::Sums row_state(const Tensor& state, long rows) {
+  vocab_loss::Sums f{};
+  f.rowm = state.data_ptr<float>();
+  f.rowi = f.rowm + rows;
+  f.ztgt = f.rowi + rows;
+  return f;
 }
 
 void check_shapes(const Tensor& hidden, const Tensor& weight,
@@ -102,10 +146,14 @@ void check_shapes(const Tensor& hidden, const Tensor& weight,
 
 }  // namespace
 
-// -> (loss of every row, total or an undefined tensor, lse, ints)
-std::tuple<Tensor, Tensor, Tensor, Tensor> vocab_loss_forward(
-    Tensor hidden, Tensor weight, Tensor target, std::optional<Tensor> bias,
-    int64_t ignore_index, double eps, bool sum, bool mean) {
+// -> (loss of every row, total or an undefined tensor, state of the kept
+// rows, ints, kept).  kept: what vocab_loss_finish needs, empty where the
+// gradients are left to vocab_loss_backward.
+std::tuple<Tensor, Tensor, Tensor, Tensor, std::vector<std::optional<Tensor>>>
+vocab_loss_forward(Tensor hidden, Tensor weight, Tensor target,
+                   std::optional<Tensor> bias, int64_t ignore_index,
+                   double eps, bool sum, bool mean, bool need_x, bool need_w,
+                   bool need_b) {
   check_shapes(hidden, weight, bias);
   const long rows = hidden.size(0), vocab = weight.size(0);
   TORCH_CHECK(target.device() == hidden.device() && target.dim() == 1 &&
@@ -116,40 +164,32 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> vocab_loss_forward(
               "int64, one for each row, on the same GPU");
   const c10::OptionalDeviceGuard guard(hidden.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
-  const Type type = type_of(hidden);
   const auto f32 = hidden.options().dtype(at::kFloat);
   Tensor ints_t = at::empty({4 + 3 * rows}, f32.dtype(at::kInt));
   const Ints ints(ints_t, rows);
   vocab_loss::scan(target.data_ptr(), target.scalar_type() == at::kLong, rows,
                    ignore_index, vocab, ints.pos, ints.idx, ints.tgt,
                    ints.count, stream);
-  const Operands o = operands(type, hidden, weight, bias, ints, stream);
+  const bool keep = (sum || mean) && (need_x || need_w || need_b) &&
+                    keeps(rows, vocab, (int)hidden.element_size());
+  Call c = make_call(hidden, weight, bias, ints_t, eps, keep);
+  pack(&c, hidden, weight, bias, stream);
+  const auto& plan = c.o.plan;
 
-  vocab_loss::Forward f{};
-  f.plan = vocab_loss::plan(rows, vocab, (int)o.x.size(1),
-                            (int)hidden.element_size());
   Tensor loss = at::empty({rows}, f32);
-  Tensor lse = at::empty({rows}, f32);
-  const long parts = rows * f.plan.tiles;
-  Tensor work = at::empty({rows + parts * (eps != 0.0 ? 3 : 2)}, f32);
-  f.w = o.w.data_ptr();
-  f.x = o.x.data_ptr();
-  f.bias = data_or_null(o.b);
-  f.ldw = o.ldw;
-  f.rows = rows;
-  f.vocab = vocab;
-  f.ldx = (int)o.x.size(1);
-  f.eps = (float)eps;
-  f.pos = ints.pos;
-  f.tgt = ints.tgt;
-  f.count = ints.count;
-  f.ztgt = work.data_ptr<float>();
-  f.pmax = f.ztgt + rows;
-  f.psum = f.pmax + parts;
-  f.pz = f.psum + parts;
-  f.lse = lse.data_ptr<float>();
+  Tensor state = at::empty({3, rows}, f32);
+  const long bands = rows * plan.bands;
+  Tensor work = at::empty({bands * (eps != 0.0 ? 3 : 2)}, f32);
+  vocab_loss::Sums f = row_state(state, rows);
+  f.pmax = work.data_ptr<float>();
+  f.psum = f.pmax + bands;
+  f.pz = f.psum + bands;
   f.loss = loss.data_ptr<float>();
-  vocab_loss::forward(type, f, stream);
+  Tensor grad;
+  if (keep) {
+    grad = at::empty({rows, vocab_loss::padded(vocab)}, hidden.options());
+  }
+  vocab_loss::forward(c.type, c.o, f, data(grad), stream);
 
   Tensor total;
   if (sum || mean) {
@@ -157,74 +197,128 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> vocab_loss_forward(
     vocab_loss::total(f.loss, rows, ints.count, mean,
                       total.data_ptr<float>(), stream);
   }
-  return {loss, total, lse, ints_t};
+  std::vector<std::optional<Tensor>> kept;
+  if (keep) {
+    Tensor small = at::empty({4 + rows}, f32);
+    Tensor dx_slabs, dw, dw_slabs, pbias;
+    if (need_x) {
+      dx_slabs = at::empty({plan.dx_splits, rows, (long)c.o.ldx}, f32);
+    }
+    // fp16 stays in fp32 until the upstream factor, a loss's scale, is known
+    if (need_w && (plan.dw_splits > 1 || c.type == Type::fp16)) {
+      dw_slabs = at::empty({plan.dw_splits, vocab, (long)c.o.ldx}, f32);
+    } else if (need_w) {
+      dw = at::empty({vocab, (long)c.o.dim}, weight.options());
+    }
+    if (need_b) pbias = at::empty({plan.parts, vocab}, f32);
+    vocab_loss::Grads b{};
+    b.scale = small.data_ptr<float>();
+    b.coef = b.scale + 4;
+    b.pbias = floats(pbias);
+    b.dx_slabs = floats(dx_slabs);
+    b.dw_slabs = floats(dw_slabs);
+    b.grad = data(grad);
+    b.dw = data(dw);
+    vocab_loss::coefficients(c.type, c.o, nullptr, false, mean, b, stream);
+    vocab_loss::gradients_kept(c.type, c.o, f, b, stream);
+    for (const Tensor& t : {small, dx_slabs, dw, dw_slabs, pbias}) {
+      kept.push_back(t.defined() ? std::optional<Tensor>(t) : std::nullopt);
+    }
+  }
+  return {loss, total, state, ints_t, kept};
+}
+
+// The gradients that vocab_loss_forward kept, times up; uses them up.
+// -> (dx, dw, db); those not asked for are undefined
+std::tuple<Tensor, Tensor, Tensor> vocab_loss_finish(
+    Tensor up, Tensor hidden, Tensor weight, Tensor ints_t,
+    std::vector<std::optional<Tensor>> kept) {
+  check_shapes(hidden, weight, std::nullopt);
+  TORCH_CHECK(up.device() == hidden.device() && up.numel() == 1 &&
+                  up.scalar_type() == at::kFloat && kept.size() == 5 &&
+                  ints_t.numel() == 4 + 3 * hidden.size(0),
+              "linear_cross_entropy: backward state mismatch");
+  const c10::OptionalDeviceGuard guard(hidden.device());
+  const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
+  Call c = make_call(hidden, weight, std::nullopt, ints_t, 0.0, true);
+  Tensor small = *kept[0], dx, dw, db;
+  Tensor dx_slabs = kept[1].value_or(Tensor());
+  Tensor dw_slabs = kept[3].value_or(Tensor());
+  Tensor pbias = kept[4].value_or(Tensor());
+  if (dx_slabs.defined()) {
+    dx = at::empty({c.o.rows, (long)c.o.dim}, hidden.options());
+  }
+  if (dw_slabs.defined()) {
+    dw = at::empty({c.o.vocab, (long)c.o.dim}, weight.options());
+  } else if (kept[2]) {
+    dw = *kept[2];
+  }
+  if (pbias.defined()) db = at::empty({c.o.vocab}, weight.options());
+  vocab_loss::Grads b{};
+  b.scale = small.data_ptr<float>();
+  b.pbias = floats(pbias);
+  b.part = c.o.plan.part;
+  b.dx_slabs = floats(dx_slabs);
+  b.dw_slabs = floats(dw_slabs);
+  b.dx = data(dx);
+  b.dw = data(dw);
+  b.db = data(db);
+  vocab_loss::finish_kept(c.type, c.o, b, up.data_ptr<float>(), stream);
+  return {dx, dw, db};
 }
 
 // -> (dx, dw, db); those not asked for are undefined
 std::tuple<Tensor, Tensor, Tensor> vocab_loss_backward(
     Tensor up, Tensor hidden, Tensor weight, std::optional<Tensor> bias,
-    Tensor lse, Tensor ints_t, double eps, bool each, bool mean, bool need_x,
-    bool need_w, bool need_b) {
+    Tensor state, Tensor ints_t, double eps, bool each, bool mean,
+    bool need_x, bool need_w, bool need_b) {
   check_shapes(hidden, weight, bias);
   const long rows = hidden.size(0), vocab = weight.size(0);
-  const int dim = (int)hidden.size(1);
   TORCH_CHECK(up.device() == hidden.device() &&
                   up.scalar_type() == at::kFloat && up.is_contiguous() &&
                   up.numel() == (each ? rows : 1) &&
-                  lse.numel() == rows && ints_t.numel() == 4 + 3 * rows,
+                  state.numel() == 3 * rows &&
+                  ints_t.numel() == 4 + 3 * rows,
               "linear_cross_entropy: backward state mismatch");
   const c10::OptionalDeviceGuard guard(hidden.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
-  const Type type = type_of(hidden);
   const auto f32 = hidden.options().dtype(at::kFloat);
-  const Ints ints(ints_t, rows);
-  const Operands o = operands(type, hidden, weight, bias, ints, stream);
-  const int ldx = (int)o.x.size(1);
+  Call c = make_call(hidden, weight, bias, ints_t, eps, false);
+  pack(&c, hidden, weight, bias, stream);
+  const auto& plan = c.o.plan;
+  const long dim = c.o.dim, ldx = c.o.ldx;
 
-  vocab_loss::Backward b{};
-  b.plan = vocab_loss::plan(rows, vocab, ldx, (int)hidden.element_size());
-  b.piece = b.plan.piece;
-  b.dx_splits = b.plan.dx_splits;
-  b.dw_splits = b.plan.dw_splits;
-  Tensor dx, dw, db;
-  if (need_x) dx = at::empty({rows, dim}, hidden.options());
-  if (need_w) dw = at::empty({vocab, dim}, weight.options());
-  if (need_b) db = at::empty({vocab}, weight.options());
+  Tensor dx, dw, db, pbias, dx_slabs, dw_slabs;
+  if (need_x) {
+    dx = at::empty({rows, dim}, hidden.options());
+    dx_slabs = at::empty({plan.dx_splits, rows, ldx}, f32);
+  }
+  if (need_w) {
+    dw = at::empty({vocab, dim}, weight.options());
+    if (plan.dw_splits > 1) {
+      dw_slabs = at::empty({plan.dw_splits, plan.piece, ldx}, f32);
+    }
+  }
+  if (need_b) {
+    db = at::empty({vocab}, weight.options());
+    pbias = at::empty({plan.parts, vocab}, f32);
+  }
   Tensor small = at::empty({4 + rows}, f32);
+  Tensor grad =
+      at::empty({rows, vocab_loss::padded(plan.piece)}, hidden.options());
+  vocab_loss::Grads b{};
   b.scale = small.data_ptr<float>();
   b.coef = b.scale + 4;
-  Tensor grad =
-      at::empty({rows, (long)padded(b.piece)}, hidden.options());
-  Tensor pbias, dx_slabs, dw_slabs;
-  if (need_b) pbias = at::empty({b.plan.row_tiles, vocab}, f32);
-  if (need_x) dx_slabs = at::empty({b.dx_splits, rows, (long)ldx}, f32);
-  if (need_w && b.dw_splits > 1) {
-    dw_slabs = at::empty({b.dw_splits, b.piece, (long)ldx}, f32);
-  }
-  b.w = o.w.data_ptr();
-  b.x = o.x.data_ptr();
-  b.bias = data_or_null(o.b);
-  b.ldw = o.ldw;
-  b.rows = rows;
-  b.vocab = vocab;
-  b.ldx = ldx;
-  b.dim = dim;
-  b.eps = (float)eps;
-  b.pos = ints.pos;
-  b.idx = ints.idx;
-  b.tgt = ints.tgt;
-  b.count = ints.count;
-  b.lse = lse.data_ptr<float>();
-  b.up = up.data_ptr<float>();
-  b.each = each;
-  b.mean = mean;
-  b.pbias = need_b ? pbias.data_ptr<float>() : nullptr;
-  b.dx_slabs = need_x ? dx_slabs.data_ptr<float>() : nullptr;
-  b.dw_slabs = dw_slabs.defined() ? dw_slabs.data_ptr<float>() : nullptr;
-  b.grad = grad.data_ptr();
-  b.dx = need_x ? dx.data_ptr() : nullptr;
-  b.dw = need_w ? dw.data_ptr() : nullptr;
-  b.db = need_b ? db.data_ptr() : nullptr;
-  vocab_loss::backward(type, b, stream);
+  b.pbias = floats(pbias);
+  b.part = plan.part;
+  b.dx_slabs = floats(dx_slabs);
+  b.dw_slabs = floats(dw_slabs);
+  b.grad = data(grad);
+  b.dx = data(dx);
+  b.dw = data(dw);
+  b.db = data(db);
+  vocab_loss::coefficients(c.type, c.o, up.data_ptr<float>(), each, mean, b,
+                           stream);
+  vocab_loss::gradients_again(c.type, c.o, row_state(state, rows), b, stream);
   return {dx, dw, db};
 }

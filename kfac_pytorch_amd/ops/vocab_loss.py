@@ -11,9 +11,11 @@ tensors of their own.
               - eps / V sum_v z[n, v]
 
 On the GPU, hand-written MFMA kernels (``csrc/vocab_loss.hip``) make the logits
-tile by tile in registers; the backward pass makes them once more, piece by
-piece of the vocabulary, in the inputs' type.  Sums, losses and the log-sum-exp
-are fp32.  On the CPU the plain expression above runs.
+tile by tile in registers.  Where gradients are asked for, the forward pass of
+a reduced loss computes them in the same go; otherwise the backward pass makes
+the logits once more, piece by piece of the vocabulary.  Products are of the
+inputs' type, sums, losses and the log-sum-exp fp32.  On the CPU the plain
+expression above runs.
 """
 
 from __future__ import annotations
@@ -30,13 +32,22 @@ _TYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
 class _VocabLoss(torch.autograd.Function):
+    """A reduced loss leaves its gradients for an upstream factor of 1, which
+    the first backward pass uses up; a loss of single rows, a second backward
+    pass, or a call too large to keep its probabilities makes the logits
+    again."""
+
     @staticmethod
     def forward(ctx, hidden, weight, bias, target, ignore_index, eps,
                 reduction):
         from kfac_pytorch_amd.ops import _ext
-        loss, total, lse, ints = _ext.vocab_loss_forward(
-            hidden, weight, target, bias, ignore_index, eps, reduction)
-        ctx.save_for_backward(hidden, weight, bias, lse, ints)
+        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1],
+                bias is not None and ctx.needs_input_grad[2])
+        loss, total, state, ints, kept = _ext.vocab_loss_forward(
+            hidden, weight, target, bias, ignore_index, eps, reduction, need)
+        ctx.save_for_backward(hidden, weight, bias, state, ints)
+        ctx.kept = kept
+        ctx.need = need
         ctx.eps = eps
         ctx.reduction = reduction
         return loss if reduction == "none" else total
@@ -45,11 +56,16 @@ class _VocabLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, up):
         from kfac_pytorch_amd.ops import _ext
-        hidden, weight, bias, lse, ints = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        dx, dw, db = _ext.vocab_loss_backward(
-            up.contiguous(), hidden, weight, bias, lse, ints, ctx.eps,
-            ctx.reduction, need[0], need[1], need[2] and bias is not None)
+        hidden, weight, bias, state, ints = ctx.saved_tensors
+        up = up.contiguous()
+        kept, ctx.kept = ctx.kept, None
+        if kept:
+            dx, dw, db = _ext.vocab_loss_finish(up, hidden, weight, ints,
+                                                kept)
+        else:
+            dx, dw, db = _ext.vocab_loss_backward(
+                up, hidden, weight, bias, state, ints, ctx.eps,
+                ctx.reduction, ctx.need)
         return dx, dw, db, None, None, None, None
 
 
@@ -107,7 +123,13 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
     floating arguments are cast as ``F.linear`` casts them.  A target outside
     the vocabulary raises on the CPU; on the GPU, where raising would mean to
     wait for the device, that row's loss and the gradients become NaN.
-    Gradients can be taken once (no double backward).
+    There is no double backward.
+
+    On the GPU a reduced loss computes its gradients in the forward pass if
+    any is asked for (evaluate under ``torch.no_grad()``).  Memory: the
+    gradients, and while the call lasts rows x V values of the inputs' type
+    if that is 4 GiB at most; else, and for ``"none"``, 256 MB pieces of it
+    during the backward pass.
     """
     _check(hidden, weight, target, bias, label_smoothing, reduction)
     kind = hidden.device.type
@@ -152,7 +174,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
                                 float(label_smoothing), reduction)
     else:
         from kfac_pytorch_amd.ops import _ext
-        loss, total, _, _ = _ext.vocab_loss_forward(
+        loss, total, _, _, _ = _ext.vocab_loss_forward(
             rows, weight, flat, bias, int(ignore_index),
             float(label_smoothing), reduction)
         loss = loss if reduction == "none" else total

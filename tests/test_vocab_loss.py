@@ -6,9 +6,11 @@ fp16 2^-11, fp32 2^-24).  With S = sum_d |x||w| + |b|:
 * a logit's fp32 sum over d terms is off by at most about (d + 2) 2^-24 S, and
   a loss is a difference and a log-sum of logits: two logits' error, plus the
   exponentials' (a few 2^-23) and the rounding of the loss itself.
-* g = c (p - y) is p times (1 + that error), rounded once to the inputs' type
-  (fp32: not at all); a gradient is a sum of products of g, off by
-  (u + logit error + terms 2^-24) sum |g||w|, plus u of its own rounding.
+* g = c (p - y) is p times (1 + that error), rounded to the inputs' type (fp32:
+  not at all) -- twice where the powers were kept in it: p by u, then g by u;
+  a gradient is a sum of products of g, off by (2u + logit error + terms
+  2^-24) sum (|g| + c eps / V) |w|, plus u of its own rounding, and for dw
+  once more, where an upstream factor comes after it.
 """
 
 import math
@@ -89,13 +91,14 @@ def check_all(ref, loss, grads, x, w, b, dtype, rows, lift=0.0):
     # the smallest steps of fp16 and of exp's flush to zero
     tiny = 2.0 ** -24 if dtype == torch.float16 else 2.0 ** -120
     round_g = 0.0 if dtype == torch.float32 else u
-    # p = exp(z - lse) is off by the logits' error times p; off the target p
-    # is at most |g| / c + eps / V, at the target at most 1
+    # p = exp(z - lse) is off by the logits' error times p, and by u p where
+    # the powers are kept in the inputs' type; off the target p is at most
+    # |g| / c + eps / V; at the target, always made from fp32, at most 1
     gabs = ref["g"].abs()
     rel = round_g + 8 * 2.0 ** -24
     wa, xa = w.double().cpu().abs(), x.double().cpu().abs()
     xa = torch.where(ref["keep"][:, None], xa, torch.zeros(()).double())
-    p_err = e * (gabs + ref["share"] * ref["c"][:, None])
+    p_err = (e + round_g) * (gabs + ref["share"] * ref["c"][:, None])
     at_target = e * ref["c"]
     sx = rel * ref["sx"] + p_err @ wa + (2 * at_target)[:, None] * wa.amax(0)
     sw = rel * ref["sw"] + p_err.t() @ xa \
@@ -104,7 +107,7 @@ def check_all(ref, loss, grads, x, w, b, dtype, rows, lift=0.0):
     check("dx", grads[0], ref["dx"], sx + (vocab + 8) * terms * ref["sx"]
           + u * ref["dx"].abs() + sx * u + tiny)
     check("dw", grads[1], ref["dw"], sw + (rows + 8) * terms * ref["sw"]
-          + u * ref["dw"].abs() + sw * u + tiny)
+          + 2 * u * ref["dw"].abs() + 2 * sw * u + tiny)
     if b is not None:
         sb = 8 * 2.0 ** -24 * ref["sb"] + p_err.sum(0) + 2 * at_target.max()
         check("db", grads[2], ref["db"], sb + (rows + 8) * terms * ref["sb"]
@@ -177,6 +180,52 @@ def test_wide_tiles(rows, dim, vocab, dtype):
     loss, grads = run(x, w, b, t, 0.05, "none", up)
     check_all(formula(x, w, b, t, 0.05, up), loss, grads, x, w, b, dtype,
               rows)
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_pieces_of_the_vocabulary():
+    """Single rows' losses beyond 256 MB of g: two pieces, against the whole
+    call with the same factors kept."""
+    rows, dim, vocab = 4100, 16, 17000
+    x, w, b, t = inputs(rows, dim, vocab, torch.float32, True, 0.1, 21)
+    assert rows * vocab * 4 > 256 << 20
+    up = torch.ones(rows, device="cuda")
+    loss, grads = run(x, w, b, t, 0.1, "none", up)
+    total, kept = run(x, w, b, t, 0.1, "sum")
+    # fp32: two orders of summation of the same g
+    z = (x.double() @ w.double().t() + b.double())
+    z = (z - torch.logsumexp(z, 1, keepdim=True)).exp()
+    size = z @ w.double().abs() + w.double().abs()[t.clamp(min=0)] + 1
+    bound = (vocab + 64) * 2.0 ** -24 * size
+    assert ((grads[0].double() - kept[0].double()).abs() <= bound).all()
+    count = torch.bincount(t[t >= 0], minlength=vocab)[:, None]
+    size = (z.t() @ x.double().abs()) + (count + 1) * x.double().abs().amax(0)
+    bound = (rows + 64) * 2.0 ** -24 * size
+    assert ((grads[1].double() - kept[1].double()).abs() <= bound).all()
+    size = z.sum(0) + count.squeeze(1) + 1
+    bound = (rows + 64) * 2.0 ** -24 * size
+    assert ((grads[2].double() - kept[2].double()).abs() <= bound).all()
+    assert abs(float(loss.double().sum() - total)) <= 2e-6 * float(total)
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("dtype", list(HALF), ids=["bf16", "fp16", "fp32"])
+def test_backward_twice(dtype):
+    """The first backward pass uses up what the forward pass kept; the second
+    makes it again."""
+    x, w, b, t = inputs(90, 64, 300, dtype, True, 0.2, 31)
+    leaves = [a.requires_grad_() for a in (x, w, b)]
+    loss = ops.linear_cross_entropy(x, w, t, bias=b, reduction="sum")
+    up = torch.tensor(2.5, device="cuda")
+    first = torch.autograd.grad(loss, leaves, up, retain_graph=True)
+    second = torch.autograd.grad(loss, leaves, up)
+    ref = formula(x.detach(), w.detach(), b.detach(), t, 0.0,
+                  torch.full((90,), 2.5))
+    for grads in (first, second):
+        check_all(ref, None, grads, x.detach(), w.detach(), b.detach(),
+                  dtype, 90)
 
 
 @pytest.mark.gpu
