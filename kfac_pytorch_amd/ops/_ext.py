@@ -181,10 +181,11 @@ def vocab_loss_forward(hidden, weight, target, bias, ignore_index: int,
                                       reduction == "mean", *need)
 
 
-def vocab_loss_finish(up, hidden, weight, ints, kept):
+def vocab_loss_finish(up, hidden, weight, ints, reduction: str, kept):
     """(d hidden, d weight, d bias) from what the forward pass kept, which is
     used up; None for those not asked for."""
-    return _load().vocab_loss_finish(up, hidden, weight, ints, kept)
+    return _load().vocab_loss_finish(up, hidden, weight, ints,
+                                     reduction == "mean", kept)
 
 
 def vocab_loss_backward(up, hidden, weight, bias, state, ints, eps: float,

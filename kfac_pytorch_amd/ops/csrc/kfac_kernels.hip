@@ -433,7 +433,8 @@ vocab_loss_forward(torch::Tensor hidden, torch::Tensor weight,
                    bool need_x, bool need_w, bool need_b);
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> vocab_loss_finish(
     torch::Tensor up, torch::Tensor hidden, torch::Tensor weight,
-    torch::Tensor ints, std::vector<std::optional<torch::Tensor>> kept);
+    torch::Tensor ints, bool mean,
+    std::vector<std::optional<torch::Tensor>> kept);
 std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> vocab_loss_backward(
     torch::Tensor up, torch::Tensor hidden, torch::Tensor weight,
     std::optional<torch::Tensor> bias, torch::Tensor state,

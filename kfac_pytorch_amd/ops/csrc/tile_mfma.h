@@ -339,6 +339,45 @@ __device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
   arrive();
 }
 
+// Writes 16 columns of a wave's part of C, ROWS rows each, as rows of memory:
+// out[j * ld + c] for column j and row c.  A lane holds 4 neighbouring rows of
+// one column, v[ROWS / 16][4]; written from there, a store would be pieces of
+// 32 bytes.  They go through LDS (`lds`, the wave's own, ROWS * 16 values) and
+// leave as whole rows, 16 bytes a lane.  `cols` columns and `rows` rows exist
+// (rows a multiple of a chunk, out and ld aligned to 16 bytes).
+template <class T, int ROWS>
+__device__ __forceinline__ void store_columns(const T (&v)[ROWS / 16][4],
+                                              char* lds, T* out, long ld,
+                                              int cols, int rows, int lane) {
+  constexpr int E = 16 / sizeof(T), CH = ROWS / E, LINE = ROWS * sizeof(T);
+  constexpr int EACH = 64 / CH > 0 ? 64 / CH : 1;  // columns at a time
+  static_assert(CH <= 64 && 16 % EACH == 0, "a column is at most one store");
+  struct alignas(16) Chunk {
+    T v[E];
+  };
+  const int i = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int m = 0; m < ROWS / 16; ++m) {
+    const int at = m * 16 + g * 4;
+    __builtin_memcpy(lds + i * LINE + (((at / E) ^ (i & (CH - 1))) * 16) +
+                         (at % E) * sizeof(T),
+                     v[m], 4 * sizeof(T));
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int q = 0; q < 16 / EACH; ++q) {
+    const int j = q * EACH + lane / CH, c = lane % CH;
+    const Chunk t = *reinterpret_cast<const Chunk*>(
+        lds + j * LINE + ((c ^ (j & (CH - 1))) * 16));
+    if (j < cols && c * E < rows) {
+      *reinterpret_cast<Chunk*>(out + (long)j * ld + c * E) = t;
+    }
+  }
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // Which tile a workgroup takes.  Workgroups go to the 8 XCDs in turn; each
 // XCD has an L2 of its own, so each gets one run of neighbouring tiles, and a
 // run walks 8 tiles of m for each tile of n before the next n.

@@ -47,12 +47,13 @@ struct Operands {
 struct Sums {
   float *pmax, *psum, *pz;             // [row][band]
   float *rowm, *rowi, *ztgt, *loss;    // [row]
+  float* total;
 };
 
 struct Grads {
   float *coef, *scale, *pbias, *dx_slabs, *dw_slabs;
   void *grad, *dx, *dw, *db;
-  int part;
+  bool mean;
 };
 
 void scan(const void* target, bool wide_ints, long rows, long ignore,
@@ -66,9 +67,10 @@ void forward(Type t, const Operands& o, const Sums& f, void* grad,
              hipStream_t s);
 void total(const float* loss, long rows, const int* count, bool mean,
            float* out, hipStream_t s);
-// up: one value, one for each row (`each`), or null for 1
+// up: one value, or one for each row (`each`)
 void coefficients(Type t, const Operands& o, const float* up, bool each,
-                  bool mean, const Grads& b, hipStream_t s);
+                  const Grads& b, hipStream_t s);
+// these also write f.total
 void gradients_kept(Type t, const Operands& o, const Sums& f, const Grads& b,
                     hipStream_t s);
 void finish_kept(Type t, const Operands& o, const Grads& b, const float* up,

@@ -78,35 +78,56 @@ constexpr float LIFT<_Float16> = 32768.f;
 // ------------------------------------------------------- kept rows, one block
 // pos[n]: the row's place among the kept ones, or -1; idx, tgt: the kept rows'
 // numbers and targets, BAD for a target outside [0, vocab).
-constexpr int SCAN = 1024;
+constexpr int SCAN = 1024;   // threads
+constexpr int EACH = 8;      // targets of a thread in flight
 
 template <class I>
 __global__ __launch_bounds__(SCAN) void scan_kernel(
     const I* __restrict__ target, long rows, long ignore, long vocab,
     int* __restrict__ pos, int* __restrict__ idx, int* __restrict__ tgt,
     int* __restrict__ count) {
-  __shared__ int sums[SCAN / 64];
+  constexpr int WAVES = SCAN / 64, PARTS = WAVES * EACH;  // 128 counts
+  __shared__ int sums[PARTS];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   int done = 0;
-  for (long base = 0; base < rows; base += SCAN) {
-    const long n = base + t;
-    const long v = n < rows ? (long)target[n] : ignore;
-    const bool keep = n < rows && v != ignore;
-    const unsigned long long mask = __ballot(keep);
-    if (lane == 0) sums[wave] = __popcll(mask);
-    __syncthreads();
-    int before = done, all = 0;
+  for (long base = 0; base < rows; base += SCAN * EACH) {
+    long v[EACH];
+    unsigned long long mask[EACH];
 #pragma unroll
-    for (int w = 0; w < SCAN / 64; ++w) {
-      const int s = sums[w];
-      before += w < wave ? s : 0;
-      all += s;
+    for (int k = 0; k < EACH; ++k) {
+      const long n = base + k * SCAN + t;
+      v[k] = n < rows ? (long)target[n] : ignore;
     }
-    const int at = before + __popcll(mask & ((1ull << lane) - 1));
-    if (n < rows) pos[n] = keep ? at : -1;
-    if (keep) {
-      idx[at] = (int)n;
-      tgt[at] = (v >= 0 && v < vocab) ? (int)v : BAD;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      mask[k] = __ballot(v[k] != ignore);
+      if (lane == 0) sums[k * WAVES + wave] = __popcll(mask[k]);
+    }
+    __syncthreads();
+    // every wave scans the counts: exclusive sums of pairs of them
+    const int a = sums[2 * lane], b = sums[2 * lane + 1];
+    int s = a + b;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(s, d);
+      s += lane >= d ? o : 0;
+    }
+    const int all = __shfl(s, 63);
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      const int part = k * WAVES + wave;
+      const int end = __shfl(s, part >> 1), first = __shfl(a, part >> 1),
+                second = __shfl(b, part >> 1);
+      const int before =
+          done + end - second - (part & 1 ? 0 : first);
+      const long n = base + k * SCAN + t;
+      const bool keep = v[k] != ignore;
+      const int at = before + __popcll(mask[k] & ((1ull << lane) - 1));
+      if (n < rows) pos[n] = keep ? at : -1;
+      if (keep) {
+        idx[at] = (int)n;
+        tgt[at] = (v[k] >= 0 && v[k] < vocab) ? (int)v[k] : BAD;
+      }
     }
     done += all;
     __syncthreads();
@@ -226,6 +247,8 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
     }
   }
   const bool whole = m0 + S::BM <= p.vocab;
+  char* stage = smem + wave * (2 * S::MI * 256 * sizeof(T));
+  static_assert(S::NW * 2 * S::MI * 256 * sizeof(T) <= S::LDS, "LDS");
 
   if constexpr (MODE != AGAIN) {
     float zs[S::NI];
@@ -280,21 +303,21 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
       const float ref = safe(m);
       const int n = nbase + ni * 16;
       float s = 0.f;
+      T out[S::MI][4];
 #pragma unroll
       for (int mi = 0; mi < S::MI; ++mi) {
-        T out[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float e = power(acc[mi][ni][r], ref);
           s += e;
-          out[r] = (T)(e * LIFT<T>);
+          out[mi][r] = (T)(e * LIFT<T>);
         }
-        if constexpr (MODE == KEEP) {
-          const int v = vbase + mi * 16;
-          if (n < rows && v < p.ldg) {
-            __builtin_memcpy(grad + (long)n * p.ldg + v, out, sizeof(out));
-          }
-        }
+      }
+      if constexpr (MODE == KEEP) {
+        tile::store_columns<T, S::MI * 16>(
+            out, stage + (ni & 1) * (S::MI * 256 * sizeof(T)),
+            grad + (long)(n0 + wcol + ni * 16) * p.ldg + m0 + wrow, p.ldg,
+            rows - (n0 + wcol + ni * 16), (int)p.ldg - (m0 + wrow), lane);
       }
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
@@ -354,21 +377,24 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
         }
       }
     }
-    float* red = reinterpret_cast<float*>(smem);
 #pragma unroll
-    for (int mi = 0; mi < S::MI; ++mi) {
-      const int v = vbase + mi * 16;
+    for (int ni = 0; ni < S::NI; ++ni) {
+      T out[S::MI][4];
 #pragma unroll
-      for (int ni = 0; ni < S::NI; ++ni) {
-        const int n = nbase + ni * 16;
-        T out[4];
+      for (int mi = 0; mi < S::MI; ++mi) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) out[r] = (T)acc[mi][ni][r];
-        if (n < rows && v < p.ldg) {
-          __builtin_memcpy(grad + (long)n * p.ldg + v, out, sizeof(out));
-        }
+        for (int r = 0; r < 4; ++r) out[mi][r] = (T)acc[mi][ni][r];
       }
-      if (p.pbias) {  // summed before the rounding
+      tile::store_columns<T, S::MI * 16>(
+          out, stage + (ni & 1) * (S::MI * 256 * sizeof(T)),
+          grad + (long)(n0 + wcol + ni * 16) * p.ldg + m0 + wrow, p.ldg,
+          rows - (n0 + wcol + ni * 16), (int)p.ldg - (m0 + wrow), lane);
+    }
+    if (p.pbias) {  // summed before the rounding
+      __syncthreads();
+      float* red = reinterpret_cast<float*>(smem);
+#pragma unroll
+      for (int mi = 0; mi < S::MI; ++mi) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           float s = 0.f;
@@ -385,8 +411,6 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
           }
         }
       }
-    }
-    if (p.pbias) {
       __syncthreads();
       for (int q = threadIdx.x; q < S::BM; q += S::THREADS) {
         if (m0 + q >= p.vocab) continue;
@@ -416,56 +440,129 @@ __global__ __launch_bounds__(256) void join_kernel(
     return;
   }
   const long at = (long)p * bands;
-  float m = -INFINITY;
-  for (int k = lane; k < bands; k += 64) m = fmaxf(m, pmax[at + k]);
-  m = safe(wave_max(m));
-  float s = 0.f, z = 0.f;
-  for (int k = lane; k < bands; k += 64) {
-    s = fmaf(psum[at + k], __builtin_amdgcn_exp2f(safe(pmax[at + k]) - m), s);
-    if (pz) z += pz[at + k];
+  constexpr int U = 8;  // bands of a lane in flight
+  float m = -INFINITY, s = 0.f, z = 0.f;
+  for (int base = lane; base < bands; base += 64 * U) {
+    float a[U], b[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const int k = base + 64 * j;
+      a[j] = k < bands ? pmax[at + k] : -INFINITY;
+      b[j] = k < bands ? psum[at + k] : 0.f;
+      if (pz) z += k < bands ? pz[at + k] : 0.f;
+    }
+    float top = m;
+#pragma unroll
+    for (int j = 0; j < U; ++j) top = fmaxf(top, a[j]);
+    s *= __builtin_amdgcn_exp2f(m - safe(top));
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      s = fmaf(b[j], __builtin_amdgcn_exp2f(a[j] - safe(top)), s);
+    }
+    m = top;
   }
-  s = wave_sum(s);
+  const float top = safe(wave_max(m));
+  s = wave_sum(s * __builtin_amdgcn_exp2f(m - top));
   z = wave_sum(z);
   if (lane == 0) {
-    rowm[p] = m;
-    rowi[p] = 1.f / s;
+    const bool bad = tgt[p] == BAD;
+    rowm[p] = top;
+    rowi[p] = bad ? NAN : 1.f / s;
     // the powers are of the rounded log2(e): dividing by it undoes that
-    double v = ((double)m + log2((double)s)) / (double)LOG2E -
+    double v = ((double)top + log2((double)s)) / (double)LOG2E -
                (1.0 - (double)eps) * (double)ztgt[p];
     if (pz) v -= (double)share * (double)z;
-    loss[n] = tgt[p] == BAD ? NAN : (float)v;
+    loss[n] = bad ? NAN : (float)v;
   }
 }
 
+// The sum of all losses (/ count for the mean), by one workgroup of any size,
+// in a fixed order.
+__device__ __forceinline__ void total_body(const float* loss, long rows,
+                                           int count, bool mean,
+                                           float* total) {
+  __shared__ double part[16];
+  double s = 0.0;
+  for (long n = threadIdx.x; n < rows; n += blockDim.x) s += (double)loss[n];
+#pragma unroll
+  for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    double t = 0.0;
+    for (unsigned k = 0; k < blockDim.x >> 6; ++k) t += part[k];
+    *total = (float)(mean ? t / (double)count : t);
+  }
+}
+
+__global__ __launch_bounds__(1024) void total_kernel(
+    const float* __restrict__ loss, long rows, const int* __restrict__ count,
+    int mean, float* __restrict__ total) {
+  total_body(loss, rows, *count, mean, total);
+}
+
+// ------------------------------------------------------ factors and scales
+// d(total)/d(loss) of a row is one (mean: 1 / count) times the upstream
+// factor.  fp16 holds g to 6e-8 only, and 1 / count times a small probability
+// is soon below that: there g is made with the factor brought to [2^14, 2^15)
+// by a power of two (|g| is at most the factor, and the type ends at 65504),
+// and the products are scaled back in fp32.
+struct Factor {
+  const float* scale;  // [1]: the inverse of that power, or null: from count
+  const int* count;
+  bool mean, lift;
+
+  __device__ __forceinline__ int exponent(float one) const {
+    return lift ? 14 - (((int)__float_as_uint(one) >> 23) - 127) : 0;
+  }
+  __device__ __forceinline__ float one() const {
+    return mean ? 1.f / (float)*count : 1.f;
+  }
+  // with the power of two
+  __device__ __forceinline__ float lifted() const {
+    return ldexpf(one(), exponent(one()));
+  }
+  __device__ __forceinline__ float inverse() const {
+    if (scale) return scale[1];
+    return *count > 0 ? ldexpf(1.f, -exponent(one())) : 1.f;
+  }
+};
+
 // ------------------------------------------------- g from the kept powers
 // In place: g = c (power 2^(band - row) / sum - eps / V), the target's entry
-// anew from its z.  A workgroup takes PROWS tokens, a lane one 16-byte chunk
-// of each of them, and sums the bias gradient down the rows in passing.
-constexpr int PROWS = 64;
-
+// anew from its z.  A workgroup takes `part` tokens, a lane one 16-byte chunk
+// of each of them, and sums the bias gradient down the rows in passing; one
+// more workgroup adds up the losses.  Bound by memory: 16 tokens a workgroup
+// where there would be too few of them otherwise.
 template <class T>
 __global__ __launch_bounds__(256) void probs_kernel(
-    T* __restrict__ grad, long ldg, int vocab, const int* __restrict__ count,
+    T* __restrict__ grad, long ldg, int vocab, int part,
     const int* __restrict__ tgt, const float* __restrict__ pmax, int bands,
     int band, const float* __restrict__ rowm, const float* __restrict__ rowi,
-    const float* __restrict__ ztgt, const float* __restrict__ coef, float eps,
-    float share, float* __restrict__ pbias) {
+    const float* __restrict__ ztgt, const Factor factor, float eps,
+    float share, float* __restrict__ pbias, const float* __restrict__ loss,
+    long all, float* __restrict__ total) {
   constexpr int E = 16 / sizeof(T);
-  const int rows = *count;
-  const int n0 = blockIdx.x * PROWS;
+  const int rows = *factor.count;
+  if (blockIdx.x == gridDim.x - 1) {
+    if (blockIdx.y == 0) total_body(loss, all, rows, factor.mean, total);
+    return;
+  }
+  const int n0 = blockIdx.x * part;
   const int v = (blockIdx.y * 256 + threadIdx.x) * E;
   if (n0 >= rows || v >= ldg) return;
-  const int n1 = rows - n0 < PROWS ? rows : n0 + PROWS;
+  const int n1 = rows - n0 < part ? rows : n0 + part;
   const int mine = v / band;
+  const float c = factor.lifted();
   float sum[E] = {};
-#pragma unroll 4
+#pragma unroll 8
   for (int n = n0; n < n1; ++n) {
     struct alignas(16) Chunk {
       T v[E];
     };
     Chunk* at = reinterpret_cast<Chunk*>(grad + (long)n * ldg + v);
     Chunk t = *at;
-    const float c = coef[n], m = rowm[n], i = rowi[n];
+    const float m = rowm[n], i = rowi[n];
     const float k = __builtin_amdgcn_exp2f(safe(pmax[(long)n * bands + mine]) -
                                            m) * i * c * (1.f / LIFT<T>);
     const int hit = tgt[n] - v;
@@ -487,30 +584,9 @@ __global__ __launch_bounds__(256) void probs_kernel(
   }
 }
 
-// one block, in a fixed order: total = sum of loss (/ count for the mean)
-__global__ __launch_bounds__(1024) void total_kernel(
-    const float* __restrict__ loss, long rows, const int* __restrict__ count,
-    int mean, float* __restrict__ total) {
-  __shared__ double part[16];
-  double s = 0.0;
-  for (long n = threadIdx.x; n < rows; n += 1024) s += (double)loss[n];
-#pragma unroll
-  for (int k = 32; k > 0; k >>= 1) s += __shfl_xor(s, k);
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = s;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double t = 0.0;
-    for (int k = 0; k < 16; ++k) t += part[k];
-    *total = (float)(mean ? t / (double)*count : t);
-  }
-}
-
 // ---------------------------------------------------------- row coefficients
-// coef[i] = d(total)/d(loss of kept row i) times a power of two, scale[0];
-// scale[1] is its inverse.  Without `up` the upstream factor is 1.  fp16 holds g to 6e-8 only, and c_n = 1/rows times
-// a small probability is soon below that: there the largest |c_n| is brought
-// to [2^14, 2^15) (|g| <= |c_n|, and the type ends at 65504) and the products
-// are scaled back in fp32.
+// coef[i] = the factor of kept row i times the power of two, scale[0];
+// scale[1] is its inverse.
 __global__ __launch_bounds__(1024) void coef_kernel(
     const float* __restrict__ up, int each, int mean,
     const int* __restrict__ idx, const int* __restrict__ tgt,
@@ -519,8 +595,7 @@ __global__ __launch_bounds__(1024) void coef_kernel(
   __shared__ float part[16];
   __shared__ float shared_scale;
   const int rows = *count;
-  const float first = up && !each ? *up : 1.f;
-  const float one = mean ? first / (float)rows : first;
+  const float one = each ? 1.f : (mean ? *up / (float)rows : *up);
   float top = 0.f;
   if (lift) {
     if (each) {
@@ -552,25 +627,6 @@ __global__ __launch_bounds__(1024) void coef_kernel(
     const float c = (each ? up[idx[i]] : one) * shared_scale;
     coef[i] = tgt[i] == BAD ? NAN : c;
   }
-}
-
-// what the products are multiplied by at the end
-__device__ __forceinline__ float factor(const float* scale, const float* up) {
-  return scale[1] * (up ? *up : 1.f);
-}
-
-template <class T>
-__global__ void bias_kernel(const float* __restrict__ pbias, long vocab,
-                            int part, const int* __restrict__ count,
-                            const float* __restrict__ scale,
-                            const float* __restrict__ up,
-                            T* __restrict__ out) {
-  const long v = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (v >= vocab) return;
-  const int parts = (*count + part - 1) / part;  // of `part` tokens
-  float s = 0.f;
-  for (int k = 0; k < parts; ++k) s += pbias[(long)k * vocab + v];
-  out[v] = (T)(s * factor(scale, up));
 }
 
 // ------------------------------------------------------------- dx += g w
@@ -610,74 +666,14 @@ __global__ __launch_bounds__(S::THREADS) void dx_kernel(
   }
 }
 
-// Adds slabs of fp32 rows (ldim values, a multiple of 4) into rows of `dim`
-// values of T.  pos: which slab row a row takes, none (zeros) for -1.
-template <class T>
-__global__ __launch_bounds__(256) void add_kernel(
-    const float* __restrict__ slabs, long slab, int splits, int ldim, int dim,
-    long rows, const int* __restrict__ pos, const float* __restrict__ scale,
-    const float* __restrict__ up, T* __restrict__ out) {
-  const float f = factor(scale, up);
-  const int groups = (dim + 3) / 4;
-  const long total = rows * groups;
-  for (long k = (long)blockIdx.x * blockDim.x + threadIdx.x; k < total;
-       k += (long)gridDim.x * blockDim.x) {
-    const long n = k / groups;
-    const int d = (int)(k - n * groups) * 4;
-    const long p = pos ? pos[n] : n;
-    f32x4 s = {};
-    if (p >= 0) {
-      const float* at = slabs + p * ldim + d;
-#pragma unroll 8
-      for (int j = 0; j < splits; ++j) {
-        s += *reinterpret_cast<const f32x4*>(at + j * slab);
-      }
-    }
-    T o[4];
-#pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = (T)(s[r] * f);
-    if (d + 4 <= dim) {
-      __builtin_memcpy(out + n * dim + d, o, sizeof(o));
-    } else {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (d + r < dim) out[n * dim + d + r] = o[r];
-      }
-    }
-  }
-}
-
-// out *= up, where that changes anything; out is 16-byte aligned
-template <class T>
-__global__ __launch_bounds__(256) void times_kernel(
-    T* __restrict__ out, long n, const float* __restrict__ up) {
-  const float f = *up;
-  if (f == 1.f) return;
-  constexpr int E = 16 / sizeof(T);
-  struct alignas(16) Chunk {
-    T v[E];
-  };
-  for (long k = (long)blockIdx.x * blockDim.x + threadIdx.x; k * E < n;
-       k += (long)gridDim.x * blockDim.x) {
-    if ((k + 1) * E <= n) {
-      Chunk c = reinterpret_cast<Chunk*>(out)[k];
-#pragma unroll
-      for (int j = 0; j < E; ++j) c.v[j] = (T)((float)c.v[j] * f);
-      reinterpret_cast<Chunk*>(out)[k] = c;
-    } else {
-      for (long j = k * E; j < n; ++j) out[j] = (T)((float)out[j] * f);
-    }
-  }
-}
-
 // ------------------------------------------------------------- dw = g^T x
 // Rows of the tile are hidden units, columns vocabulary entries, k tokens.
 template <class T, class S>
 __global__ __launch_bounds__(S::THREADS) void dw_kernel(
     const T* __restrict__ x, long ldx, const T* __restrict__ grad, long ldg,
     int piece, int dim, int ldim, const int* count, int mt, int nt, int run,
-    const float* __restrict__ scale, T* __restrict__ out,
-    float* __restrict__ slabs, long slab) {
+    const Factor factor, T* __restrict__ out, float* __restrict__ slabs,
+    long slab) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int split = blockIdx.x / (mt * nt);
   int tm, tn;
@@ -691,30 +687,164 @@ __global__ __launch_bounds__(S::THREADS) void dw_kernel(
                                   (int)ldg, kbeg, kend, kend, smem, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;
-  const float inv = scale[1];
+  const float inv = factor.inverse();
+  const int d0 = m0 + (wave / S::WN) * (S::MI * 16);
+  char* stage = smem + wave * (2 * S::MI * 256 * sizeof(T));
 #pragma unroll
-  for (int mi = 0; mi < S::MI; ++mi) {
-    const int d = m0 + (wave / S::WN) * (S::MI * 16) + mi * 16 + g * 4;
+  for (int ni = 0; ni < S::NI; ++ni) {
+    const int v0 = n0 + (wave % S::WN) * (S::NI * 16) + ni * 16;
+    if (!slabs && dim % (16 / (int)sizeof(T)) == 0) {
+      T o[S::MI][4];
 #pragma unroll
-    for (int ni = 0; ni < S::NI; ++ni) {
-      const int v = n0 + (wave % S::WN) * (S::NI * 16) + ni * 16 + i;
-      if (v >= piece || d >= dim) continue;
+      for (int mi = 0; mi < S::MI; ++mi) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[mi][r] = (T)(acc[mi][ni][r] * inv);
+      }
+      tile::store_columns<T, S::MI * 16>(
+          o, stage + (ni & 1) * (S::MI * 256 * sizeof(T)),
+          out + (long)v0 * dim + d0, dim, piece - v0, dim - d0, lane);
+      continue;
+    }
+    const int v = v0 + i;
+    if (v >= piece) continue;
+#pragma unroll
+    for (int mi = 0; mi < S::MI; ++mi) {
+      const int d = d0 + mi * 16 + g * 4;
+      if (d >= dim) continue;
       if (slabs) {
-        float* p = slabs + split * slab + (long)v * ldim + d;
-        *reinterpret_cast<f32x4*>(p) = acc[mi][ni];
-      } else if (dim % 4 == 0) {
-        T o[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = (T)(acc[mi][ni][r] * inv);
-        __builtin_memcpy(out + (long)v * dim + d, o, 4 * sizeof(T));
+        *reinterpret_cast<f32x4*>(slabs + split * slab + (long)v * ldim + d) =
+            acc[mi][ni];
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          if (d + r < dim) out[(long)v * dim + d + r] = (T)(acc[mi][ni][r] * inv);
+          if (d + r < dim) {
+            out[(long)v * dim + d + r] = (T)(acc[mi][ni][r] * inv);
+          }
         }
       }
     }
   }
+}
+
+// ------------------------------------------------------------- the endings
+// Slabs of fp32 rows (ldim values, a multiple of 4) added into rows of `dim`
+// values of T.  pos: which slab row a row takes, none (zeros) for -1.
+struct Adding {
+  const float* slabs;
+  long slab, rows;
+  int splits, ldim, dim;
+  const int* pos;
+  void* out;
+  int blocks;
+};
+
+template <class T>
+__device__ __forceinline__ void add_body(const Adding& a, float f,
+                                         int block) {
+  const int groups = (a.dim + 3) / 4;
+  const long total = a.rows * groups;
+  for (long k = (long)block * 256 + threadIdx.x; k < total;
+       k += (long)a.blocks * 256) {
+    const long n = k / groups;
+    const int d = (int)(k - n * groups) * 4;
+    const long p = a.pos ? a.pos[n] : n;
+    f32x4 s = {};
+    if (p >= 0) {
+      const float* at = a.slabs + p * a.ldim + d;
+#pragma unroll 8
+      for (int j = 0; j < a.splits; ++j) {
+        s += *reinterpret_cast<const f32x4*>(at + j * a.slab);
+      }
+    }
+    T o[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = (T)(s[r] * f);
+    T* out = (T*)a.out + n * a.dim + d;
+    if (d + 4 <= a.dim) {
+      __builtin_memcpy(out, o, sizeof(o));
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (d + r < a.dim) out[r] = o[r];
+      }
+    }
+  }
+}
+
+// db from its parts, of `part` tokens each: 64 entries a workgroup, 4 waves
+// that take every fourth part
+struct Bias {
+  const float* parts;
+  long vocab;
+  int part;
+  void* out;
+  int blocks;
+};
+
+template <class T>
+__device__ __forceinline__ void bias_body(const Bias& b, int rows, float f,
+                                          int block) {
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const long v = (long)block * 64 + lane;
+  const int parts = (rows + b.part - 1) / b.part;
+  float s = 0.f;
+  if (v < b.vocab) {
+#pragma unroll 8
+    for (int k = wave; k < parts; k += 4) s += b.parts[(long)k * b.vocab + v];
+  }
+  sums[wave][lane] = s;
+  __syncthreads();
+  if (wave == 0 && v < b.vocab) {
+    ((T*)b.out)[v] =
+        (T)((sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]) *
+            f);
+  }
+}
+
+// out *= up, where that changes anything; out is 16-byte aligned
+struct Times {
+  void* out;
+  long n;
+  int blocks;
+};
+
+template <class T>
+__device__ __forceinline__ void times_body(const Times& t, float f,
+                                           int block) {
+  if (f == 1.f) return;
+  constexpr int E = 16 / sizeof(T);
+  struct alignas(16) Chunk {
+    T v[E];
+  };
+  T* out = (T*)t.out;
+  for (long k = (long)block * 256 + threadIdx.x; k * E < t.n;
+       k += (long)t.blocks * 256) {
+    if ((k + 1) * E <= t.n) {
+      Chunk c = reinterpret_cast<Chunk*>(out)[k];
+#pragma unroll
+      for (int j = 0; j < E; ++j) c.v[j] = (T)((float)c.v[j] * f);
+      reinterpret_cast<Chunk*>(out)[k] = c;
+    } else {
+      for (long j = k * E; j < t.n; ++j) out[j] = (T)((float)out[j] * f);
+    }
+  }
+}
+
+// The endings of one call in one launch, each with workgroups of its own.
+template <class T>
+__global__ __launch_bounds__(256) void end_kernel(
+    const Adding dx, const Adding dw, const Bias db, const Times dw_times,
+    const Factor factor, const float* __restrict__ up) {
+  const float u = up ? *up : 1.f;
+  const float f = factor.inverse() * u;
+  int block = blockIdx.x;
+  if (block < dx.blocks) return add_body<T>(dx, f, block);
+  block -= dx.blocks;
+  if (block < dw.blocks) return add_body<T>(dw, f, block);
+  block -= dw.blocks;
+  if (block < db.blocks) return bias_body<T>(db, *factor.count, f, block);
+  times_body<T>(dw_times, u, block - db.blocks);
 }
 
 int blocks_for(long work) {
@@ -771,15 +901,20 @@ struct Run {
     check(hipGetLastError());
   }
 
+  static Factor factor(const Operands& o, const Grads& b) {
+    return Factor{b.scale, o.count, b.mean, sizeof(T) == 2 &&
+                  std::is_same_v<T, _Float16>};
+  }
+
   static void probs(const Operands& o, const Sums& f, const Grads& b,
                     hipStream_t s) {
     const long ldg = padded(o.vocab);
-    const dim3 grid(ceil_div(o.rows, PROWS),
+    const dim3 grid(ceil_div(o.rows, o.plan.part) + 1,
                     ceil_div(ldg * sizeof(T) / 16, 256));
     probs_kernel<T><<<grid, 256, 0, s>>>(
-        (T*)b.grad, ldg, (int)o.vocab, o.count, o.tgt, f.pmax, o.plan.bands,
-        o.plan.band, f.rowm, f.rowi, f.ztgt, b.coef, o.eps,
-        o.eps / (float)o.vocab, b.pbias);
+        (T*)b.grad, ldg, (int)o.vocab, o.plan.part, o.tgt, f.pmax,
+        o.plan.bands, o.plan.band, f.rowm, f.rowi, f.ztgt, factor(o, b),
+        o.eps, o.eps / (float)o.vocab, b.pbias, f.loss, o.rows, f.total);
     check(hipGetLastError());
   }
 
@@ -820,34 +955,41 @@ struct Run {
       with_lds(dw_kernel<T, S>, S::LDS);
       dw_kernel<T, S><<<md * vt * splits, S::THREADS, S::LDS, s>>>(
           (const T*)o.x, o.ldx, (const T*)b.grad, ldg, piece, o.dim, ldim,
-          o.count, md, vt, run, b.scale, (T*)b.dw + v0 * o.dim, b.dw_slabs,
+          o.count, md, vt, run, factor(o, b), (T*)b.dw + v0 * o.dim,
+          b.dw_slabs,
           (long)piece * ldim);
       check(hipGetLastError());
     }
   }
 
-  // rows [v0, v0 + piece) of dw from its slabs
-  static void end_dw(const Operands& o, const Grads& b, long v0, int piece,
-                     const float* up, hipStream_t s) {
-    add_kernel<T><<<blocks_for((long)piece * ((o.dim + 3) / 4)), 256, 0, s>>>(
-        b.dw_slabs, (long)piece * o.ldx, o.plan.dw_splits, o.ldx, o.dim,
-        piece, nullptr, b.scale, up, (T*)b.dw + v0 * o.dim);
+  // What is left of rows [v0, v0 + piece) of dw, and of dx and db where they
+  // are given, times up (null: 1).
+  static void end(const Operands& o, const Grads& b, long v0, int piece,
+                  bool rest, const float* up, hipStream_t s) {
+    const int groups = (o.dim + 3) / 4;
+    Adding dx{}, dw{};
+    Bias db{};
+    Times times{};
+    if (rest && b.dx) {
+      dx = Adding{b.dx_slabs, o.rows * o.ldx, o.rows, o.plan.dx_splits, o.ldx,
+                  o.dim, o.pos, b.dx, blocks_for(o.rows * groups)};
+    }
+    if (b.dw && b.dw_slabs) {
+      dw = Adding{b.dw_slabs, (long)piece * o.ldx, piece, o.plan.dw_splits,
+                  o.ldx, o.dim, nullptr, (T*)b.dw + v0 * o.dim,
+                  blocks_for((long)piece * groups)};
+    } else if (b.dw && up) {
+      times.out = b.dw;
+      times.n = o.vocab * o.dim;
+      times.blocks = std::min(blocks_for(times.n / 8), 2048);
+    }
+    if (rest && b.db) {
+      db = Bias{b.pbias, o.vocab, o.plan.part, b.db, ceil_div(o.vocab, 64)};
+    }
+    const int blocks = dx.blocks + dw.blocks + db.blocks + times.blocks;
+    if (blocks == 0) return;
+    end_kernel<T><<<blocks, 256, 0, s>>>(dx, dw, db, times, factor(o, b), up);
     check(hipGetLastError());
-  }
-
-  static void end(const Operands& o, const Grads& b, const float* up,
-                  hipStream_t s) {
-    if (b.dx) {
-      add_kernel<T><<<blocks_for(o.rows * ((o.dim + 3) / 4)), 256, 0, s>>>(
-          b.dx_slabs, o.rows * o.ldx, o.plan.dx_splits, o.ldx, o.dim, o.rows,
-          o.pos, b.scale, up, (T*)b.dx);
-      check(hipGetLastError());
-    }
-    if (b.db) {
-      bias_kernel<T><<<ceil_div(o.vocab, 256), 256, 0, s>>>(
-          b.pbias, o.vocab, b.part, o.count, b.scale, up, (T*)b.db);
-      check(hipGetLastError());
-    }
   }
 };
 
@@ -882,8 +1024,13 @@ Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   const long most = std::min<long>(
       std::max<long>((256l << 20) / (rows * size), p.edge), 1l << 20);
   p.piece = keep ? vocab : std::min(vocab, most / p.edge * p.edge);
-  p.parts = keep ? ceil_div(rows, PROWS) : ceil_div(rows, p.edge);
-  p.part = keep ? PROWS : p.edge;
+  p.part = p.edge;
+  if (keep) {
+    const long columns = ceil_div(vocab * size, 4096);
+    p.part = 64;
+    while (p.part > 16 && columns * ceil_div(rows, p.part) < 1024) p.part /= 2;
+  }
+  p.parts = ceil_div(rows, p.part);
   const long dx_tiles =
       (long)ceil_div(ldim, p.edge) * ceil_div(rows, p.edge);
   const long dw_tiles =
@@ -943,8 +1090,8 @@ void total(const float* loss, long rows, const int* count, bool mean,
 }
 
 void coefficients(Type t, const Operands& o, const float* up, bool each,
-                  bool mean, const Grads& b, hipStream_t s) {
-  coef_kernel<<<1, 1024, 0, s>>>(up, each, mean, o.idx, o.tgt, o.count,
+                  const Grads& b, hipStream_t s) {
+  coef_kernel<<<1, 1024, 0, s>>>(up, each, b.mean, o.idx, o.tgt, o.count,
                                  t == Type::fp16, b.coef, b.scale);
   check(hipGetLastError());
 }
@@ -966,14 +1113,7 @@ void finish_kept(Type t, const Operands& o, const Grads& b, const float* up,
                  hipStream_t s) {
   by_type(t, [&](auto* q) {
     using T = std::remove_pointer_t<decltype(q)>;
-    Run<T>::end(o, b, up, s);
-    if (b.dw && b.dw_slabs) {
-      Run<T>::end_dw(o, b, 0, (int)o.vocab, up, s);
-    } else if (b.dw) {
-      const long n = o.vocab * o.dim;
-      times_kernel<T><<<blocks_for(n / 8), 256, 0, s>>>((T*)b.dw, n, up);
-      check(hipGetLastError());
-    }
+    Run<T>::end(o, b, 0, (int)o.vocab, true, up, s);
   });
 }
 
@@ -990,11 +1130,8 @@ void gradients_again(Type t, const Operands& o, const Sums& f, const Grads& b,
         Run<T>::template again<Mid>(o, f, b, v0, piece, s);
         Run<T>::template products<Mid>(o, b, v0, piece, s);
       }
-      if (b.dw && b.dw_slabs) {
-        Run<T>::end_dw(o, b, v0, piece, nullptr, s);
-      }
+      Run<T>::end(o, b, v0, piece, v0 + piece == o.vocab, nullptr, s);
     }
-    Run<T>::end(o, b, nullptr, s);
   });
 }
 

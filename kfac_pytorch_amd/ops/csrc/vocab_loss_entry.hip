@@ -194,12 +194,13 @@ vocab_loss_forward(Tensor hidden, Tensor weight, Tensor target,
   Tensor total;
   if (sum || mean) {
     total = at::empty({}, f32);
-    vocab_loss::total(f.loss, rows, ints.count, mean,
-                      total.data_ptr<float>(), stream);
+    f.total = total.data_ptr<float>();
+    if (!keep) {
+      vocab_loss::total(f.loss, rows, ints.count, mean, f.total, stream);
+    }
   }
   std::vector<std::optional<Tensor>> kept;
   if (keep) {
-    Tensor small = at::empty({4 + rows}, f32);
     Tensor dx_slabs, dw, dw_slabs, pbias;
     if (need_x) {
       dx_slabs = at::empty({plan.dx_splits, rows, (long)c.o.ldx}, f32);
@@ -212,16 +213,14 @@ vocab_loss_forward(Tensor hidden, Tensor weight, Tensor target,
     }
     if (need_b) pbias = at::empty({plan.parts, vocab}, f32);
     vocab_loss::Grads b{};
-    b.scale = small.data_ptr<float>();
-    b.coef = b.scale + 4;
+    b.mean = mean;
     b.pbias = floats(pbias);
     b.dx_slabs = floats(dx_slabs);
     b.dw_slabs = floats(dw_slabs);
     b.grad = data(grad);
     b.dw = data(dw);
-    vocab_loss::coefficients(c.type, c.o, nullptr, false, mean, b, stream);
     vocab_loss::gradients_kept(c.type, c.o, f, b, stream);
-    for (const Tensor& t : {small, dx_slabs, dw, dw_slabs, pbias}) {
+    for (const Tensor& t : {dx_slabs, dw, dw_slabs, pbias}) {
       kept.push_back(t.defined() ? std::optional<Tensor>(t) : std::nullopt);
     }
   }
@@ -231,33 +230,32 @@ vocab_loss_forward(Tensor hidden, Tensor weight, Tensor target,
 // The gradients that vocab_loss_forward kept, times up; uses them up.
 // -> (dx, dw, db); those not asked for are undefined
 std::tuple<Tensor, Tensor, Tensor> vocab_loss_finish(
-    Tensor up, Tensor hidden, Tensor weight, Tensor ints_t,
+    Tensor up, Tensor hidden, Tensor weight, Tensor ints_t, bool mean,
     std::vector<std::optional<Tensor>> kept) {
   check_shapes(hidden, weight, std::nullopt);
   TORCH_CHECK(up.device() == hidden.device() && up.numel() == 1 &&
-                  up.scalar_type() == at::kFloat && kept.size() == 5 &&
+                  up.scalar_type() == at::kFloat && kept.size() == 4 &&
                   ints_t.numel() == 4 + 3 * hidden.size(0),
               "linear_cross_entropy: backward state mismatch");
   const c10::OptionalDeviceGuard guard(hidden.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   Call c = make_call(hidden, weight, std::nullopt, ints_t, 0.0, true);
-  Tensor small = *kept[0], dx, dw, db;
-  Tensor dx_slabs = kept[1].value_or(Tensor());
-  Tensor dw_slabs = kept[3].value_or(Tensor());
-  Tensor pbias = kept[4].value_or(Tensor());
+  Tensor dx, dw, db;
+  Tensor dx_slabs = kept[0].value_or(Tensor());
+  Tensor dw_slabs = kept[2].value_or(Tensor());
+  Tensor pbias = kept[3].value_or(Tensor());
   if (dx_slabs.defined()) {
     dx = at::empty({c.o.rows, (long)c.o.dim}, hidden.options());
   }
   if (dw_slabs.defined()) {
     dw = at::empty({c.o.vocab, (long)c.o.dim}, weight.options());
-  } else if (kept[2]) {
-    dw = *kept[2];
+  } else if (kept[1]) {
+    dw = *kept[1];
   }
   if (pbias.defined()) db = at::empty({c.o.vocab}, weight.options());
   vocab_loss::Grads b{};
-  b.scale = small.data_ptr<float>();
+  b.mean = mean;
   b.pbias = floats(pbias);
-  b.part = c.o.plan.part;
   b.dx_slabs = floats(dx_slabs);
   b.dw_slabs = floats(dw_slabs);
   b.dx = data(dx);
@@ -309,15 +307,15 @@ std::tuple<Tensor, Tensor, Tensor> vocab_loss_backward(
   vocab_loss::Grads b{};
   b.scale = small.data_ptr<float>();
   b.coef = b.scale + 4;
+  b.mean = mean;
   b.pbias = floats(pbias);
-  b.part = plan.part;
   b.dx_slabs = floats(dx_slabs);
   b.dw_slabs = floats(dw_slabs);
   b.grad = data(grad);
   b.dx = data(dx);
   b.dw = data(dw);
   b.db = data(db);
-  vocab_loss::coefficients(c.type, c.o, up.data_ptr<float>(), each, mean, b,
+  vocab_loss::coefficients(c.type, c.o, up.data_ptr<float>(), each, b,
                            stream);
   vocab_loss::gradients_again(c.type, c.o, row_state(state, rows), b, stream);
   return {dx, dw, db};

@@ -60,8 +60,8 @@ class _VocabLoss(torch.autograd.Function):
         up = up.contiguous()
         kept, ctx.kept = ctx.kept, None
         if kept:
-            dx, dw, db = _ext.vocab_loss_finish(up, hidden, weight, ints,
-                                                kept)
+            dx, dw, db = _ext.vocab_loss_finish(
+                up, hidden, weight, ints, ctx.reduction, kept)
         else:
             dx, dw, db = _ext.vocab_loss_backward(
                 up, hidden, weight, bias, state, ints, ctx.eps,
