@@ -20,10 +20,12 @@ inline void check(hipError_t e) {
   }
 }
 
+enum class Tile { wide, mid, small };  // 256 x 256, 128 x 128, 128 x 64
+
 // How a call of given sizes is cut up.
 struct Plan {
-  bool wide;              // tiles of 256 x 256, else of 128 x 128
-  int edge, band, bands;  // of a tile; entries of a band, bands of a row
+  Tile logits, dx, dw;
+  int band, bands;        // entries of a band, bands of a row
   long piece;             // entries of the vocabulary at a time
   int part, parts;        // tokens of a part of the bias gradient's sum
   int dx_splits, dw_splits;

@@ -855,6 +855,17 @@ int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 
 using Wide = Shape<256, 256, 2, 4>;
 using Mid = Shape<128, 128, 2, 4>;
+using Small = Shape<128, 64, 2, 2>;
+
+// calls f with a value of the tile's shape
+template <class F>
+void by_shape(Tile t, F f) {
+  switch (t) {
+    case Tile::wide: f(Wide()); break;
+    case Tile::mid: f(Mid()); break;
+    case Tile::small: f(Small()); break;
+  }
+}
 
 template <class F>
 void with_lds(F* kernel, int bytes) {
@@ -879,7 +890,6 @@ struct Run {
     check(hipGetLastError());
   }
 
-  template <class S>
   static void forward(const Operands& o, const Sums& f, T* grad,
                       hipStream_t s) {
     Logits p{};
@@ -889,12 +899,15 @@ struct Run {
     p.pz = o.eps != 0.f ? f.pz : nullptr;
     p.ztgt = f.ztgt;
     p.bands = o.plan.bands;
-    if (grad) {
-      p.ldg = padded(o.vocab);
-      logits<S, KEEP>(o, p, grad, s);
-    } else {
-      logits<S, SUMS>(o, p, nullptr, s);
-    }
+    p.ldg = padded(o.vocab);
+    by_shape(o.plan.logits, [&](auto shape) {
+      using S = decltype(shape);
+      if (grad) {
+        logits<S, KEEP>(o, p, grad, s);
+      } else {
+        logits<S, SUMS>(o, p, nullptr, s);
+      }
+    });
     join_kernel<<<ceil_div(o.rows, 4), 256, 0, s>>>(
         f.pmax, f.psum, p.pz, f.ztgt, o.pos, o.tgt, o.rows, p.bands, o.eps,
         o.eps / (float)o.vocab, f.rowm, f.rowi, f.loss);
@@ -918,7 +931,6 @@ struct Run {
     check(hipGetLastError());
   }
 
-  template <class S>
   static void again(const Operands& o, const Sums& f, const Grads& b,
                     long v0, int piece, hipStream_t s) {
     Logits p{};
@@ -932,33 +944,50 @@ struct Run {
     p.share = o.eps / (float)o.vocab;
     p.pbias = b.pbias;
     p.all = o.vocab;
-    logits<S, AGAIN>(o, p, (T*)b.grad, s);
+    by_shape(o.plan.logits, [&](auto shape) {
+      logits<decltype(shape), AGAIN>(o, p, (T*)b.grad, s);
+    });
   }
 
   template <class S>
+  static void dx_product(const Operands& o, const Grads& b, long v0,
+                         int piece, hipStream_t s) {
+    const int md = ceil_div(o.ldx, S::BM), nt = ceil_div(o.rows, S::BN);
+    const int splits = o.plan.dx_splits;
+    const long ldg = padded(piece);
+    const int run = ceil_div(ceil_div(ldg, splits), 64) * 64;
+    with_lds(dx_kernel<T, S>, S::LDS);
+    dx_kernel<T, S><<<md * nt * splits, S::THREADS, S::LDS, s>>>(
+        (const T*)o.w + v0 * o.ldw, o.ldw, (const T*)b.grad, ldg, piece,
+        o.ldx, o.count, md, nt, run, v0 == 0, b.dx_slabs, o.rows * o.ldx);
+    check(hipGetLastError());
+  }
+
+  template <class S>
+  static void dw_product(const Operands& o, const Grads& b, long v0,
+                         int piece, hipStream_t s) {
+    const int md = ceil_div(o.ldx, S::BM), vt = ceil_div(piece, S::BN);
+    const int splits = o.plan.dw_splits;
+    const int run = ceil_div(ceil_div(o.rows, splits), 64) * 64;
+    with_lds(dw_kernel<T, S>, S::LDS);
+    dw_kernel<T, S><<<md * vt * splits, S::THREADS, S::LDS, s>>>(
+        (const T*)o.x, o.ldx, (const T*)b.grad, padded(piece), piece, o.dim,
+        o.ldx, o.count, md, vt, run, factor(o, b), (T*)b.dw + v0 * o.dim,
+        b.dw_slabs, (long)piece * o.ldx);
+    check(hipGetLastError());
+  }
+
   static void products(const Operands& o, const Grads& b, long v0, int piece,
                        hipStream_t s) {
-    const int ldim = o.ldx, md = ceil_div(ldim, S::BM);
-    const long ldg = padded(piece);
     if (b.dx_slabs) {
-      const int nt = ceil_div(o.rows, S::BN), splits = o.plan.dx_splits;
-      const int run = ceil_div(ceil_div(ldg, splits), 64) * 64;
-      with_lds(dx_kernel<T, S>, S::LDS);
-      dx_kernel<T, S><<<md * nt * splits, S::THREADS, S::LDS, s>>>(
-          (const T*)o.w + v0 * o.ldw, o.ldw, (const T*)b.grad, ldg, piece,
-          ldim, o.count, md, nt, run, v0 == 0, b.dx_slabs, o.rows * ldim);
-      check(hipGetLastError());
+      by_shape(o.plan.dx, [&](auto shape) {
+        dx_product<decltype(shape)>(o, b, v0, piece, s);
+      });
     }
     if (b.dw || b.dw_slabs) {
-      const int vt = ceil_div(piece, S::BN), splits = o.plan.dw_splits;
-      const int run = ceil_div(ceil_div(o.rows, splits), 64) * 64;
-      with_lds(dw_kernel<T, S>, S::LDS);
-      dw_kernel<T, S><<<md * vt * splits, S::THREADS, S::LDS, s>>>(
-          (const T*)o.x, o.ldx, (const T*)b.grad, ldg, piece, o.dim, ldim,
-          o.count, md, vt, run, factor(o, b), (T*)b.dw + v0 * o.dim,
-          b.dw_slabs,
-          (long)piece * ldim);
-      check(hipGetLastError());
+      by_shape(o.plan.dw, [&](auto shape) {
+        dw_product<decltype(shape)>(o, b, v0, piece, s);
+      });
     }
   }
 
@@ -1002,10 +1031,26 @@ void by_type(Type t, F f) {
   }
 }
 
-// Wide tiles do twice the work per byte that goes through LDS and take a CU
-// each; they pay once they fill the card.
-bool wide(long m, long n) {
-  return (long)ceil_div(m, 256) * ceil_div(n, 256) >= 256;
+constexpr int EDGE_M[] = {256, 128, 128};
+constexpr int EDGE_N[] = {256, 128, 64};
+constexpr int BAND[] = {128, 64, 64};
+// workgroups that run at once: one, two and three for each of 256 CUs
+constexpr int SLOTS[] = {256, 512, 768};
+
+long tiles(Tile t, long m, long n) {
+  return (long)ceil_div(m, EDGE_M[(int)t]) * ceil_div(n, EDGE_N[(int)t]);
+}
+
+// Wide tiles do twice the work per byte that goes through LDS, but one
+// workgroup fills a CU: they pay once there are enough for all CUs (8192 x
+// 16384 x 768 in bf16: 217 us against 251; 300 x 9521 x 512: 19.6 against
+// 9.6).  fp32 products are 16 times slower for the same loads, so small tiles,
+// three workgroups to a CU, lose nothing and leave less of a last round (700 x
+// 33278 x 256: 108 us against 138 and 124); so do a few rows (35 x 33278 x
+// 256: 6.2 us against 12.2 and 7.7).
+Tile tile_for(long m, long n, int size, long few) {
+  if (size == 4 || n <= few) return Tile::small;
+  return tiles(Tile::wide, m, n) >= 192 ? Tile::wide : Tile::mid;
 }
 
 }  // namespace
@@ -1014,32 +1059,35 @@ long padded(long n) { return (n + 7) / 8 * 8; }
 
 Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   Plan p;
-  p.wide = wide(vocab, rows);
-  p.edge = p.wide ? 256 : 128;
-  p.band = p.wide ? 128 : 64;
-  p.bands = ceil_div(vocab, p.edge) * (p.edge / p.band);
+  p.logits = tile_for(vocab, rows, size, 64);
+  p.band = BAND[(int)p.logits];
+  const int edge_m = EDGE_M[(int)p.logits], edge_n = EDGE_N[(int)p.logits];
+  p.bands = ceil_div(vocab, edge_m) * (edge_m / p.band);
   // a piece of the vocabulary: 256 MB of g at most, which the card's last
   // cache then holds between the three products; offsets within a tile of g
   // stay below 2^31 for rows of up to a million entries
   const long most = std::min<long>(
-      std::max<long>((256l << 20) / (rows * size), p.edge), 1l << 20);
-  p.piece = keep ? vocab : std::min(vocab, most / p.edge * p.edge);
-  p.part = p.edge;
+      std::max<long>((256l << 20) / (rows * size), edge_m), 1l << 20);
+  p.piece = keep ? vocab : std::min(vocab, most / edge_m * edge_m);
+  p.part = edge_n;
   if (keep) {
     const long columns = ceil_div(vocab * size, 4096);
     p.part = 64;
     while (p.part > 16 && columns * ceil_div(rows, p.part) < 1024) p.part /= 2;
   }
   p.parts = ceil_div(rows, p.part);
-  const long dx_tiles =
-      (long)ceil_div(ldim, p.edge) * ceil_div(rows, p.edge);
-  const long dw_tiles =
-      (long)ceil_div(ldim, p.edge) * ceil_div(p.piece, p.edge);
-  const long want = p.wide ? 256 : 512;
+  // dx has few tiles and a long k: a tile that fits the call's size, its k
+  // cut up until the card is full once (fp32: twice, its rounds are long)
+  p.dx = p.logits;
+  const long dx_tiles = tiles(p.dx, ldim, rows);
+  const long slots = SLOTS[(int)p.dx] * (size == 4 ? 2 : 1);
   p.dx_splits = (int)std::max<long>(
-      1, std::min<long>({want / dx_tiles, p.piece / 512, 64}));
+      1, std::min<long>({slots / dx_tiles, p.piece / 512, 64}));
+  // dw has many tiles and its k are the rows
+  p.dw = tile_for(ldim, p.piece, size, 0);
+  const long dw_tiles = tiles(p.dw, ldim, p.piece);
   p.dw_splits = (int)std::max<long>(
-      1, std::min<long>({want / dw_tiles, rows / 512, 16}));
+      1, std::min<long>({SLOTS[(int)p.dw] / 2 / dw_tiles, rows / 512, 16}));
   return p;
 }
 
@@ -1075,11 +1123,7 @@ void forward(Type t, const Operands& o, const Sums& f, void* grad,
              hipStream_t s) {
   by_type(t, [&](auto* q) {
     using T = std::remove_pointer_t<decltype(q)>;
-    if (o.plan.wide) {
-      Run<T>::template forward<Wide>(o, f, (T*)grad, s);
-    } else {
-      Run<T>::template forward<Mid>(o, f, (T*)grad, s);
-    }
+    Run<T>::forward(o, f, (T*)grad, s);
   });
 }
 
@@ -1101,11 +1145,7 @@ void gradients_kept(Type t, const Operands& o, const Sums& f, const Grads& b,
   by_type(t, [&](auto* q) {
     using T = std::remove_pointer_t<decltype(q)>;
     Run<T>::probs(o, f, b, s);
-    if (o.plan.wide) {
-      Run<T>::template products<Wide>(o, b, 0, (int)o.vocab, s);
-    } else {
-      Run<T>::template products<Mid>(o, b, 0, (int)o.vocab, s);
-    }
+    Run<T>::products(o, b, 0, (int)o.vocab, s);
   });
 }
 
@@ -1123,13 +1163,8 @@ void gradients_again(Type t, const Operands& o, const Sums& f, const Grads& b,
     using T = std::remove_pointer_t<decltype(q)>;
     for (long v0 = 0; v0 < o.vocab; v0 += o.plan.piece) {
       const int piece = (int)std::min(o.plan.piece, o.vocab - v0);
-      if (o.plan.wide) {
-        Run<T>::template again<Wide>(o, f, b, v0, piece, s);
-        Run<T>::template products<Wide>(o, b, v0, piece, s);
-      } else {
-        Run<T>::template again<Mid>(o, f, b, v0, piece, s);
-        Run<T>::template products<Mid>(o, b, v0, piece, s);
-      }
+      Run<T>::again(o, f, b, v0, piece, s);
+      Run<T>::products(o, b, v0, piece, s);
       Run<T>::end(o, b, v0, piece, v0 + piece == o.vocab, nullptr, s);
     }
   });
