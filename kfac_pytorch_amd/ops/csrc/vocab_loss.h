@@ -58,9 +58,13 @@ struct Grads {
   bool mean;
 };
 
-void scan(const void* target, bool wide_ints, long rows, long ignore,
-          long vocab, int* pos, int* idx, int* tgt, int* count,
-          hipStream_t s);
+// The kept rows of a call: numbers them (pos, idx, tgt, count) and packs their
+// hidden states into rows of ldo values.
+void prepare(Type t, const void* target, bool wide_ints, long rows,
+             long ignore, long vocab, int* pos, int* idx, int* tgt,
+             int* count, const void* in, long ld, long step, int cols,
+             void* out, int ldo, hipStream_t s);
+// The same of rows that are numbered already, or of all rows (idx null).
 void pack(Type t, const void* in, long ld, long step, long rows, int cols,
           const int* idx, const int* count, void* out, int ldo,
           hipStream_t s);

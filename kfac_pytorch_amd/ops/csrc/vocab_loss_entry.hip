@@ -75,14 +75,18 @@ Call make_call(const Tensor& hidden, const Tensor& weight,
   return c;
 }
 
-void pack(Call* c, const Tensor& hidden, const Tensor& weight,
-          const std::optional<Tensor>& bias, hipStream_t stream) {
+void pack_hidden(Call* c, const Tensor& hidden, hipStream_t stream) {
   auto& o = c->o;
   c->x = at::empty({o.rows, o.ldx}, hidden.options());
   vocab_loss::pack(c->type, hidden.data_ptr(), hidden.stride(0),
                    hidden.stride(1), o.rows, o.dim, o.idx, o.count,
                    c->x.data_ptr(), o.ldx, stream);
   o.x = c->x.data_ptr();
+}
+
+void pack_weight(Call* c, const Tensor& weight,
+                 const std::optional<Tensor>& bias, hipStream_t stream) {
+  auto& o = c->o;
   if (direct(weight)) {
     c->w = weight;
     o.ldw = weight.stride(0);
@@ -167,13 +171,17 @@ vocab_loss_forward(Tensor hidden, Tensor weight, Tensor target,
   const auto f32 = hidden.options().dtype(at::kFloat);
   Tensor ints_t = at::empty({4 + 3 * rows}, f32.dtype(at::kInt));
   const Ints ints(ints_t, rows);
-  vocab_loss::scan(target.data_ptr(), target.scalar_type() == at::kLong, rows,
-                   ignore_index, vocab, ints.pos, ints.idx, ints.tgt,
-                   ints.count, stream);
   const bool keep = (sum || mean) && (need_x || need_w || need_b) &&
                     keeps(rows, vocab, (int)hidden.element_size());
   Call c = make_call(hidden, weight, bias, ints_t, eps, keep);
-  pack(&c, hidden, weight, bias, stream);
+  c.x = at::empty({rows, (long)c.o.ldx}, hidden.options());
+  c.o.x = c.x.data_ptr();
+  vocab_loss::prepare(c.type, target.data_ptr(),
+                      target.scalar_type() == at::kLong, rows, ignore_index,
+                      vocab, ints.pos, ints.idx, ints.tgt, ints.count,
+                      hidden.data_ptr(), hidden.stride(0), hidden.stride(1),
+                      c.o.dim, c.x.data_ptr(), c.o.ldx, stream);
+  pack_weight(&c, weight, bias, stream);
   const auto& plan = c.o.plan;
 
   Tensor loss = at::empty({rows}, f32);
@@ -282,7 +290,8 @@ std::tuple<Tensor, Tensor, Tensor> vocab_loss_backward(
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   const auto f32 = hidden.options().dtype(at::kFloat);
   Call c = make_call(hidden, weight, bias, ints_t, eps, false);
-  pack(&c, hidden, weight, bias, stream);
+  pack_hidden(&c, hidden, stream);
+  pack_weight(&c, weight, bias, stream);
   const auto& plan = c.o.plan;
   const long dim = c.o.dim, ldx = c.o.ldx;
 

@@ -184,6 +184,19 @@ def test_wide_tiles(rows, dim, vocab, dtype):
 
 @pytest.mark.gpu
 @needs_gpu
+@pytest.mark.parametrize("rows", [16384, 16385, 20000])
+@pytest.mark.parametrize("ignored", [0.0, 0.6])
+def test_many_rows(rows, ignored):
+    """Either way of numbering the kept rows."""
+    x, w, b, t = inputs(rows, 8, 40, torch.float32, False, ignored, rows)
+    up = torch.linspace(0.5, 2.0, rows, device="cuda")
+    loss, grads = run(x, w, b, t, 0.0, "none", up)
+    check_all(formula(x, w, b, t, 0.0, up), loss, grads, x, w, b,
+              torch.float32, rows)
+
+
+@pytest.mark.gpu
+@needs_gpu
 def test_pieces_of_the_vocabulary():
     """Single rows' losses beyond 256 MB of g: two pieces, against the whole
     call with the same factors kept."""
