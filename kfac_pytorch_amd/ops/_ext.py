@@ -170,31 +170,12 @@ def has_jacobi_eigh(m: int) -> bool:
 
 
 # -- cross entropy of a vocabulary projection ---------------------------------
-def vocab_loss_forward(hidden, weight, target, bias, ignore_index: int,
-                       eps: float, reduction: str,
-                       need=(False, False, False)):
-    """(loss of every row, total or None, state, ints, kept).  state and ints
-    are what ``vocab_loss_backward`` needs, kept what ``vocab_loss_finish``
-    does (empty: there is nothing to finish)."""
-    return _load().vocab_loss_forward(hidden, weight, target, bias,
-                                      ignore_index, eps, reduction == "sum",
-                                      reduction == "mean", *need)
-
-
-def vocab_loss_finish(up, hidden, weight, ints, reduction: str, kept):
-    """(d hidden, d weight, d bias) from what the forward pass kept, which is
-    used up; None for those not asked for."""
-    return _load().vocab_loss_finish(up, hidden, weight, ints,
-                                     reduction == "mean", kept)
-
-
-def vocab_loss_backward(up, hidden, weight, bias, state, ints, eps: float,
-                        reduction: str, need):
-    """(d hidden, d weight, d bias), the logits made again; None for those
-    not asked for."""
-    return _load().vocab_loss_backward(up, hidden, weight, bias, state, ints,
-                                       eps, reduction == "none",
-                                       reduction == "mean", *need)
+def linear_cross_entropy(hidden, weight, target, bias, ignore_index: int,
+                         eps: float, reduction: int) -> torch.Tensor:
+    """Differentiable; reduction 0: none, 1: mean, 2: sum.  At least one
+    row."""
+    return _load().linear_cross_entropy(hidden, weight, target, bias,
+                                        ignore_index, eps, reduction)
 
 
 # -- one norm or inner product over many tensors ------------------------------

@@ -289,6 +289,17 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(
 // false where they are not so.
 template <int NP>
 bool as_rows(const std::array<const Tensor*, NP>& t, Entry<NP>* e) {
+  bool dense = true;
+  for (int i = 0; i < NP; ++i) dense &= t[i]->is_contiguous();
+  if (dense) {
+    e->cols = t[0]->numel();
+    e->rows = 1;
+    for (int i = 0; i < NP; ++i) {
+      e->p[i] = t[i]->const_data_ptr();
+      e->ld[i] = 0;
+    }
+    return true;
+  }
   const auto sizes = t[0]->sizes();
   // dims of more than one value, largest stride of the first operand first
   std::vector<int> dims;
@@ -329,7 +340,7 @@ bool as_rows(const std::array<const Tensor*, NP>& t, Entry<NP>* e) {
   const long rows = kept.size() == 2 ? kept[0].size : 1;
   e->cols = kept.back().size;
   for (int i = 0; i < NP; ++i) {
-    e->p[i] = t[i]->data_ptr();
+    e->p[i] = t[i]->const_data_ptr();
     e->ld[i] = kept.size() == 2 ? kept[0].stride[i] : 0;
   }
   if (rows >= (1l << 31)) return false;
@@ -404,23 +415,45 @@ void by_type(at::ScalarType t, F f) {
   }
 }
 
-void check_all(const std::vector<Tensor>& a, const char* name) {
-  for (const Tensor& t : a) {
-    TORCH_CHECK(t.is_cuda() && t.device() == a[0].device(), name,
-                ": tensors must be on one GPU");
-    TORCH_CHECK(t.scalar_type() == at::kFloat ||
-                    t.scalar_type() == at::kBFloat16 ||
-                    t.scalar_type() == at::kHalf,
-                name, ": dtype must be fp32, bf16 or fp16, got ",
-                t.scalar_type());
+// Lists of dense tensors on one GPU, pairwise of one shape; those to be
+// written have no two values at one place, and none is there twice.
+void check_lists(const char* name,
+                 std::initializer_list<const std::vector<Tensor>*> lists) {
+  const std::vector<Tensor>& first = **lists.begin();
+  for (const auto* list : lists) {
+    TORCH_CHECK_VALUE(list->size() == first.size(), name, ": lists of ",
+                      first.size(), " and ", list->size(), " tensors");
+    for (size_t i = 0; i < first.size(); ++i) {
+      const Tensor& t = (*list)[i];
+      TORCH_CHECK_VALUE(t.device() == first[0].device(), name,
+                        ": tensors on ", first[0].device(), " and ",
+                        t.device());
+      const auto type = t.scalar_type();
+      TORCH_CHECK_TYPE(t.layout() == at::kStrided &&
+                           (type == at::kFloat || type == at::kBFloat16 ||
+                            type == at::kHalf),
+                       name, ": dense fp32, bf16 or fp16 expected on the "
+                             "GPU, got ", type, ", ", t.layout());
+      TORCH_CHECK_VALUE(list == &first || t.sizes() == first[i].sizes(),
+                        name, ": shapes ", first[i].sizes(), " and ",
+                        t.sizes(), " differ");
+    }
   }
 }
 
-void check_out(const std::vector<Tensor>& out, const char* name) {
+void check_outputs(const char* name, const std::vector<Tensor>& out) {
+  std::vector<const void*> seen;
+  seen.reserve(out.size());
   for (const Tensor& t : out) {
-    TORCH_CHECK(at::has_internal_overlap(t) != at::MemOverlap::Yes, name,
-                ": an output's values share memory");
+    TORCH_CHECK_VALUE(t.is_contiguous() || at::has_internal_overlap(t) !=
+                                               at::MemOverlap::Yes,
+                      name, ": an output's values share memory");
+    if (t.numel()) seen.push_back(t.const_data_ptr());
   }
+  std::sort(seen.begin(), seen.end());
+  TORCH_CHECK_VALUE(std::adjacent_find(seen.begin(), seen.end()) ==
+                        seen.end(),
+                    name, ": the same tensor is to be written twice");
 }
 
 constexpr at::ScalarType TYPES[] = {at::kFloat, at::kBFloat16, at::kHalf};
@@ -480,20 +513,15 @@ void scale_pass(const std::vector<Tensor>& in, const std::vector<Tensor>& out,
 Tensor grad_norm(std::vector<Tensor> tensors,
                  std::optional<std::vector<Tensor>> out, double max_norm,
                  int64_t kind) {
-  TORCH_CHECK(!tensors.empty(), "grad_norm: no tensors");
-  check_all(tensors, "grad_norm");
+  TORCH_CHECK_VALUE(!tensors.empty(), "grad_norm: no tensors");
+  if (out) {
+    check_lists("clip_by_global_norm", {&tensors, &*out});
+    check_outputs("clip_by_global_norm", *out);
+  } else {
+    check_lists("global_norm", {&tensors});
+  }
   const c10::OptionalDeviceGuard guard(tensors[0].device());
   const hipStream_t s = c10::hip::getCurrentHIPStream().stream();
-  if (out) {
-    TORCH_CHECK(out->size() == tensors.size(), "grad_norm: out");
-    check_all(*out, "grad_norm");
-    check_out(*out, "grad_norm");
-    for (size_t i = 0; i < tensors.size(); ++i) {
-      TORCH_CHECK((*out)[i].sizes() == tensors[i].sizes() &&
-                      (*out)[i].device() == tensors[i].device(),
-                  "grad_norm: out");
-    }
-  }
   std::vector<Tensor> keep;
   Batch<1> batch[3];
   int blocks = 0;
@@ -546,20 +574,9 @@ Tensor grad_norm(std::vector<Tensor> tensors,
 // -> nu; writes out
 Tensor trust_region(std::vector<Tensor> updates, std::vector<Tensor> grads,
                     std::vector<Tensor> out, double lr, double kl) {
-  TORCH_CHECK(!updates.empty() && updates.size() == grads.size() &&
-                  updates.size() == out.size(),
-              "trust_region: lists must match");
-  check_all(updates, "trust_region");
-  check_all(grads, "trust_region");
-  check_all(out, "trust_region");
-  check_out(out, "trust_region");
-  for (size_t i = 0; i < updates.size(); ++i) {
-    TORCH_CHECK(updates[i].sizes() == grads[i].sizes() &&
-                    updates[i].sizes() == out[i].sizes() &&
-                    updates[i].device() == grads[i].device() &&
-                    updates[i].device() == out[i].device(),
-                "trust_region: tensors must match");
-  }
+  TORCH_CHECK_VALUE(!updates.empty(), "kl_clip: no tensors");
+  check_lists("kl_clip", {&updates, &grads, &out});
+  check_outputs("kl_clip", out);
   const c10::OptionalDeviceGuard guard(updates[0].device());
   const hipStream_t s = c10::hip::getCurrentHIPStream().stream();
   std::vector<Tensor> keep;

@@ -425,21 +425,11 @@ std::vector<torch::Tensor> jacobi_eigh_batched(
     std::vector<torch::Tensor> mats);
 
 // defined in vocab_loss_entry.hip
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor,
-           std::vector<std::optional<torch::Tensor>>>
-vocab_loss_forward(torch::Tensor hidden, torch::Tensor weight,
-                   torch::Tensor target, std::optional<torch::Tensor> bias,
-                   int64_t ignore_index, double eps, bool sum, bool mean,
-                   bool need_x, bool need_w, bool need_b);
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> vocab_loss_finish(
-    torch::Tensor up, torch::Tensor hidden, torch::Tensor weight,
-    torch::Tensor ints, bool mean,
-    std::vector<std::optional<torch::Tensor>> kept);
-std::tuple<torch::Tensor, torch::Tensor, torch::Tensor> vocab_loss_backward(
-    torch::Tensor up, torch::Tensor hidden, torch::Tensor weight,
-    std::optional<torch::Tensor> bias, torch::Tensor state,
-    torch::Tensor ints, double eps, bool each, bool mean, bool need_x,
-    bool need_w, bool need_b);
+torch::Tensor linear_cross_entropy(torch::Tensor hidden, torch::Tensor weight,
+                                   torch::Tensor target,
+                                   std::optional<torch::Tensor> bias,
+                                   int64_t ignore_index, double eps,
+                                   int64_t reduction);
 
 // defined in grad_scale.hip
 torch::Tensor grad_norm(std::vector<torch::Tensor> tensors,
@@ -463,12 +453,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "batched LDS-resident Jacobi symmetric eigensolver (packed W, V)");
   m.def("jacobi_eigh_max_dim", &jacobi_eigh_max_dim,
         "largest dim the Jacobi kernel handles");
-  m.def("vocab_loss_forward", &vocab_loss_forward,
+  m.def("linear_cross_entropy", &linear_cross_entropy,
         "cross entropy of a vocabulary projection, no logits in memory");
-  m.def("vocab_loss_backward", &vocab_loss_backward,
-        "gradients of vocab_loss_forward, from its operands");
-  m.def("vocab_loss_finish", &vocab_loss_finish,
-        "gradients that vocab_loss_forward kept, times the upstream factor");
   m.def("grad_norm", &grad_norm,
         "norm over many tensors, and their rescale by it");
   m.def("trust_region", &trust_region,

@@ -34,6 +34,7 @@
 #include "vocab_loss.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 namespace vocab_loss {
@@ -925,11 +926,18 @@ void by_shape(Tile t, F f) {
   }
 }
 
-template <class F>
-void with_lds(F* kernel, int bytes) {
-  check(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel),
+// Allows a kernel its LDS, once on each device.
+template <auto KERNEL>
+void with_lds(int bytes) {
+  static std::atomic<uint64_t> done{0};
+  int device = 0;
+  check(hipGetDevice(&device));
+  const uint64_t bit = 1ull << (device & 63);
+  if (done.load(std::memory_order_relaxed) & bit) return;
+  check(hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL),
                             hipFuncAttributeMaxDynamicSharedMemorySize,
                             bytes));
+  done.fetch_or(bit, std::memory_order_relaxed);
 }
 
 template <class T>
@@ -942,7 +950,7 @@ struct Run {
     p.nt = ceil_div(o.rows, S::BN);
     p.count = o.count;
     p.tgt = o.tgt;
-    with_lds(logits_kernel<T, S, MODE>, S::LDS);
+    with_lds<logits_kernel<T, S, MODE>>(S::LDS);
     logits_kernel<T, S, MODE><<<p.mt * p.nt, S::THREADS, S::LDS, s>>>(
         (const T*)o.w, (const T*)o.x, (const T*)o.bias, grad, p);
     check(hipGetLastError());
@@ -1014,7 +1022,7 @@ struct Run {
     const int splits = o.plan.dx_splits;
     const long ldg = padded(piece);
     const int run = ceil_div(ceil_div(ldg, splits), 64) * 64;
-    with_lds(dx_kernel<T, S>, S::LDS);
+    with_lds<dx_kernel<T, S>>(S::LDS);
     dx_kernel<T, S><<<md * nt * splits, S::THREADS, S::LDS, s>>>(
         (const T*)o.w + v0 * o.ldw, o.ldw, (const T*)b.grad, ldg, piece,
         o.ldx, o.count, md, nt, run, v0 == 0, b.dx_slabs, o.rows * o.ldx);
@@ -1027,7 +1035,7 @@ struct Run {
     const int md = ceil_div(o.ldx, S::BM), vt = ceil_div(piece, S::BN);
     const int splits = o.plan.dw_splits;
     const int run = ceil_div(ceil_div(o.rows, splits), 64) * 64;
-    with_lds(dw_kernel<T, S>, S::LDS);
+    with_lds<dw_kernel<T, S>>(S::LDS);
     dw_kernel<T, S><<<md * vt * splits, S::THREADS, S::LDS, s>>>(
         (const T*)o.x, o.ldx, (const T*)b.grad, padded(piece), piece, o.dim,
         o.ldx, o.count, md, vt, run, factor(o, b), (T*)b.dw + v0 * o.dim,

@@ -1,17 +1,22 @@
-// Entry points of the vocabulary-loss kernels: checks, workspaces, streams.
+// Entry point of the vocabulary loss on the GPU: checks, autocast, autograd,
+// workspaces, streams.
 #include <torch/extension.h>
 
+#include <ATen/autocast_mode.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include "vocab_loss.h"
 
 #include <optional>
-#include <tuple>
+#include <vector>
 
 namespace {
 
 using torch::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
 using vocab_loss::Type;
 
 Type type_of(const Tensor& t) {
@@ -20,19 +25,28 @@ Type type_of(const Tensor& t) {
     case at::kHalf: return Type::fp16;
     case at::kFloat: return Type::fp32;
     default:
-      TORCH_CHECK(false, "linear_cross_entropy: dtype must be bf16, fp16 or "
-                         "fp32, got ", t.scalar_type());
+      TORCH_CHECK_TYPE(false, "linear_cross_entropy: bf16, fp16 or fp32 "
+                              "expected on the GPU, got ", t.scalar_type());
   }
 }
 
-// The integers of a call, one buffer: count, then three arrays over the rows.
-struct Ints {
+enum Reduction { NONE, MEAN, SUM };
+
+// What a call keeps of its rows, one buffer of 32-bit values: the count, three
+// arrays of whole numbers and three of floats.
+struct State {
   int *count, *pos, *idx, *tgt;
-  Ints(const Tensor& t, long rows) {
+  float *rowm, *rowi, *ztgt;
+
+  static long size(long rows) { return 4 + 6 * rows; }
+  State(const Tensor& t, long rows) {
     count = t.data_ptr<int>();
     pos = count + 4;
     idx = pos + rows;
     tgt = idx + rows;
+    rowm = reinterpret_cast<float*>(tgt + rows);
+    rowi = rowm + rows;
+    ztgt = rowi + rows;
   }
 };
 
@@ -55,8 +69,7 @@ struct Call {
 };
 
 Call make_call(const Tensor& hidden, const Tensor& weight,
-               const std::optional<Tensor>& bias, const Tensor& ints_t,
-               double eps, bool keep) {
+               const State& state, double eps, bool keep) {
   Call c;
   c.type = type_of(hidden);
   c.size = (int)hidden.element_size();
@@ -67,25 +80,15 @@ Call make_call(const Tensor& hidden, const Tensor& weight,
   o.ldx = (int)vocab_loss::padded(o.dim);
   o.eps = (float)eps;
   o.plan = vocab_loss::plan(o.rows, o.vocab, o.ldx, c.size, keep);
-  const Ints ints(ints_t, o.rows);
-  o.pos = ints.pos;
-  o.idx = ints.idx;
-  o.tgt = ints.tgt;
-  o.count = ints.count;
+  o.pos = state.pos;
+  o.idx = state.idx;
+  o.tgt = state.tgt;
+  o.count = state.count;
   return c;
 }
 
-void pack_hidden(Call* c, const Tensor& hidden, hipStream_t stream) {
-  auto& o = c->o;
-  c->x = at::empty({o.rows, o.ldx}, hidden.options());
-  vocab_loss::pack(c->type, hidden.data_ptr(), hidden.stride(0),
-                   hidden.stride(1), o.rows, o.dim, o.idx, o.count,
-                   c->x.data_ptr(), o.ldx, stream);
-  o.x = c->x.data_ptr();
-}
-
-void pack_weight(Call* c, const Tensor& weight,
-                 const std::optional<Tensor>& bias, hipStream_t stream) {
+void pack_weight(Call* c, const Tensor& weight, const Tensor& bias,
+                 hipStream_t stream) {
   auto& o = c->o;
   if (direct(weight)) {
     c->w = weight;
@@ -98,8 +101,8 @@ void pack_weight(Call* c, const Tensor& weight,
     o.ldw = o.ldx;
   }
   o.w = c->w.data_ptr();
-  if (bias) {
-    c->b = bias->contiguous();
+  if (bias.defined()) {
+    c->b = bias.contiguous();
     o.bias = c->b.data_ptr();
   }
 }
@@ -112,7 +115,8 @@ void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // The powers of a whole call are kept up to this many bytes (while the call
 // lasts); beyond, the backward pass makes the logits again.  Kept, 8192 x
-// 128000 x 4096 in bf16 takes 2 GiB and a quarter less time.
+// 128000 x 4096 in bf16 takes 2 GiB and a fifth less time (25.7 against 20.8
+// ms).
 constexpr long MOST_KEPT = 4l << 30;
 
 bool keeps(long rows, long vocab, int size) {
@@ -120,212 +124,336 @@ bool keeps(long rows, long vocab, int size) {
   return row < (1l << 22) && rows * row <= MOST_KEPT;
 }
 
-vocab_loss::Sums row_state(const Tensor& state, long rows) {
-  vocab_loss::Sums f{};
-  f.rowm = state.data_ptr<float>();
-  f.rowi = f.rowm + rows;
-  f.ztgt = f.rowi + rows;
-  return f;
-}
+// What the forward pass leaves for vocab_finish; undefined where not needed.
+struct Kept {
+  Tensor dx_slabs, dw, dw_slabs, pbias;
+};
 
-void check_shapes(const Tensor& hidden, const Tensor& weight,
-                  const std::optional<Tensor>& bias) {
-  TORCH_CHECK(hidden.is_cuda() && weight.device() == hidden.device(),
-              "linear_cross_entropy: hidden and weight must be on one GPU");
-  TORCH_CHECK(hidden.dim() == 2 && weight.dim() == 2 &&
-                  hidden.size(1) == weight.size(1),
-              "linear_cross_entropy: shape mismatch");
-  TORCH_CHECK(hidden.scalar_type() == weight.scalar_type() &&
-                  (!bias || (bias->scalar_type() == weight.scalar_type() &&
-                             bias->device() == weight.device() &&
-                             bias->dim() == 1 &&
-                             bias->size(0) == weight.size(0))),
-              "linear_cross_entropy: hidden, weight and bias must agree");
-  TORCH_CHECK(hidden.size(0) > 0 && hidden.size(1) > 0 && weight.size(0) > 0,
-              "linear_cross_entropy: empty operand");
-  TORCH_CHECK(hidden.size(0) < (1l << 30) && weight.size(0) < (1l << 30) &&
-                  hidden.size(1) * hidden.element_size() < (1l << 22),
-              "linear_cross_entropy: sizes out of range");
-}
+struct Need {
+  bool x, w, b;
+  bool any() const { return x || w || b; }
+};
 
-}  // namespace
+struct Loss {
+  Tensor loss, state;
+  bool keep;
+  Kept kept;
+};
 
-// -> (loss of every row, total or an undefined tensor, state of the kept
-// rows, ints, kept).  kept: what vocab_loss_finish needs, empty where the
-// gradients are left to vocab_loss_backward.
-std::tuple<Tensor, Tensor, Tensor, Tensor, std::vector<std::optional<Tensor>>>
-vocab_loss_forward(Tensor hidden, Tensor weight, Tensor target,
-                   std::optional<Tensor> bias, int64_t ignore_index,
-                   double eps, bool sum, bool mean, bool need_x, bool need_w,
-                   bool need_b) {
-  check_shapes(hidden, weight, bias);
-  const long rows = hidden.size(0), vocab = weight.size(0);
-  TORCH_CHECK(target.device() == hidden.device() && target.dim() == 1 &&
-                  target.size(0) == rows && target.is_contiguous() &&
-                  (target.scalar_type() == at::kLong ||
-                   target.scalar_type() == at::kInt),
-              "linear_cross_entropy: target must be contiguous int32 or "
-              "int64, one for each row, on the same GPU");
+// The loss (a scalar, or of every row).  With gradients needed and a reduced
+// loss it also makes these, for an upstream factor of 1, if the powers fit.
+Loss vocab_forward(const Tensor& hidden, const Tensor& weight,
+                   const Tensor& bias, const Tensor& target,
+                   int64_t ignore_index, double eps, Reduction reduction,
+                   Need need) {
   const c10::OptionalDeviceGuard guard(hidden.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   const auto f32 = hidden.options().dtype(at::kFloat);
-  Tensor ints_t = at::empty({4 + 3 * rows}, f32.dtype(at::kInt));
-  const Ints ints(ints_t, rows);
-  const bool keep = (sum || mean) && (need_x || need_w || need_b) &&
-                    keeps(rows, vocab, (int)hidden.element_size());
-  Call c = make_call(hidden, weight, bias, ints_t, eps, keep);
-  c.x = at::empty({rows, (long)c.o.ldx}, hidden.options());
-  c.o.x = c.x.data_ptr();
-  vocab_loss::prepare(c.type, target.data_ptr(),
-                      target.scalar_type() == at::kLong, rows, ignore_index,
-                      vocab, ints.pos, ints.idx, ints.tgt, ints.count,
-                      hidden.data_ptr(), hidden.stride(0), hidden.stride(1),
-                      c.o.dim, c.x.data_ptr(), c.o.ldx, stream);
-  pack_weight(&c, weight, bias, stream);
+  const long rows = hidden.size(0), vocab = weight.size(0);
+  const bool mean = reduction == MEAN;
+  Loss r;
+  r.state = at::empty({State::size(rows)}, f32.dtype(at::kInt));
+  const State state(r.state, rows);
+  r.keep = reduction != NONE && need.any() &&
+           keeps(rows, vocab, (int)hidden.element_size());
+  Call c = make_call(hidden, weight, state, eps, r.keep);
   const auto& plan = c.o.plan;
 
-  Tensor loss = at::empty({rows}, f32);
-  Tensor state = at::empty({3, rows}, f32);
+  // packed x, then the bands
+  const long xbytes = (rows * c.o.ldx * c.size + 255) / 256 * 256;
   const long bands = rows * plan.bands;
-  Tensor work = at::empty({bands * (eps != 0.0 ? 3 : 2)}, f32);
-  vocab_loss::Sums f = row_state(state, rows);
-  f.pmax = work.data_ptr<float>();
+  Tensor work = at::empty({xbytes / 4 + bands * (eps != 0.0 ? 3 : 2)}, f32);
+  c.o.x = work.data_ptr();
+  vocab_loss::prepare(c.type, target.data_ptr(),
+                      target.scalar_type() == at::kLong, rows, ignore_index,
+                      vocab, state.pos, state.idx, state.tgt, state.count,
+                      hidden.data_ptr(), hidden.stride(0), hidden.stride(1),
+                      c.o.dim, work.data_ptr(), c.o.ldx, stream);
+  pack_weight(&c, weight, bias, stream);
+
+  Tensor each = at::empty({rows}, f32);
+  vocab_loss::Sums f{};
+  f.pmax = work.data_ptr<float>() + xbytes / 4;
   f.psum = f.pmax + bands;
   f.pz = f.psum + bands;
-  f.loss = loss.data_ptr<float>();
+  f.rowm = state.rowm;
+  f.rowi = state.rowi;
+  f.ztgt = state.ztgt;
+  f.loss = each.data_ptr<float>();
   Tensor grad;
-  if (keep) {
+  if (r.keep) {
     grad = at::empty({rows, vocab_loss::padded(vocab)}, hidden.options());
   }
   vocab_loss::forward(c.type, c.o, f, data(grad), stream);
 
-  Tensor total;
-  if (sum || mean) {
-    total = at::empty({}, f32);
-    f.total = total.data_ptr<float>();
-    if (!keep) {
-      vocab_loss::total(f.loss, rows, ints.count, mean, f.total, stream);
+  r.loss = each;
+  if (reduction != NONE) {
+    r.loss = at::empty({}, f32);
+    f.total = r.loss.data_ptr<float>();
+    if (!r.keep) {
+      vocab_loss::total(f.loss, rows, state.count, mean, f.total, stream);
     }
   }
-  std::vector<std::optional<Tensor>> kept;
-  if (keep) {
-    Tensor dx_slabs, dw, dw_slabs, pbias;
-    if (need_x) {
-      dx_slabs = at::empty({plan.dx_splits, rows, (long)c.o.ldx}, f32);
+  if (r.keep) {
+    Kept& k = r.kept;
+    if (need.x) {
+      k.dx_slabs = at::empty({plan.dx_splits, rows, (long)c.o.ldx}, f32);
     }
     // fp16 stays in fp32 until the upstream factor, a loss's scale, is known
-    if (need_w && (plan.dw_splits > 1 || c.type == Type::fp16)) {
-      dw_slabs = at::empty({plan.dw_splits, vocab, (long)c.o.ldx}, f32);
-    } else if (need_w) {
-      dw = at::empty({vocab, (long)c.o.dim}, weight.options());
+    if (need.w && (plan.dw_splits > 1 || c.type == Type::fp16)) {
+      k.dw_slabs = at::empty({plan.dw_splits, vocab, (long)c.o.ldx}, f32);
+    } else if (need.w) {
+      k.dw = at::empty({vocab, (long)c.o.dim}, weight.options());
     }
-    if (need_b) pbias = at::empty({plan.parts, vocab}, f32);
+    if (need.b) k.pbias = at::empty({plan.parts, vocab}, f32);
     vocab_loss::Grads b{};
     b.mean = mean;
-    b.pbias = floats(pbias);
-    b.dx_slabs = floats(dx_slabs);
-    b.dw_slabs = floats(dw_slabs);
+    b.pbias = floats(k.pbias);
+    b.dx_slabs = floats(k.dx_slabs);
+    b.dw_slabs = floats(k.dw_slabs);
     b.grad = data(grad);
-    b.dw = data(dw);
+    b.dw = data(k.dw);
     vocab_loss::gradients_kept(c.type, c.o, f, b, stream);
-    for (const Tensor& t : {dx_slabs, dw, dw_slabs, pbias}) {
-      kept.push_back(t.defined() ? std::optional<Tensor>(t) : std::nullopt);
-    }
   }
-  return {loss, total, state, ints_t, kept};
+  return r;
 }
 
-// The gradients that vocab_loss_forward kept, times up; uses them up.
-// -> (dx, dw, db); those not asked for are undefined
-std::tuple<Tensor, Tensor, Tensor> vocab_loss_finish(
-    Tensor up, Tensor hidden, Tensor weight, Tensor ints_t, bool mean,
-    std::vector<std::optional<Tensor>> kept) {
-  check_shapes(hidden, weight, std::nullopt);
-  TORCH_CHECK(up.device() == hidden.device() && up.numel() == 1 &&
-                  up.scalar_type() == at::kFloat && kept.size() == 4 &&
-                  ints_t.numel() == 4 + 3 * hidden.size(0),
-              "linear_cross_entropy: backward state mismatch");
+struct Gradients {
+  Tensor dx, dw, db;  // undefined where not asked for
+};
+
+// What vocab_forward kept, times up; uses it up.
+Gradients vocab_finish(const Tensor& up, const Tensor& hidden,
+                       const Tensor& weight, const Tensor& state_t, bool mean,
+                       const Kept& k) {
   const c10::OptionalDeviceGuard guard(hidden.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
-  Call c = make_call(hidden, weight, std::nullopt, ints_t, 0.0, true);
-  Tensor dx, dw, db;
-  Tensor dx_slabs = kept[0].value_or(Tensor());
-  Tensor dw_slabs = kept[2].value_or(Tensor());
-  Tensor pbias = kept[3].value_or(Tensor());
-  if (dx_slabs.defined()) {
-    dx = at::empty({c.o.rows, (long)c.o.dim}, hidden.options());
+  const State state(state_t, hidden.size(0));
+  Call c = make_call(hidden, weight, state, 0.0, true);
+  Gradients g;
+  if (k.dx_slabs.defined()) {
+    g.dx = at::empty({c.o.rows, (long)c.o.dim}, hidden.options());
   }
-  if (dw_slabs.defined()) {
-    dw = at::empty({c.o.vocab, (long)c.o.dim}, weight.options());
-  } else if (kept[1]) {
-    dw = *kept[1];
+  if (k.dw_slabs.defined()) {
+    g.dw = at::empty({c.o.vocab, (long)c.o.dim}, weight.options());
+  } else {
+    g.dw = k.dw;
   }
-  if (pbias.defined()) db = at::empty({c.o.vocab}, weight.options());
+  if (k.pbias.defined()) g.db = at::empty({c.o.vocab}, weight.options());
   vocab_loss::Grads b{};
   b.mean = mean;
-  b.pbias = floats(pbias);
-  b.dx_slabs = floats(dx_slabs);
-  b.dw_slabs = floats(dw_slabs);
-  b.dx = data(dx);
-  b.dw = data(dw);
-  b.db = data(db);
+  b.pbias = floats(k.pbias);
+  b.dx_slabs = floats(k.dx_slabs);
+  b.dw_slabs = floats(k.dw_slabs);
+  b.dx = data(g.dx);
+  b.dw = data(g.dw);
+  b.db = data(g.db);
   vocab_loss::finish_kept(c.type, c.o, b, up.data_ptr<float>(), stream);
-  return {dx, dw, db};
+  return g;
 }
 
-// -> (dx, dw, db); those not asked for are undefined
-std::tuple<Tensor, Tensor, Tensor> vocab_loss_backward(
-    Tensor up, Tensor hidden, Tensor weight, std::optional<Tensor> bias,
-    Tensor state, Tensor ints_t, double eps, bool each, bool mean,
-    bool need_x, bool need_w, bool need_b) {
-  check_shapes(hidden, weight, bias);
-  const long rows = hidden.size(0), vocab = weight.size(0);
-  TORCH_CHECK(up.device() == hidden.device() &&
-                  up.scalar_type() == at::kFloat && up.is_contiguous() &&
-                  up.numel() == (each ? rows : 1) &&
-                  state.numel() == 3 * rows &&
-                  ints_t.numel() == 4 + 3 * rows,
-              "linear_cross_entropy: backward state mismatch");
+// The gradients from the operands: the logits are made again.
+Gradients vocab_backward(const Tensor& up, const Tensor& hidden,
+                         const Tensor& weight, const Tensor& bias,
+                         const Tensor& state_t, double eps,
+                         Reduction reduction, Need need) {
   const c10::OptionalDeviceGuard guard(hidden.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   const auto f32 = hidden.options().dtype(at::kFloat);
-  Call c = make_call(hidden, weight, bias, ints_t, eps, false);
-  pack_hidden(&c, hidden, stream);
+  const long rows = hidden.size(0), vocab = weight.size(0);
+  const State state(state_t, rows);
+  Call c = make_call(hidden, weight, state, eps, false);
+  const long dim = c.o.dim, ldx = c.o.ldx;
+  c.x = at::empty({rows, ldx}, hidden.options());
+  vocab_loss::pack(c.type, hidden.data_ptr(), hidden.stride(0),
+                   hidden.stride(1), rows, c.o.dim, c.o.idx, c.o.count,
+                   c.x.data_ptr(), c.o.ldx, stream);
+  c.o.x = c.x.data_ptr();
   pack_weight(&c, weight, bias, stream);
   const auto& plan = c.o.plan;
-  const long dim = c.o.dim, ldx = c.o.ldx;
 
-  Tensor dx, dw, db, pbias, dx_slabs, dw_slabs;
-  if (need_x) {
-    dx = at::empty({rows, dim}, hidden.options());
+  Gradients g;
+  Tensor pbias, dx_slabs, dw_slabs;
+  if (need.x) {
+    g.dx = at::empty({rows, dim}, hidden.options());
     dx_slabs = at::empty({plan.dx_splits, rows, ldx}, f32);
   }
-  if (need_w) {
-    dw = at::empty({vocab, dim}, weight.options());
+  if (need.w) {
+    g.dw = at::empty({vocab, dim}, weight.options());
     if (plan.dw_splits > 1) {
       dw_slabs = at::empty({plan.dw_splits, plan.piece, ldx}, f32);
     }
   }
-  if (need_b) {
-    db = at::empty({vocab}, weight.options());
+  if (need.b) {
+    g.db = at::empty({vocab}, weight.options());
     pbias = at::empty({plan.parts, vocab}, f32);
   }
   Tensor small = at::empty({4 + rows}, f32);
   Tensor grad =
       at::empty({rows, vocab_loss::padded(plan.piece)}, hidden.options());
+  vocab_loss::Sums f{};
+  f.rowm = state.rowm;
+  f.rowi = state.rowi;
+  f.ztgt = state.ztgt;
   vocab_loss::Grads b{};
   b.scale = small.data_ptr<float>();
   b.coef = b.scale + 4;
-  b.mean = mean;
+  b.mean = reduction == MEAN;
   b.pbias = floats(pbias);
   b.dx_slabs = floats(dx_slabs);
   b.dw_slabs = floats(dw_slabs);
   b.grad = data(grad);
-  b.dx = data(dx);
-  b.dw = data(dw);
-  b.db = data(db);
-  vocab_loss::coefficients(c.type, c.o, up.data_ptr<float>(), each, b,
-                           stream);
-  vocab_loss::gradients_again(c.type, c.o, row_state(state, rows), b, stream);
-  return {dx, dw, db};
+  b.dx = data(g.dx);
+  b.dw = data(g.dw);
+  b.db = data(g.db);
+  vocab_loss::coefficients(c.type, c.o, up.data_ptr<float>(),
+                           reduction == NONE, b, stream);
+  vocab_loss::gradients_again(c.type, c.o, f, b, stream);
+  return g;
+}
+
+// A reduced loss leaves its gradients for an upstream factor of 1, which the
+// first backward pass uses up; a loss of single rows, a second backward pass,
+// or a call too large to keep its powers makes the logits again.
+class VocabLoss : public torch::autograd::Function<VocabLoss> {
+ public:
+  static Tensor forward(AutogradContext* ctx, const Tensor& hidden,
+                        const Tensor& weight,
+                        const std::optional<Tensor>& bias,
+                        const Tensor& target, int64_t ignore_index,
+                        double eps, int64_t reduction) {
+    const Tensor b = bias.value_or(Tensor());
+    const Need need{hidden.requires_grad(), weight.requires_grad(),
+                    b.defined() && b.requires_grad()};
+    const Loss r = vocab_forward(hidden, weight, b, target, ignore_index, eps,
+                                 (Reduction)reduction, need);
+    ctx->save_for_backward({hidden, weight, b, r.state});
+    auto& saved = ctx->saved_data;
+    saved["eps"] = eps;
+    saved["reduction"] = reduction;
+    saved["need"] = (int64_t)(need.x | need.w << 1 | need.b << 2);
+    if (r.keep) {
+      // those that are defined, and which they are
+      const Tensor all[] = {r.kept.dx_slabs, r.kept.dw, r.kept.dw_slabs,
+                            r.kept.pbias};
+      std::vector<Tensor> kept;
+      int64_t which = 0;
+      for (int i = 0; i < 4; ++i) {
+        if (!all[i].defined()) continue;
+        kept.push_back(all[i]);
+        which |= 1 << i;
+      }
+      saved["kept"] = kept;
+      saved["which"] = which;
+    }
+    return r.loss;
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list tensors = ctx->get_saved_variables();
+    const Tensor &hidden = tensors[0], &weight = tensors[1],
+                 &bias = tensors[2], &state = tensors[3];
+    auto& saved = ctx->saved_data;
+    const auto reduction = (Reduction)saved["reduction"].toInt();
+    const bool differentiable = at::GradMode::is_enabled();
+    Gradients g;
+    {
+      const at::NoGradGuard none;
+      const Tensor up = grads[0].contiguous();
+      const auto at = saved.find("kept");
+      if (at != saved.end()) {
+        const std::vector<Tensor> kept = at->second.toTensorVector();
+        const int64_t which = saved["which"].toInt();
+        saved.erase(at);
+        Tensor all[4];
+        for (int i = 0, j = 0; i < 4; ++i) {
+          if (which >> i & 1) all[i] = kept[j++];
+        }
+        g = vocab_finish(up, hidden, weight, state, reduction == MEAN,
+                         Kept{all[0], all[1], all[2], all[3]});
+      } else {
+        const int64_t bits = saved["need"].toInt();
+        g = vocab_backward(
+            up, hidden, weight, bias, state, saved["eps"].toDouble(),
+            reduction,
+            Need{(bits & 1) != 0, (bits & 2) != 0, (bits & 4) != 0});
+      }
+    }
+    variable_list out = {g.dx,     g.dw,     g.db,    Tensor(),
+                         Tensor(), Tensor(), Tensor()};
+    if (differentiable) {  // but differentiating these once more is an error
+      for (Tensor& t : out) {
+        if (!t.defined()) continue;
+        const auto error = std::make_shared<torch::autograd::DelayedError>(
+            "linear_cross_entropy has no double backward", 1);
+        t.requires_grad_();
+        t = (*error)({t})[0];
+      }
+    }
+    return out;
+  }
+};
+
+}  // namespace
+
+// hidden (..., d), weight (V, d), target (...), bias (V,) or none; reduction 0:
+// none, 1: mean, 2: sum.  At least one row.
+Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
+                            std::optional<Tensor> bias, int64_t ignore_index,
+                            double eps, int64_t reduction) {
+#define CHECK_VALUE(cond, ...) \
+  TORCH_CHECK_VALUE(cond, "linear_cross_entropy: ", __VA_ARGS__)
+  CHECK_VALUE(eps >= 0.0 && eps <= 1.0,
+              "label_smoothing must be in [0, 1], got ", eps);
+  CHECK_VALUE(hidden.dim() >= 1 && weight.dim() == 2 &&
+                  hidden.size(-1) == weight.size(1),
+              "hidden (..., d) and weight (V, d) expected, got ",
+              hidden.sizes(), " and ", weight.sizes());
+  CHECK_VALUE(target.sizes() == hidden.sizes().slice(0, hidden.dim() - 1),
+              "target must have hidden's shape without its last dimension, "
+              "got ", target.sizes());
+  CHECK_VALUE(!bias || (bias->dim() == 1 && bias->size(0) == weight.size(0)),
+              "bias must have weight's first dimension, got ",
+              bias->sizes());
+  TORCH_CHECK_TYPE(target.scalar_type() == at::kLong ||
+                       target.scalar_type() == at::kInt,
+                   "linear_cross_entropy: target must be int64 or int32, "
+                   "got ", target.scalar_type());
+  CHECK_VALUE(weight.numel() > 0, "weight is empty");
+  CHECK_VALUE(hidden.is_cuda() && weight.device() == hidden.device() &&
+                  target.device() == hidden.device() &&
+                  (!bias || bias->device() == hidden.device()),
+              "all tensors must be on ", hidden.device());
+  if (at::autocast::is_autocast_enabled(at::kCUDA)) {
+    const auto t = at::autocast::get_autocast_dtype(at::kCUDA);
+    hidden = at::autocast::cached_cast(t, hidden, at::kCUDA);
+    weight = at::autocast::cached_cast(t, weight, at::kCUDA);
+    if (bias) bias = at::autocast::cached_cast(t, *bias, at::kCUDA);
+  }
+  TORCH_CHECK_TYPE(hidden.scalar_type() == weight.scalar_type() &&
+                       (!bias || bias->scalar_type() == weight.scalar_type()),
+                   "linear_cross_entropy: hidden, weight and bias must have "
+                   "one dtype, got ", hidden.scalar_type(), ", ",
+                   weight.scalar_type(), bias ? ", " : "",
+                   bias ? c10::toString(bias->scalar_type()) : "");
+  type_of(hidden);
+  const Tensor rows =
+      hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)});
+  const Tensor flat = target.reshape({-1}).contiguous();
+  CHECK_VALUE(rows.size(0) > 0 && rows.size(0) < (1l << 30) &&
+                  weight.size(0) < (1l << 30) &&
+                  rows.size(1) * rows.element_size() < (1l << 22),
+              "sizes out of range: ", rows.sizes(), " and ", weight.sizes());
+#undef CHECK_VALUE
+  const bool grads =
+      at::GradMode::is_enabled() &&
+      (rows.requires_grad() || weight.requires_grad() ||
+       (bias && bias->requires_grad()));
+  const Tensor loss =
+      grads ? VocabLoss::apply(rows, weight, bias, flat, ignore_index, eps,
+                               reduction)
+            : vocab_forward(rows, weight, bias.value_or(Tensor()), flat,
+                            ignore_index, eps, (Reduction)reduction, Need{})
+                  .loss;
+  return reduction == NONE ? loss.view(target.sizes()) : loss;
 }

@@ -22,7 +22,6 @@ __all__ = ["global_norm", "clip_by_global_norm", "clip_grad_norm_",
            "kl_clip"]
 
 _KINDS = {2.0: 0, 1.0: 1, math.inf: 2}
-_TYPES = (torch.float32, torch.bfloat16, torch.float16)
 Tensors = Union[torch.Tensor, Iterable[torch.Tensor]]
 
 
@@ -32,6 +31,8 @@ def _as_list(tensors: Tensors) -> List[torch.Tensor]:
     return list(tensors)
 
 
+# The GPU calls make the same checks in C++, where hundreds of tensors take
+# some microseconds.
 def _check_lists(name: str, *lists: Sequence[torch.Tensor]) -> None:
     first = lists[0]
     for other in lists[1:]:
@@ -51,9 +52,6 @@ def _check_lists(name: str, *lists: Sequence[torch.Tensor]) -> None:
             if not t.dtype.is_floating_point or t.layout != torch.strided:
                 raise TypeError(f"{name}: dense floating tensors expected, "
                                 f"got {t.dtype}, {t.layout}")
-            if t.is_cuda and t.dtype not in _TYPES:
-                raise TypeError(f"{name}: fp32, bf16 or fp16 expected on the "
-                                f"GPU, got {t.dtype}")
 
 
 def _check_outputs(name: str, out: Sequence[torch.Tensor]) -> None:
@@ -91,11 +89,11 @@ def global_norm(tensors: Tensors, norm_type: float = 2.0) -> torch.Tensor:
     kind = _kind("global_norm", norm_type)
     if not tensors:
         return torch.zeros(())
+    if tensors[0].is_cuda:
+        from kfac_pytorch_amd.ops import _ext
+        return _ext.grad_norm(tensors, None, math.inf, kind)[0]
     _check_lists("global_norm", tensors)
-    if not tensors[0].is_cuda:
-        return _cpu_norm(tensors, float(norm_type))
-    from kfac_pytorch_amd.ops import _ext
-    return _ext.grad_norm(tensors, None, math.inf, kind)[0]
+    return _cpu_norm(tensors, float(norm_type))
 
 
 @torch.no_grad()
@@ -116,24 +114,23 @@ def clip_by_global_norm(
     if not max_norm >= 0:
         raise ValueError(f"clip_by_global_norm: max_norm must not be "
                          f"negative, got {max_norm}")
-    if out is None:
-        out = [torch.empty_like(t) for t in tensors]
-    out = _as_list(out)
+    out = [torch.empty_like(t) for t in tensors] if out is None \
+        else _as_list(out)
     if not tensors:
         if out:
             raise ValueError("clip_by_global_norm: out without tensors")
         return out, torch.zeros(())
+    if tensors[0].is_cuda:
+        from kfac_pytorch_amd.ops import _ext
+        return out, _ext.grad_norm(tensors, out, max_norm, kind)[0]
     _check_lists("clip_by_global_norm", tensors, out)
     _check_outputs("clip_by_global_norm", out)
-    if not tensors[0].is_cuda:
-        norm = _cpu_norm(tensors, float(norm_type))
-        factor = (max_norm / (norm.double() + 1e-6)).clamp(max=1.0).float()
-        for t, o in zip(tensors, out):
-            o.copy_(t * factor.to(t.dtype) if t.dtype == torch.float64
-                    else t.float() * factor)
-        return out, norm
-    from kfac_pytorch_amd.ops import _ext
-    return out, _ext.grad_norm(tensors, out, max_norm, kind)[0]
+    norm = _cpu_norm(tensors, float(norm_type))
+    factor = (max_norm / (norm.double() + 1e-6)).clamp(max=1.0).float()
+    for t, o in zip(tensors, out):
+        o.copy_(t * factor.to(t.dtype) if t.dtype == torch.float64
+                else t.float() * factor)
+    return out, norm
 
 
 def clip_grad_norm_(parameters: Tensors, max_norm: float,
@@ -180,16 +177,15 @@ def kl_clip(updates: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], *,
         if grads or out:
             raise ValueError("kl_clip: gradients without updates")
         return out, torch.ones(())
+    if updates[0].is_cuda:
+        from kfac_pytorch_amd.ops import _ext
+        return out, _ext.trust_region(updates, grads, out, lr, kl)
     _check_lists("kl_clip", updates, grads, out)
     _check_outputs("kl_clip", out)
-    if not updates[0].is_cuda:
-        total = sum((u.double() * g.double()).sum()
-                    for u, g in zip(updates, grads)) * lr ** 2
-        nu = (kl / total.abs().clamp_min(1e-30)).sqrt().clamp(max=1.0)
-        nu = nu.float()
-        for u, o in zip(updates, out):
-            o.copy_(u * nu.to(u.dtype) if u.dtype == torch.float64
-                    else u.float() * nu)
-        return out, nu
-    from kfac_pytorch_amd.ops import _ext
-    return out, _ext.trust_region(updates, grads, out, lr, kl)
+    total = sum((u.double() * g.double()).sum()
+                for u, g in zip(updates, grads)) * lr ** 2
+    nu = (kl / total.abs().clamp_min(1e-30)).sqrt().clamp(max=1.0).float()
+    for u, o in zip(updates, out):
+        o.copy_(u * nu.to(u.dtype) if u.dtype == torch.float64
+                else u.float() * nu)
+    return out, nu

@@ -27,52 +27,10 @@ import torch.nn.functional as F
 
 __all__ = ["linear_cross_entropy", "projection_loss"]
 
-_REDUCTIONS = ("mean", "sum", "none")
-_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 
 
-class _VocabLoss(torch.autograd.Function):
-    """A reduced loss leaves its gradients for an upstream factor of 1, which
-    the first backward pass uses up; a loss of single rows, a second backward
-    pass, or a call too large to keep its probabilities makes the logits
-    again."""
-
-    @staticmethod
-    def forward(ctx, hidden, weight, bias, target, ignore_index, eps,
-                reduction):
-        from kfac_pytorch_amd.ops import _ext
-        need = (ctx.needs_input_grad[0], ctx.needs_input_grad[1],
-                bias is not None and ctx.needs_input_grad[2])
-        loss, total, state, ints, kept = _ext.vocab_loss_forward(
-            hidden, weight, target, bias, ignore_index, eps, reduction, need)
-        ctx.save_for_backward(hidden, weight, bias, state, ints)
-        ctx.kept = kept
-        ctx.need = need
-        ctx.eps = eps
-        ctx.reduction = reduction
-        return loss if reduction == "none" else total
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, up):
-        from kfac_pytorch_amd.ops import _ext
-        hidden, weight, bias, state, ints = ctx.saved_tensors
-        up = up.contiguous()
-        kept, ctx.kept = ctx.kept, None
-        if kept:
-            dx, dw, db = _ext.vocab_loss_finish(
-                up, hidden, weight, ints, ctx.reduction, kept)
-        else:
-            dx, dw, db = _ext.vocab_loss_backward(
-                up, hidden, weight, bias, state, ints, ctx.eps,
-                ctx.reduction, ctx.need)
-        return dx, dw, db, None, None, None, None
-
-
-def _check(hidden, weight, target, bias, label_smoothing, reduction):
-    if reduction not in _REDUCTIONS:
-        raise ValueError(f"linear_cross_entropy: reduction must be one of "
-                         f"{_REDUCTIONS}, got {reduction!r}")
+def _check(hidden, weight, target, bias, label_smoothing):
     if not 0.0 <= label_smoothing <= 1.0:
         raise ValueError("linear_cross_entropy: label_smoothing must be in "
                          f"[0, 1], got {label_smoothing}")
@@ -131,7 +89,18 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
     if that is 4 GiB at most; else, and for ``"none"``, 256 MB pieces of it
     during the backward pass.
     """
-    _check(hidden, weight, target, bias, label_smoothing, reduction)
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"linear_cross_entropy: reduction must be one of "
+                         f"{tuple(_REDUCTIONS)}, got {reduction!r}")
+    if hidden.is_cuda and target.numel():
+        # the same checks, autocast and autograd are behind this call: a
+        # step's last operator is short enough for Python to be seen
+        from kfac_pytorch_amd.ops import _ext
+        return _ext.linear_cross_entropy(hidden, weight, target, bias,
+                                         ignore_index, label_smoothing,
+                                         _REDUCTIONS[reduction])
+
+    _check(hidden, weight, target, bias, label_smoothing)
     kind = hidden.device.type
     if torch.is_autocast_enabled(kind):
         t = torch.get_autocast_dtype(kind)
@@ -142,42 +111,14 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
         raise TypeError("linear_cross_entropy: hidden, weight and bias must "
                         f"have one dtype, got {hidden.dtype}, {weight.dtype}"
                         + (f", {bias.dtype}" if bias is not None else ""))
-
-    if not hidden.is_cuda:
-        wide = (lambda a: a if a is None or a.dtype == torch.float64
-                else a.float())
-        with torch.autocast(kind, enabled=False):
-            z = F.linear(wide(hidden), wide(weight), wide(bias))
-            loss = F.cross_entropy(
-                z.reshape(-1, z.size(-1)), target.reshape(-1).long(),
-                ignore_index=ignore_index, label_smoothing=label_smoothing,
-                reduction=reduction)
-        return loss.view(target.shape) if reduction == "none" else loss
-
-    if hidden.dtype not in _TYPES:
-        raise TypeError("linear_cross_entropy: bf16, fp16 or fp32 expected "
-                        f"on the GPU, got {hidden.dtype}")
-    rows = hidden.reshape(-1, hidden.size(-1))
-    if rows.size(0) == 0:
-        # F.cross_entropy's values, with a graph to hidden, weight and bias
-        zero = rows.sum() + weight[:0].sum()
-        zero = zero + (bias[:0].sum() if bias is not None else 0.0)
-        if reduction == "none":
-            return zero.float() + torch.empty(
-                target.shape, device=hidden.device)
-        return zero.float() / 0.0 if reduction == "mean" else zero.float()
-    flat = target.reshape(-1).contiguous()
-    if torch.is_grad_enabled() and (
-            rows.requires_grad or weight.requires_grad
-            or (bias is not None and bias.requires_grad)):
-        loss = _VocabLoss.apply(rows, weight, bias, flat, int(ignore_index),
-                                float(label_smoothing), reduction)
-    else:
-        from kfac_pytorch_amd.ops import _ext
-        loss, total, _, _, _ = _ext.vocab_loss_forward(
-            rows, weight, flat, bias, int(ignore_index),
-            float(label_smoothing), reduction)
-        loss = loss if reduction == "none" else total
+    wide = (lambda a: a if a is None or a.dtype == torch.float64
+            else a.float())
+    with torch.autocast(kind, enabled=False):
+        z = F.linear(wide(hidden), wide(weight), wide(bias))
+        loss = F.cross_entropy(
+            z.reshape(-1, z.size(-1)), target.reshape(-1).long(),
+            ignore_index=ignore_index, label_smoothing=label_smoothing,
+            reduction=reduction)
     return loss.view(target.shape) if reduction == "none" else loss
 
 

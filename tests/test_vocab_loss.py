@@ -243,6 +243,22 @@ def test_backward_twice(dtype):
 
 @pytest.mark.gpu
 @needs_gpu
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_no_double_backward(reduction):
+    x, w, b, t = inputs(9, 16, 30, torch.float32, False)
+    x.requires_grad_()
+    loss = ops.linear_cross_entropy(x, w, t, reduction=reduction).sum()
+    dx, = torch.autograd.grad(loss, x, create_graph=True)
+    want, = torch.autograd.grad(
+        F.cross_entropy(x @ w.t(), t, reduction=reduction).sum(), x)
+    # sums of up to 30 terms of at most 1 * 4
+    assert (dx - want).abs().max() <= 64 * 2.0 ** -24 * 4
+    with pytest.raises(RuntimeError, match="double backward"):
+        dx.sum().backward()
+
+
+@pytest.mark.gpu
+@needs_gpu
 def test_ignored_rows_may_hold_anything():
     x, w, b, t = inputs(130, 64, 300, torch.bfloat16, True, 0.4, 3)
     want = run(x, w, b, t)
