@@ -44,14 +44,15 @@ constexpr int UNROLL = 4;
 constexpr int CHUNK = THREADS * UNROLL;    // groups of a chunk
 constexpr int MOST_BLOCKS = 8192;
 
-// NP operands seen as rows x cols, neighbouring columns next to each other
+// NP operands seen as rows x columns, neighbouring columns next to each other,
+// in groups of 16 bytes of the first operand.
 template <int NP>
 struct Entry {
   const void* p[NP];
-  long ld[NP];
+  int ld[NP];             // values from a row to the next
   unsigned rows, groups;  // groups of a row
-  long cols;
-  unsigned start, pad;    // first chunk
+  unsigned tail;          // values of a row's last group
+  unsigned start;         // first chunk
 };
 
 // kernel arguments stay below 4 KB
@@ -116,8 +117,8 @@ __device__ __forceinline__ int find(const List<NP>& list, unsigned chunk) {
 }
 
 struct Place {
-  long row;
-  long col;
+  unsigned row;
+  unsigned long col;
   int have;  // values of the group, 0 past the end
 };
 
@@ -127,20 +128,20 @@ __device__ __forceinline__ Place place(const Entry<NP>& e, unsigned chunk,
   const unsigned long g = (unsigned long)(chunk - e.start) * CHUNK +
                           (unsigned)(k * THREADS) + threadIdx.x;
   Place at;
+  unsigned in;  // group within its row
+  bool there;
   if (e.rows == 1) {
     at.row = 0;
-    at.col = (long)g * N;
-    at.have = g < e.groups ? (int)std::min<long>(N, e.cols - at.col) : 0;
+    in = (unsigned)g;
+    there = g < e.groups;
   } else {
-    // rows of many: the host keeps rows * groups below 2^32
-    const unsigned s = (unsigned)g;
-    const unsigned r = s / e.groups;
-    at.row = r;
-    at.col = (long)(s - r * e.groups) * N;
-    at.have = g < (unsigned long)e.rows * e.groups
-                  ? (int)std::min<long>(N, e.cols - at.col)
-                  : 0;
+    // the host keeps rows * groups below 2^32
+    at.row = (unsigned)g / e.groups;
+    in = (unsigned)g - at.row * e.groups;
+    there = g < (unsigned long)e.rows * e.groups;
   }
+  at.col = (unsigned long)in * N;
+  at.have = !there ? 0 : in == e.groups - 1 ? (int)e.tail : N;
   return at;
 }
 
@@ -181,7 +182,7 @@ __global__ __launch_bounds__(THREADS) void norm_kernel(
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
       const Place at = place<1, N>(e, chunk, k);
-      fetch((const T*)e.p[0] + at.row * e.ld[0] + at.col, at.have, f[k]);
+      fetch((const T*)e.p[0] + (long)at.row * e.ld[0] + at.col, at.have, f[k]);
     }
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
@@ -215,8 +216,8 @@ __global__ __launch_bounds__(THREADS) void dot_kernel(
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
       const Place at = place<2, N>(e, chunk, k);
-      fetch((const U*)e.p[0] + at.row * e.ld[0] + at.col, at.have, u[k]);
-      fetch((const G*)e.p[1] + at.row * e.ld[1] + at.col, at.have, g[k]);
+      fetch((const U*)e.p[0] + (long)at.row * e.ld[0] + at.col, at.have, u[k]);
+      fetch((const G*)e.p[1] + (long)at.row * e.ld[1] + at.col, at.have, g[k]);
     }
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
@@ -280,28 +281,35 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
       const Place at = place<2, N>(e, chunk, k);
-      fetch((const I*)e.p[0] + at.row * e.ld[0] + at.col, at.have, v[k]);
+      fetch((const I*)e.p[0] + (long)at.row * e.ld[0] + at.col, at.have, v[k]);
     }
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
       const Place at = place<2, N>(e, chunk, k);
 #pragma unroll
       for (int i = 0; i < N; ++i) v[k][i] *= f;
-      put((O*)const_cast<void*>(e.p[1]) + at.row * e.ld[1] + at.col, at.have,
+      put((O*)const_cast<void*>(e.p[1]) + (long)at.row * e.ld[1] + at.col, at.have,
           v[k]);
     }
   }
 }
 
 // ------------------------------------------------------------------- host
+template <int NP>
+struct Item {
+  Entry<NP> e;
+  long cols;
+};
+
 // Several operands of one shape as rows x cols with unit column stride;
 // false where they are not so.
 template <int NP>
-bool as_rows(const std::array<const Tensor*, NP>& t, Entry<NP>* e) {
+bool as_rows(const std::array<const Tensor*, NP>& t, Item<NP>* item) {
+  Entry<NP>* e = &item->e;
   bool dense = true;
   for (int i = 0; i < NP; ++i) dense &= t[i]->is_contiguous();
   if (dense) {
-    e->cols = t[0]->numel();
+    item->cols = t[0]->numel();
     e->rows = 1;
     for (int i = 0; i < NP; ++i) {
       e->p[i] = t[i]->const_data_ptr();
@@ -347,10 +355,12 @@ bool as_rows(const std::array<const Tensor*, NP>& t, Entry<NP>* e) {
   }
   if (kept.size() > 2) return false;
   const long rows = kept.size() == 2 ? kept[0].size : 1;
-  e->cols = kept.back().size;
+  item->cols = kept.back().size;
   for (int i = 0; i < NP; ++i) {
     e->p[i] = t[i]->const_data_ptr();
-    e->ld[i] = kept.size() == 2 ? kept[0].stride[i] : 0;
+    const long ld = kept.size() == 2 ? kept[0].stride[i] : 0;
+    if (ld >= (1l << 31)) return false;
+    e->ld[i] = (int)ld;
   }
   if (rows >= (1l << 31)) return false;
   e->rows = (unsigned)rows;
@@ -359,44 +369,46 @@ bool as_rows(const std::array<const Tensor*, NP>& t, Entry<NP>* e) {
 
 template <int NP>
 struct Batch {
-  std::vector<Entry<NP>> entries;
+  std::vector<Item<NP>> items;
 
   // sizes: bytes of a value of each operand
-  void add(Entry<NP> e, const std::array<long, NP>& sizes) {
-    if (!entries.empty() && e.rows == 1 && entries.back().rows == 1) {
-      Entry<NP>& last = entries.back();
+  void add(const Item<NP>& item, const std::array<long, NP>& sizes) {
+    if (!items.empty() && item.e.rows == 1 && items.back().e.rows == 1) {
+      Item<NP>& last = items.back();
       bool joins = true;
       for (int i = 0; i < NP; ++i) {
-        joins &= (const char*)last.p[i] + last.cols * sizes[i] ==
-                 (const char*)e.p[i];
+        joins &= (const char*)last.e.p[i] + last.cols * sizes[i] ==
+                 (const char*)item.e.p[i];
       }
       if (joins) {
-        last.cols += e.cols;
+        last.cols += item.cols;
         return;
       }
     }
-    entries.push_back(e);
+    items.push_back(item);
   }
 
-  // groups of `n` values; splits what 32 bits cannot count
+  // groups of `n` values
   void group(int n) {
-    for (auto& e : entries) {
-      const long g = (e.cols + n - 1) / n;
-      TORCH_CHECK(g < (1l << 32) && (e.rows == 1 || g * e.rows < (1l << 32)),
+    for (auto& item : items) {
+      const long g = (item.cols + n - 1) / n;
+      TORCH_CHECK(g < (1l << 32) &&
+                      (item.e.rows == 1 || g * item.e.rows < (1l << 32)),
                   "tensor too large");
-      e.groups = (unsigned)g;
+      item.e.groups = (unsigned)g;
+      item.e.tail = (unsigned)(item.cols - (g - 1) * n);
     }
   }
 
   template <class F>
   void launch(F f) {
-    for (size_t first = 0; first < entries.size();
+    for (size_t first = 0; first < items.size();
          first += List<NP>::MAX) {
       List<NP> list;
-      list.n = (int)std::min<size_t>(List<NP>::MAX, entries.size() - first);
+      list.n = (int)std::min<size_t>(List<NP>::MAX, items.size() - first);
       unsigned at = 0;
       for (int i = 0; i < list.n; ++i) {
-        list.e[i] = entries[first + i];
+        list.e[i] = items[first + i].e;
         list.e[i].start = at;
         at += (unsigned)(((unsigned long)list.e[i].rows *
                               list.e[i].groups + CHUNK - 1) / CHUNK);
@@ -469,8 +481,8 @@ constexpr at::ScalarType TYPES[] = {at::kFloat, at::kBFloat16, at::kHalf};
 
 
 template <int NP>
-Entry<NP> must(const std::array<const Tensor*, NP>& t) {
-  Entry<NP> e{};
+Item<NP> must(const std::array<const Tensor*, NP>& t) {
+  Item<NP> e{};
   TORCH_CHECK(as_rows<NP>(t, &e), "tensor layout");
   return e;
 }
@@ -486,7 +498,7 @@ void scale_pass(const std::vector<Tensor>& in, const std::vector<Tensor>& out,
             in[i].numel() == 0) {
           continue;
         }
-        Entry<2> e{};
+        Item<2> e{};
         if (!as_rows<2>({&in[i], &out[i]}, &e)) {
           Tensor a = in[i].contiguous();
           Tensor b = at::empty(out[i].sizes(), out[i].options());
@@ -497,7 +509,7 @@ void scale_pass(const std::vector<Tensor>& in, const std::vector<Tensor>& out,
         batch.add(e, {(long)in[i].element_size(),
                       (long)out[i].element_size()});
       }
-      if (batch.entries.empty()) continue;
+      if (batch.items.empty()) continue;
       by_type(ti, [&](auto* pi) {
         using I = std::remove_pointer_t<decltype(pi)>;
         by_type(to, [&](auto* po) {
@@ -537,7 +549,7 @@ Tensor grad_norm(std::vector<Tensor> tensors,
   for (int k = 0; k < 3; ++k) {
     for (const Tensor& t : tensors) {
       if (t.scalar_type() != TYPES[k] || t.numel() == 0) continue;
-      Entry<1> e{};
+      Item<1> e{};
       if (!as_rows<1>({&t}, &e)) {
         keep.push_back(t.contiguous());
         e = must<1>({&keep.back()});
@@ -598,7 +610,7 @@ Tensor trust_region(std::vector<Tensor> updates, std::vector<Tensor> grads,
           updates[i].numel() == 0) {
         continue;
       }
-      Entry<2> e{};
+      Item<2> e{};
       if (!as_rows<2>({&updates[i], &grads[i]}, &e)) {
         keep.push_back(updates[i].contiguous());
         keep.push_back(grads[i].contiguous());
@@ -615,7 +627,7 @@ Tensor trust_region(std::vector<Tensor> updates, std::vector<Tensor> grads,
   Tensor sums = at::empty({std::max(blocks, 1)}, f32.dtype(at::kDouble));
   double* at_sums = sums.data_ptr<double>();
   for (int k = 0; k < 9; ++k) {
-    if (batch[k].entries.empty()) continue;
+    if (batch[k].items.empty()) continue;
     by_type(TYPES[k / 3], [&](auto* pu) {
       using U = std::remove_pointer_t<decltype(pu)>;
       by_type(TYPES[k % 3], [&](auto* pg) {
