@@ -64,12 +64,17 @@ __device__ __forceinline__ void load_to_lds(Rsrc r, char* to, uint32_t off,
       : "m0", "memory");
 }
 
-// all loads to LDS of this wave have arrived, all its LDS reads too, and the
-// other waves are as far
+// All LDS reads of this wave have arrived and all but its last LATER loads to
+// LDS, and the other waves are as far.  (vmcnt counts loads in the order they
+// were started; other accesses in flight only make the wait longer.)
+template <int LATER>
 __device__ __forceinline__ void arrive() {
+  static_assert(LATER < 64, "six bits of count");
   __builtin_amdgcn_sched_barrier(0);
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
+  __builtin_amdgcn_s_waitcnt((LATER & 15) | 7 << 4 | (LATER >> 4) << 14);
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
   __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -127,13 +132,14 @@ __device__ __forceinline__ void spread() {
   __builtin_amdgcn_sched_group_barrier(0x008, MATRIX, 0);
 }
 
-// A tile shape: BM x BN of C by WM x WN waves.
-template <int BM_, int BN_, int WM_, int WN_>
+// A tile shape: BM x BN of C by WM x WN waves, with ST slices of k in LDS or
+// on their way there.
+template <int BM_, int BN_, int WM_, int WN_, int ST_ = 2>
 struct Shape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, ST = ST_;
   static constexpr int NW = WM * WN, THREADS = NW * 64;
   static constexpr int MI = BM / WM / 16, NI = BN / WN / 16;
-  static constexpr int LDS = 2 * (BM + BN) * 128;
+  static constexpr int SLICE = (BM + BN) * 128, LDS = ST * SLICE;
 };
 
 // One operand of a tile: R rows (of C's rows or columns).
@@ -273,12 +279,10 @@ __device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
   a.init(A, lda, m0, M, KA ? krows : kend, wave, lane);
   b.init(B, ldb, n0, N, KB ? krows : kend, wave, lane);
 
-  // Two slices are in LDS or on their way there, and two halves of a slice
+  // S::ST slices are in LDS or on their way there, and two halves of a slice
   // in registers: the matrix cores work on one half while the other is read.
   // Loads and reads past the last slice are harmless (zeros, unused), which
   // keeps the loop free of branches.
-  char* cur = smem;
-  char* nxt = smem + S::LDS / 2;
   Frag fa[2][S::MI], fb[2][S::NI];
   constexpr int FRAGS = S::MI + S::NI, LOADS = OA::LOADS + OB::LOADS;
   // one fragment of half ks; those of B first, the first products need them
@@ -307,36 +311,44 @@ __device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
   };
   a.start(kbeg);
   b.start(kbeg);
+  int issued = kbeg;  // k of the next slice to be loaded
+  auto load_slice = [&](char* lds) {
 #pragma unroll
-  for (int j = 0; j < LOADS; ++j) load(cur, kbeg, j);
-  a.next();
-  b.next();
-  arrive();
+    for (int j = 0; j < LOADS; ++j) load(lds, issued, j);
+    a.next();
+    b.next();
+    issued += BK;
+  };
 #pragma unroll
-  for (int j = 0; j < LOADS; ++j) load(nxt, kbeg + BK, j);
+  for (int t = 0; t < S::ST - 1; ++t) load_slice(smem + t * S::SLICE);
+  arrive<(S::ST - 2) * LOADS>();
+  load_slice(smem + (S::ST - 1) * S::SLICE);
+  char* cur = smem;
 #pragma unroll
   for (int i = 0; i < FRAGS; ++i) read(cur, 0, 0, i);
   for (int k0 = kbeg; k0 < kend; k0 += BK) {
+    char* nxt = cur + S::SLICE;
+    if (nxt == smem + S::LDS) nxt = smem;
 #pragma unroll
     for (int i = 0; i < FRAGS; ++i) read(cur, 1, 1, i);
-    a.next();
-    b.next();
     multiply(0);
     spread<S::MI * S::NI * MMAS<T>, S::MI * OA::READS + S::NI * OB::READS>();
-    arrive();  // cur is in registers, nxt is in LDS
+    // cur is in registers, nxt in LDS
+    arrive<(S::ST - 2) * LOADS>();
     // the compiler keeps reads and loads, both of LDS, in this order
 #pragma unroll
     for (int i = 0; i < (FRAGS > LOADS ? FRAGS : LOADS); ++i) {
       if (i < FRAGS) read(nxt, 0, 0, i);
-      if (i < LOADS) load(cur, k0 + 2 * BK, i);
+      if (i < LOADS) load(cur, issued, i);
     }
+    issued += BK;
+    a.next();
+    b.next();
     multiply(1);
     spread<S::MI * S::NI * MMAS<T>, S::MI * OA::READS + S::NI * OB::READS>();
-    char* t = cur;
     cur = nxt;
-    nxt = t;
   }
-  arrive();
+  arrive<0>();
 }
 
 // Writes 16 columns of a wave's part of C, ROWS rows each, as rows of memory:

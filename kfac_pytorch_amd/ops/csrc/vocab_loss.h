@@ -20,7 +20,9 @@ inline void check(hipError_t e) {
   }
 }
 
-enum class Tile { wide, mid, small };  // 256 x 256, 128 x 128, 128 x 64
+// 256 x 256, 128 x 128, 128 x 64; 64 x 64 and 64 x 32 with more slices of k on
+// their way
+enum class Tile { wide, mid, small, deep, thin };
 
 // How a call of given sizes is cut up.
 struct Plan {

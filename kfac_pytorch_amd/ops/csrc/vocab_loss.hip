@@ -69,12 +69,14 @@ __device__ __forceinline__ float power(float z, float m) {
   return __builtin_amdgcn_exp2f(fmaf(z, LOG2E, -m));
 }
 
-// Powers are at most 2^0.5; fp16 gets them times 2^15, so that those down to
-// 2^-29 of the largest keep all their bits.
+// The type that powers are kept in: 16 bits are best used as fp16, also for
+// bf16 (gradients off by 2.1e-3 of their norm instead of 2.6e-3).  A power is
+// at most 2^0.5; times 2^15, those down to 2^-29 of a band's largest keep all
+// 11 bits.
 template <class T>
-constexpr float LIFT = 1.f;
-template <>
-constexpr float LIFT<_Float16> = 32768.f;
+using Power = std::conditional_t<sizeof(T) == 2, _Float16, float>;
+template <class T>
+constexpr float LIFT = sizeof(T) == 2 ? 32768.f : 1.f;
 
 // ------------------------------------------------------- kept rows, one block
 // pos[n]: the row's place among the kept ones, or -1; idx, tgt: the kept rows'
@@ -362,20 +364,20 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
       const float ref = safe(m);
       const int n = nbase + ni * 16;
       float s = 0.f;
-      T out[S::MI][4];
+      Power<T> out[S::MI][4];
 #pragma unroll
       for (int mi = 0; mi < S::MI; ++mi) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float e = power(acc[mi][ni][r], ref);
           s += e;
-          out[mi][r] = (T)(e * LIFT<T>);
+          out[mi][r] = (Power<T>)(e * LIFT<T>);
         }
       }
       if constexpr (MODE == KEEP) {
-        tile::store_columns<T, S::MI * 16>(
+        tile::store_columns<Power<T>, S::MI * 16>(
             out, stage + (ni & 1) * (S::MI * 256 * sizeof(T)),
-            grad + (long)(n0 + wcol + ni * 16) * p.ldg + m0 + wrow, p.ldg,
+            reinterpret_cast<Power<T>*>(grad) + (long)(n0 + wcol + ni * 16) * p.ldg + m0 + wrow, p.ldg,
             rows - (n0 + wcol + ni * 16), (int)p.ldg - (m0 + wrow), lane);
       }
       s += __shfl_xor(s, 16);
@@ -616,11 +618,15 @@ __global__ __launch_bounds__(256) void probs_kernel(
   float sum[E] = {};
 #pragma unroll 8
   for (int n = n0; n < n1; ++n) {
+    struct alignas(16) Powers {
+      Power<T> v[E];
+    };
     struct alignas(16) Chunk {
       T v[E];
     };
-    Chunk* at = reinterpret_cast<Chunk*>(grad + (long)n * ldg + v);
-    Chunk t = *at;
+    T* at = grad + (long)n * ldg + v;
+    const Powers t = *reinterpret_cast<const Powers*>(at);
+    Chunk g;
     const float m = rowm[n], i = rowi[n];
     const float k = __builtin_amdgcn_exp2f(safe(pmax[(long)n * bands + mine]) -
                                            m) * i * c * (1.f / LIFT<T>);
@@ -631,9 +637,9 @@ __global__ __launch_bounds__(256) void probs_kernel(
       if (hit == j) d = (power(ztgt[n], m) * i - share - (1.f - eps)) * c;
       d = v + j < vocab ? d : 0.f;
       sum[j] += d;
-      t.v[j] = (T)d;
+      g.v[j] = (T)d;
     }
-    *at = t;
+    *reinterpret_cast<Chunk*>(at) = g;
   }
   if (pbias) {
 #pragma unroll
@@ -915,6 +921,8 @@ int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 using Wide = Shape<256, 256, 2, 4>;
 using Mid = Shape<128, 128, 2, 4>;
 using Small = Shape<128, 64, 2, 2>;
+using Deep = Shape<64, 64, 2, 2, 5>;
+using Thin = Shape<64, 32, 2, 2, 4>;
 
 // calls f with a value of the tile's shape
 template <class F>
@@ -923,6 +931,8 @@ void by_shape(Tile t, F f) {
     case Tile::wide: f(Wide()); break;
     case Tile::mid: f(Mid()); break;
     case Tile::small: f(Small()); break;
+    case Tile::deep: f(Deep()); break;
+    case Tile::thin: f(Thin()); break;
   }
 }
 
@@ -1097,26 +1107,38 @@ void by_type(Type t, F f) {
   }
 }
 
-constexpr int EDGE_M[] = {256, 128, 128};
-constexpr int EDGE_N[] = {256, 128, 64};
-constexpr int BAND[] = {128, 64, 64};
-// workgroups that run at once: one, two and three for each of 256 CUs
-constexpr int SLOTS[] = {256, 512, 768};
+constexpr int EDGE_M[] = {256, 128, 128, 64, 64};
+constexpr int EDGE_N[] = {256, 128, 64, 64, 32};
+constexpr int BAND[] = {128, 64, 64, 32, 32};
+// workgroups that run at once: one to three for each of 256 CUs
+constexpr int SLOTS[] = {256, 512, 768, 512, 768};
 
 long tiles(Tile t, long m, long n) {
   return (long)ceil_div(m, EDGE_M[(int)t]) * ceil_div(n, EDGE_N[(int)t]);
 }
 
-// Wide tiles do twice the work per byte that goes through LDS, but one
-// workgroup fills a CU: they pay once there are enough for all CUs (8192 x
-// 16384 x 768 in bf16: 217 us against 251; 300 x 9521 x 512: 19.6 against
-// 9.6).  fp32 products are 16 times slower for the same loads, so small tiles,
-// three workgroups to a CU, lose nothing and leave less of a last round (700 x
-// 33278 x 256: 108 us against 138 and 124); so do a few rows (35 x 33278 x
-// 256: 6.2 us against 12.2 and 7.7).
-Tile tile_for(long m, long n, int size, long few) {
-  if (size == 4 || n <= few) return Tile::small;
-  return tiles(Tile::wide, m, n) >= 192 ? Tile::wide : Tile::mid;
+// The tile of an m x n result, by what was measured (us, forward products):
+// wide: twice the work per byte that goes through LDS, but one workgroup fills
+//   a CU: pays once there are enough for most CUs (bf16, 8192 x 16384 x 768:
+//   217, mid 251; 1024 x 9521 x 512: 18, mid 17).
+// small: fp32 products are 16 times slower for the same loads, so three
+//   workgroups to a CU lose nothing and leave less of a last round (700 x 33278
+//   x 256: 108, wide 138, mid 124); also up to 64 rows (35 x 33278 x 256: 6.2,
+//   wide 12.2, mid 7.7).
+// deep: few tiles and a long k wait for memory: 4 slices on their way (bf16,
+//   276 x 967 x 3264: 13.7, mid 24.6; fp32, 512 x 5000 x 512: 31, small 36; but
+//   bf16, 512 x 5000 x 512: 10.7, mid 8.0).
+// thin: up to 32 rows (fp32, 8 x 30522 x 768: 18.5, small 29).
+Tile tile_for(long m, long n, int size, bool rows) {
+  if (rows && n <= 32) return Tile::thin;
+  if (size == 4) {
+    return tiles(Tile::small, m, n) < 512 ? Tile::deep : Tile::small;
+  }
+  if (rows && n <= 64) {
+    return tiles(Tile::small, m, n) < 160 ? Tile::deep : Tile::small;
+  }
+  if (tiles(Tile::wide, m, n) >= 192) return Tile::wide;
+  return rows && tiles(Tile::mid, m, n) < 128 ? Tile::deep : Tile::mid;
 }
 
 }  // namespace
@@ -1125,7 +1147,7 @@ long padded(long n) { return (n + 7) / 8 * 8; }
 
 Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   Plan p;
-  p.logits = tile_for(vocab, rows, size, 64);
+  p.logits = tile_for(vocab, rows, size, true);
   p.band = BAND[(int)p.logits];
   const int edge_m = EDGE_M[(int)p.logits], edge_n = EDGE_N[(int)p.logits];
   p.bands = ceil_div(vocab, edge_m) * (edge_m / p.band);
@@ -1148,9 +1170,9 @@ Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   const long dx_tiles = tiles(p.dx, ldim, rows);
   const long slots = SLOTS[(int)p.dx] * (size == 4 ? 2 : 1);
   p.dx_splits = (int)std::max<long>(
-      1, std::min<long>({slots / dx_tiles, p.piece / 512, 64}));
+      1, std::min<long>({slots / dx_tiles, p.piece / 256, 64}));
   // dw has many tiles and its k are the rows
-  p.dw = tile_for(ldim, p.piece, size, 0);
+  p.dw = tile_for(ldim, p.piece, size, false);
   const long dw_tiles = tiles(p.dw, ldim, p.piece);
   p.dw_splits = (int)std::max<long>(
       1, std::min<long>({SLOTS[(int)p.dw] / 2 / dw_tiles, rows / 512, 16}));

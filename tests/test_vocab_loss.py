@@ -172,7 +172,12 @@ def test_reduced(dtype, eps, reduction):
     (2100, 264, 8200, torch.bfloat16),   # more than 256 wide tiles
     (2100, 260, 8200, torch.bfloat16),   # and rows that need packing
     (2100, 264, 8200, torch.float32),
+    (2100, 136, 8200, torch.float16),
+    (700, 72, 3000, torch.bfloat16),     # tiles of middle size
+    (700, 72, 3000, torch.float16),
     (40, 64, 33278, torch.float16),      # a long vocabulary, few rows
+    (40, 64, 33278, torch.bfloat16),
+    (20, 40, 9000, torch.float32),
 ])
 def test_wide_tiles(rows, dim, vocab, dtype):
     x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.1, 9)
