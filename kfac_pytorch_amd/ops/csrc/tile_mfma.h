@@ -390,11 +390,14 @@ __device__ __forceinline__ void store_columns(const T (&v)[ROWS / 16][4],
   __builtin_amdgcn_wave_barrier();
 }
 
-// Which tile a workgroup takes.  Workgroups go to the 8 XCDs in turn; each
-// XCD has an L2 of its own, so each gets one run of neighbouring tiles, and a
-// run walks 8 tiles of m for each tile of n before the next n.
-__device__ __forceinline__ void pick(int id, int mt, int nt, int* m, int* n) {
+// Which tile of mt x nt workgroup `id` takes; false: none.  Workgroups go to
+// the 8 XCDs in turn; each XCD has an L2 of its own, so each gets one run of
+// neighbouring tiles, and a run walks 8 tiles of m for each tile of n before
+// the next n.  nt is of the rows that are there (a count on the device): were
+// it of the rows that there may be, some XCDs would get most of the work.
+__device__ __forceinline__ bool pick(int id, int mt, int nt, int* m, int* n) {
   const int total = mt * nt;
+  if (id >= total) return false;
   const int q = total >> 3, r = total & 7;
   const int x = id & 7, y = id >> 3;
   const int p = x * q + (x < r ? x : r) + y;
@@ -404,6 +407,7 @@ __device__ __forceinline__ void pick(int id, int mt, int nt, int* m, int* n) {
   const int in = p - first * nt;
   *m = first + in % wide;
   *n = in / wide;
+  return true;
 }
 
 }  // namespace tile

@@ -179,9 +179,9 @@ __global__ void pack_kernel(const T* __restrict__ in, long ld, long step,
 }
 
 // Both of the above in one launch: a workgroup counts the kept rows before its
-// own PREP rows anew, numbers these and packs them.  The counting reads rows^2
-// / PREP / 2 targets in all, nothing for some thousand rows (8192 rows of 768
-// in fp16: 9 us against 6 + 8 and a launch), too much for very many.
+// own `prep` rows anew, numbers these and packs them.  The counting reads
+// rows^2 / prep / 2 targets in all, nothing for some thousand rows (8192 rows
+// of 768 in fp16: 9 us against 6 + 8 and a launch), too much for very many.
 constexpr int PREP = 16;
 constexpr long PREP_MOST = 16384;
 
@@ -190,10 +190,10 @@ __global__ __launch_bounds__(256) void prepare_kernel(
     const I* __restrict__ target, long rows, long ignore, long vocab,
     int* __restrict__ pos, int* __restrict__ idx, int* __restrict__ tgt,
     int* __restrict__ count, const T* __restrict__ in, long ld, long step,
-    int cols, T* __restrict__ out, int ldo, int wide) {
+    int cols, T* __restrict__ out, int ldo, int wide, int prep) {
   __shared__ int part[4], from[PREP], kept;
   const int t = threadIdx.x, lane = t & 63;
-  const int first = blockIdx.x * PREP;
+  const int first = blockIdx.x * prep;
   int n = 0;
 #pragma unroll 8
   for (int k = t; k < first; k += 256) n += (long)target[k] != ignore;
@@ -204,11 +204,11 @@ __global__ __launch_bounds__(256) void prepare_kernel(
   const int before = part[0] + part[1] + part[2] + part[3];
   if (t < 64) {
     const int r = first + t;
-    const long v = t < PREP && r < rows ? (long)target[r] : ignore;
+    const long v = t < prep && r < rows ? (long)target[r] : ignore;
     const bool keep = v != ignore;
     const unsigned long long mask = __ballot(keep);
     const int mine = __popcll(mask & ((1ull << lane) - 1));
-    if (t < PREP && r < rows) pos[r] = keep ? before + mine : -1;
+    if (t < prep && r < rows) pos[r] = keep ? before + mine : -1;
     if (keep) {
       idx[before + mine] = r;
       tgt[before + mine] = v >= 0 && v < vocab ? (int)v : BAD;
@@ -216,7 +216,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(
     }
     if (t == 0) {
       kept = __popcll(mask);
-      if (first + PREP >= rows) *count = before + __popcll(mask);
+      if (first + prep >= rows) *count = before + __popcll(mask);
     }
   }
   __syncthreads();
@@ -236,7 +236,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(
 struct Logits {
   long ldw;
   int ldx, v0, vocab;  // the piece [v0, v0 + vocab) of the entries
-  int mt, nt;
+  int mt;
   const int *count, *tgt;
   // sums, KEEP
   float *pmax, *psum, *pz, *ztgt;  // [row][band]; pz null without smoothing
@@ -257,11 +257,12 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
     const T* __restrict__ w, const T* __restrict__ x,
     const T* __restrict__ bias, T* __restrict__ grad, const Logits p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  int tm, tn;
-  tile::pick(blockIdx.x, p.mt, p.nt, &tm, &tn);
   const int rows = *p.count;
+  int tm, tn;
+  if (!tile::pick(blockIdx.x, p.mt, (rows + S::BN - 1) / S::BN, &tm, &tn)) {
+    return;
+  }
   const int m0 = tm * S::BM, n0 = tn * S::BN;
-  if (n0 >= rows) return;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -593,8 +594,8 @@ struct Factor {
 // In place: g = c (power 2^(band - row) / sum - eps / V), the target's entry
 // anew from its z.  A workgroup takes `part` tokens, a lane one 16-byte chunk
 // of each of them, and sums the bias gradient down the rows in passing; one
-// more workgroup adds up the losses.  Bound by memory: 16 tokens a workgroup
-// where there would be too few of them otherwise.
+// more workgroup adds up the losses.  Bound by memory: down to 4 tokens a
+// workgroup where there would be too few of them otherwise.
 template <class T>
 __global__ __launch_bounds__(256) void probs_kernel(
     T* __restrict__ grad, long ldg, int vocab, int part,
@@ -700,15 +701,16 @@ __global__ __launch_bounds__(1024) void coef_kernel(
 template <class T, class S>
 __global__ __launch_bounds__(S::THREADS) void dx_kernel(
     const T* __restrict__ w, long ldw, const T* __restrict__ grad, long ldg,
-    int piece, int dim, const int* count, int mt, int nt, int run, int first,
-    float* __restrict__ slabs, long slab) {
+    int piece, int dim, const int* count, int mt, int splits, int run,
+    int first, float* __restrict__ slabs, long slab) {
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int split = blockIdx.x / (mt * nt);
+  const int rows = *count;
+  const int nt = (rows + S::BN - 1) / S::BN;
+  const int split = nt > 0 ? blockIdx.x / (mt * nt) : splits;
+  if (split >= splits) return;
   int tm, tn;
   tile::pick(blockIdx.x - split * mt * nt, mt, nt, &tm, &tn);
-  const int rows = *count;
   const int m0 = tm * S::BM, n0 = tn * S::BN;
-  if (n0 >= rows) return;
   const int kbeg = split * run;
   const int kend = (int)ldg - kbeg < run ? (int)ldg : kbeg + run;
   f32x4 acc[S::MI][S::NI] = {};
@@ -957,11 +959,11 @@ struct Run {
     p.ldw = o.ldw;
     p.ldx = o.ldx;
     p.mt = ceil_div(p.vocab, S::BM);
-    p.nt = ceil_div(o.rows, S::BN);
+    const int nt = ceil_div(o.rows, S::BN);
     p.count = o.count;
     p.tgt = o.tgt;
     with_lds<logits_kernel<T, S, MODE>>(S::LDS);
-    logits_kernel<T, S, MODE><<<p.mt * p.nt, S::THREADS, S::LDS, s>>>(
+    logits_kernel<T, S, MODE><<<p.mt * nt, S::THREADS, S::LDS, s>>>(
         (const T*)o.w, (const T*)o.x, (const T*)o.bias, grad, p);
     check(hipGetLastError());
   }
@@ -1035,7 +1037,8 @@ struct Run {
     with_lds<dx_kernel<T, S>>(S::LDS);
     dx_kernel<T, S><<<md * nt * splits, S::THREADS, S::LDS, s>>>(
         (const T*)o.w + v0 * o.ldw, o.ldw, (const T*)b.grad, ldg, piece,
-        o.ldx, o.count, md, nt, run, v0 == 0, b.dx_slabs, o.rows * o.ldx);
+        o.ldx, o.count, md, splits, run, v0 == 0, b.dx_slabs,
+        o.rows * o.ldx);
     check(hipGetLastError());
   }
 
@@ -1161,7 +1164,7 @@ Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   if (keep) {
     const long columns = ceil_div(vocab * size, 4096);
     p.part = 64;
-    while (p.part > 16 && columns * ceil_div(rows, p.part) < 1024) p.part /= 2;
+    while (p.part > 4 && columns * ceil_div(rows, p.part) < 512) p.part /= 2;
   }
   p.parts = ceil_div(rows, p.part);
   // dx has few tiles and a long k: a tile that fits the call's size, its k
@@ -1222,10 +1225,11 @@ void prepare(Type t, const void* target, bool wide_ints, long rows,
   by_type(t, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
     auto launch = [&](auto* targets) {
-      prepare_kernel<<<ceil_div(rows, PREP), 256, 0, s>>>(
+      const int prep = rows <= 4096 ? 4 : PREP;  // few rows: more workgroups
+      prepare_kernel<<<ceil_div(rows, prep), 256, 0, s>>>(
           targets, rows, ignore, vocab, pos, idx, tgt, count, (const T*)in,
           ld, step, cols, (T*)out, ldo,
-          (int)wide_rows<T>(in, ld, step, cols, ldo));
+          (int)wide_rows<T>(in, ld, step, cols, ldo), prep);
       check(hipGetLastError());
     };
     if (wide_ints) {
