@@ -923,7 +923,7 @@ int ceil_div(long a, long b) { return (int)((a + b - 1) / b); }
 using Wide = Shape<256, 256, 2, 4>;
 using Mid = Shape<128, 128, 2, 4>;
 using Small = Shape<128, 64, 2, 2>;
-using Deep = Shape<64, 64, 2, 2, 5>;
+using Deep = Shape<64, 64, 2, 2, 3>;
 using Thin = Shape<64, 32, 2, 2, 4>;
 
 // calls f with a value of the tile's shape
@@ -1113,29 +1113,33 @@ void by_type(Type t, F f) {
 constexpr int EDGE_M[] = {256, 128, 128, 64, 64};
 constexpr int EDGE_N[] = {256, 128, 64, 64, 32};
 constexpr int BAND[] = {128, 64, 64, 32, 32};
-// workgroups that run at once: one to three for each of 256 CUs
-constexpr int SLOTS[] = {256, 512, 768, 512, 768};
+// workgroups that dx, with few tiles and a long k, is cut up for: enough to
+// fill the card once, no more, since each writes and reads fp32 partial sums
+constexpr int WANT[] = {256, 256, 1536, 256, 512};
 
 long tiles(Tile t, long m, long n) {
   return (long)ceil_div(m, EDGE_M[(int)t]) * ceil_div(n, EDGE_N[(int)t]);
 }
 
-// The tile of an m x n result, by what was measured (us, forward products):
+// The tile of an m x n result of k products, by what was measured (us, of the
+// logits where not said):
 // wide: twice the work per byte that goes through LDS, but one workgroup fills
 //   a CU: pays once there are enough for most CUs (bf16, 8192 x 16384 x 768:
 //   217, mid 251; 1024 x 9521 x 512: 18, mid 17).
-// small: fp32 products are 16 times slower for the same loads, so three
-//   workgroups to a CU lose nothing and leave less of a last round (700 x 33278
-//   x 256: 108, wide 138, mid 124); also up to 64 rows (35 x 33278 x 256: 6.2,
-//   wide 12.2, mid 7.7).
-// deep: few tiles and a long k wait for memory: 4 slices on their way (bf16,
-//   276 x 967 x 3264: 13.7, mid 24.6; fp32, 512 x 5000 x 512: 31, small 36; but
-//   bf16, 512 x 5000 x 512: 10.7, mid 8.0).
+// small: fp32 products are 16 times slower for the same loads, so more
+//   workgroups to a CU lose nothing (4096 x 9521 x 1024: 590, deep 611; mid,
+//   16 waves, 610); also up to 64 rows (bf16, 35 x 33278 x 256: 6.2, wide 12.2,
+//   mid 7.7).
+// deep: few tiles, or a short k, leave little work to a workgroup: smaller ones,
+//   with 2 slices on their way (bf16, 276 x 967 x 3264: 15.5, mid 26.7; fp32,
+//   700 x 33278 x 256: 110, small 124; its dw 103, small 112; but bf16, 512 x
+//   5000 x 512: 8.5, mid 8.0).
 // thin: up to 32 rows (fp32, 8 x 30522 x 768: 18.5, small 29).
-Tile tile_for(long m, long n, int size, bool rows) {
+Tile tile_for(long m, long n, long k, int size, bool rows) {
   if (rows && n <= 32) return Tile::thin;
   if (size == 4) {
-    return tiles(Tile::small, m, n) < 512 ? Tile::deep : Tile::small;
+    return tiles(Tile::small, m, n) * (k / 512) >= 1280 ? Tile::small
+                                                        : Tile::deep;
   }
   if (rows && n <= 64) {
     return tiles(Tile::small, m, n) < 160 ? Tile::deep : Tile::small;
@@ -1150,7 +1154,7 @@ long padded(long n) { return (n + 7) / 8 * 8; }
 
 Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   Plan p;
-  p.logits = tile_for(vocab, rows, size, true);
+  p.logits = tile_for(vocab, rows, ldim, size, true);
   p.band = BAND[(int)p.logits];
   const int edge_m = EDGE_M[(int)p.logits], edge_n = EDGE_N[(int)p.logits];
   p.bands = ceil_div(vocab, edge_m) * (edge_m / p.band);
@@ -1167,18 +1171,18 @@ Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
     while (p.part > 4 && columns * ceil_div(rows, p.part) < 512) p.part /= 2;
   }
   p.parts = ceil_div(rows, p.part);
-  // dx has few tiles and a long k: a tile that fits the call's size, its k
-  // cut up until the card is full once (fp32: twice, its rounds are long)
-  p.dx = p.logits;
-  const long dx_tiles = tiles(p.dx, ldim, rows);
-  const long slots = SLOTS[(int)p.dx] * (size == 4 ? 2 : 1);
+  // dx: a tile that fits the call's size, its k cut up
+  p.dx = size == 4 && p.logits != Tile::thin
+             ? tile_for(ldim, rows, p.piece, size, true)
+             : p.logits;
   p.dx_splits = (int)std::max<long>(
-      1, std::min<long>({slots / dx_tiles, p.piece / 256, 64}));
+      1, std::min<long>({WANT[(int)p.dx] / tiles(p.dx, ldim, rows),
+                         p.piece / 256, 64}));
   // dw has many tiles and its k are the rows
-  p.dw = tile_for(ldim, p.piece, size, false);
+  p.dw = tile_for(ldim, p.piece, rows, size, false);
   const long dw_tiles = tiles(p.dw, ldim, p.piece);
   p.dw_splits = (int)std::max<long>(
-      1, std::min<long>({SLOTS[(int)p.dw] / 2 / dw_tiles, rows / 512, 16}));
+      1, std::min<long>({256 / dw_tiles, rows / 512, 16}));
   return p;
 }
 
