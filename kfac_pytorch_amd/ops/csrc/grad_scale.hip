@@ -276,7 +276,10 @@ __global__ __launch_bounds__(THREADS) void scale_kernel(
     if (id >= list.chunks) break;
     const unsigned chunk = list.chunks - 1 - id;
     const Entry<2>& e = list.e[find(list, chunk)];
-    if (f == 1.f && e.p[0] == e.p[1]) continue;  // in place, nothing to do
+    if (f == 1.f && sizeof(I) == sizeof(O) && e.p[0] == e.p[1] &&
+        e.ld[0] == e.ld[1]) {
+      continue;  // in place, nothing to do
+    }
     float v[UNROLL][N];
 #pragma unroll
     for (int k = 0; k < UNROLL; ++k) {
@@ -525,6 +528,10 @@ void scale_pass(const std::vector<Tensor>& in, const std::vector<Tensor>& out,
   }
   for (auto& c : copies) {
     if (c.first.defined()) c.first.copy_(c.second);
+  }
+  // autograd sees that these were written
+  for (const Tensor& t : out) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   }
 }
 

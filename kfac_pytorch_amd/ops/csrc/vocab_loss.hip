@@ -8,14 +8,15 @@
 //   dx = g w,   dw = g^T x,   db = sum_n g,    c_n = d(total) / d(loss[n])
 //
 // A workgroup makes one tile of z in registers.  Of each band of its rows it
-// leaves, for every token n, a reference (the band's largest z in units of
-// log 2, rounded to a whole number, so that exp2(z log2(e) - reference) takes
-// one fused multiply-add and the reference carries no error), the sum of those
-// powers and, with smoothed labels, the sum of z; a wave per row joins them.
+// leaves, for every token n, the band's largest z, the sum of exp(z - largest)
+// (the powers) and, with smoothed labels, the sum of z; a wave per row joins
+// them.  The difference is taken before it is scaled for exp2: one fused
+// multiply-add instead would be off by the rounding of largest * log2(e), a
+// factor of 2^64 where a mask adds -1e9 to a whole band.
 //
 // Gradients, either of two ways:
-//   kept: the forward pass writes the powers themselves, in the inputs' type;
-//     once the sums are joined a pass over them makes g, and g is multiplied
+//   kept: the forward pass writes the powers themselves, in 16 bits for 16-bit
+//     inputs; once the sums are joined a pass over them makes g, and g is multiplied
 //     with w and x: 3 products in all.  They exist during the call only; what
 //     is kept for the backward pass are the gradients for an upstream factor
 //     of 1.
@@ -64,15 +65,14 @@ __device__ __forceinline__ float safe(float m) {
   return m == -INFINITY ? 0.f : m;
 }
 
-// exp(z) / 2^m for a whole m
 __device__ __forceinline__ float power(float z, float m) {
-  return __builtin_amdgcn_exp2f(fmaf(z, LOG2E, -m));
+  return __builtin_amdgcn_exp2f((z - m) * LOG2E);
 }
 
 // The type that powers are kept in: 16 bits are best used as fp16, also for
 // bf16 (gradients off by 2.1e-3 of their norm instead of 2.6e-3).  A power is
-// at most 2^0.5; times 2^15, those down to 2^-29 of a band's largest keep all
-// 11 bits.
+// at most 1; times 2^15, those down to 2^-29 of a band's largest keep all 11
+// bits.
 template <class T>
 using Power = std::conditional_t<sizeof(T) == 2, _Float16, float>;
 template <class T>
@@ -361,7 +361,6 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
       }
       m = fmaxf(m, __shfl_xor(m, 16));
       m = fmaxf(m, __shfl_xor(m, 32));
-      m = rintf(m * LOG2E);
       const float ref = safe(m);
       const int n = nbase + ni * 16;
       float s = 0.f;
@@ -378,8 +377,9 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
       if constexpr (MODE == KEEP) {
         tile::store_columns<Power<T>, S::MI * 16>(
             out, stage + (ni & 1) * (S::MI * 256 * sizeof(T)),
-            reinterpret_cast<Power<T>*>(grad) + (long)(n0 + wcol + ni * 16) * p.ldg + m0 + wrow, p.ldg,
-            rows - (n0 + wcol + ni * 16), (int)p.ldg - (m0 + wrow), lane);
+            reinterpret_cast<Power<T>*>(grad) +
+                (long)(n0 + wcol + ni * 16) * p.ldg + m0 + wrow,
+            p.ldg, rows - (n0 + wcol + ni * 16), (int)p.ldg - (m0 + wrow), lane);
       }
       s += __shfl_xor(s, 16);
       s += __shfl_xor(s, 32);
@@ -485,8 +485,8 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
   }
 }
 
-// One wave per row of the call: joins the bands.  rowm is the row's whole
-// reference and rowi the inverse of its sum, p = power(z, rowm) rowi.
+// One wave per row of the call: joins the bands.  rowm is the row's largest z
+// and rowi the inverse of its sum, p = power(z, rowm) rowi.
 __global__ __launch_bounds__(256) void join_kernel(
     const float* __restrict__ pmax, const float* __restrict__ psum,
     const float* __restrict__ pz, const float* __restrict__ ztgt,
@@ -516,22 +516,21 @@ __global__ __launch_bounds__(256) void join_kernel(
     float top = m;
 #pragma unroll
     for (int j = 0; j < U; ++j) top = fmaxf(top, a[j]);
-    s *= __builtin_amdgcn_exp2f(m - safe(top));
+    s *= power(m, safe(top));
 #pragma unroll
     for (int j = 0; j < U; ++j) {
-      s = fmaf(b[j], __builtin_amdgcn_exp2f(a[j] - safe(top)), s);
+      s = fmaf(b[j], power(a[j], safe(top)), s);
     }
     m = top;
   }
   const float top = safe(wave_max(m));
-  s = wave_sum(s * __builtin_amdgcn_exp2f(m - top));
+  s = wave_sum(s * power(m, top));
   z = wave_sum(z);
   if (lane == 0) {
     const bool bad = tgt[p] == BAD;
     rowm[p] = top;
     rowi[p] = bad ? NAN : 1.f / s;
-    // the powers are of the rounded log2(e): dividing by it undoes that
-    double v = ((double)top + log2((double)s)) / (double)LOG2E -
+    double v = (double)top + log((double)s) -
                (1.0 - (double)eps) * (double)ztgt[p];
     if (pz) v -= (double)share * (double)z;
     loss[n] = bad ? NAN : (float)v;
@@ -591,7 +590,7 @@ struct Factor {
 };
 
 // ------------------------------------------------- g from the kept powers
-// In place: g = c (power 2^(band - row) / sum - eps / V), the target's entry
+// In place: g = c (power exp(band - row) / sum - eps / V), the target's entry
 // anew from its z.  A workgroup takes `part` tokens, a lane one 16-byte chunk
 // of each of them, and sums the bias gradient down the rows in passing; one
 // more workgroup adds up the losses.  Bound by memory: down to 4 tokens a
@@ -629,8 +628,8 @@ __global__ __launch_bounds__(256) void probs_kernel(
     const Powers t = *reinterpret_cast<const Powers*>(at);
     Chunk g;
     const float m = rowm[n], i = rowi[n];
-    const float k = __builtin_amdgcn_exp2f(safe(pmax[(long)n * bands + mine]) -
-                                           m) * i * c * (1.f / LIFT<T>);
+    const float k = power(safe(pmax[(long)n * bands + mine]), m) * i * c *
+                    (1.f / LIFT<T>);
     const int hit = tgt[n] - v;
 #pragma unroll
     for (int j = 0; j < E; ++j) {

@@ -442,7 +442,10 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
   const Tensor flat = target.reshape({-1}).contiguous();
   CHECK_VALUE(rows.size(0) > 0 && rows.size(0) < (1l << 30) &&
                   weight.size(0) < (1l << 30) &&
-                  rows.size(1) * rows.element_size() < (1l << 22),
+                  rows.size(1) * rows.element_size() < (1l << 22) &&
+                  // a launch has at most 2^31 tiles
+                  (rows.size(0) / 32 + 1) * (weight.size(0) / 64 + 1) <
+                      (1l << 31),
               "sizes out of range: ", rows.sizes(), " and ", weight.sizes());
 #undef CHECK_VALUE
   const bool grads =

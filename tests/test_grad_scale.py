@@ -92,6 +92,17 @@ def test_in_place(clips, device):
 
 
 @devices
+def test_written_tensors_are_seen_by_autograd(device):
+    a = torch.ones(5, device=device, requires_grad=True)
+    b = a * 2
+    (b * b).sum().backward(retain_graph=True)
+    c = (b * b).sum()
+    ops.clip_by_global_norm([b.detach()], 0.1, out=[b.detach()])
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        c.backward()
+
+
+@devices
 def test_layouts(device):
     """Views of a bucket, strides, channels-last, expanded, mixed types."""
     flat, = tensors([(5000,)], torch.float32, device, 3)

@@ -320,6 +320,50 @@ def test_entries_masked_by_the_bias(low):
 
 @pytest.mark.gpu
 @needs_gpu
+@pytest.mark.parametrize("dtype", list(HALF), ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("reduction", ["none", "sum"])
+def test_bands_masked_by_large_values(dtype, reduction):
+    """Masks of -1e4, -1e9 and the lowest value over whole tiles: what they
+    cover weighs nothing, and nothing overflows."""
+    x, w, b, t = inputs(50, 64, 900, dtype, True, 0.1, 4)
+    lows = [-1e4, -1e9, torch.finfo(dtype).min, float("-inf")]
+    for k, low in enumerate(lows):
+        low = max(low, torch.finfo(dtype).min) if math.isfinite(low) else low
+        b[128 + 128 * k:256 + 128 * k] = low
+    kept = torch.ones(900, dtype=torch.bool, device="cuda")
+    kept[128:640] = False
+    t = torch.where((t >= 128) & (t < 640), 3, t)
+    up = torch.ones(50, device="cuda") if reduction == "none" else None
+    loss, grads = run(x, w, b, t, 0.0, reduction, up)
+    small = torch.where(t >= 640, t - 512, t)
+    ref = formula(x, w[kept], b[kept], small, 0.0, torch.ones(50))
+    check_all(ref, loss if up is not None else None,
+              [grads[0], grads[1][kept], grads[2][kept]], x, w[kept],
+              b[kept], dtype, 50)
+    assert not grads[1][~kept].any() and not grads[2][~kept].any()
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_all_entries_masked_alike():
+    """A row of nothing but the lowest value is uniform, as in
+    F.cross_entropy: the differences are zero."""
+    x = torch.zeros(3, 32, device="cuda")
+    w = torch.randn(200, 32, device="cuda")
+    t = torch.tensor([0, 7, 199], device="cuda")
+    for low in (torch.finfo(torch.float32).min, -1e30, -1e9, 1e9, 1e30):
+        b = torch.full((200,), low, device="cuda")
+        loss, grads = run(x, w, b, t, 0.0, "sum")
+        # a loss is log V next to |low|: of the rounding of low alone
+        assert abs(float(loss) - 3 * math.log(200)) <= 4 * 2.0 ** -24 * max(
+            abs(low) * 3, 64)
+        want = torch.full((200,), 3 / 200, device="cuda")
+        want[t] -= 1
+        assert (grads[2] - want).abs().max() <= 2.0 ** -20
+
+
+@pytest.mark.gpu
+@needs_gpu
 def test_infinite_and_nan_logits():
     x, w, b, t = inputs(6, 32, 200, torch.float32, True)
     t = torch.tensor([3, 3, 3, 3, 3, 3], device="cuda")
