@@ -26,7 +26,7 @@ enum class Tile { wide, mid, small, deep, thin };
 
 // How a call of given sizes is cut up.
 struct Plan {
-  Tile logits, dx, dw;
+  Tile logits, grads;
   int band, bands;        // entries of a band, bands of a row
   long piece;             // entries of the vocabulary at a time
   int part, parts;        // tokens of a part of the bias gradient's sum

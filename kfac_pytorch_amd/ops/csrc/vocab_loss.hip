@@ -734,30 +734,45 @@ __global__ __launch_bounds__(1024) void coef_kernel(
   }
 }
 
-// ------------------------------------------------------------- dx += g w
-// Rows of the tile are hidden units, columns tokens, k the piece's entries,
-// cut into `splits` runs of `run` values that add to slabs of their own.
+// ------------------------------------------- dx += g w and dw = g^T x
+// Rows of dx's tiles are hidden units, columns tokens, k the piece's entries,
+// cut into `splits` runs of `run` values that add to slabs of their own.  Rows
+// of dw's tiles are hidden units, columns vocabulary entries, k tokens.
+struct Dx {
+  long ldw;
+  int mt, splits, run, first;
+  float* slabs;
+  long slab;
+  int blocks;
+};
+
+struct Dw {
+  long ldx;
+  int mt, nt, splits, run;
+  void* out;
+  float* slabs;
+  long slab;
+  int blocks;
+};
+
 template <class T, class S>
-__global__ __launch_bounds__(S::THREADS) void dx_kernel(
-    const T* __restrict__ w, long ldw, const T* __restrict__ grad, long ldg,
-    int piece, int dim, const int* count, int mt, int splits, int run,
-    int first, float* __restrict__ slabs, long slab) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int rows = *count;
+__device__ __forceinline__ void dx_body(const T* w, const T* grad, long ldg,
+                                        int piece, int dim, int rows,
+                                        const Dx& p, int block, char* smem) {
   const int nt = (rows + S::BN - 1) / S::BN;
-  const int split = nt > 0 ? blockIdx.x / (mt * nt) : splits;
-  if (split >= splits) return;
+  const int split = nt > 0 ? block / (p.mt * nt) : p.splits;
+  if (split >= p.splits) return;
   int tm, tn;
-  tile::pick(blockIdx.x - split * mt * nt, mt, nt, &tm, &tn);
+  tile::pick(block - split * p.mt * nt, p.mt, nt, &tm, &tn);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
-  const int kbeg = split * run;
-  const int kend = (int)ldg - kbeg < run ? (int)ldg : kbeg + run;
+  const int kbeg = split * p.run;
+  const int kend = (int)ldg - kbeg < p.run ? (int)ldg : kbeg + p.run;
   f32x4 acc[S::MI][S::NI] = {};
-  tile::product<T, true, false, S>(w, ldw, m0, dim, grad, ldg, n0, rows, kbeg,
-                                   kend, piece, smem, acc);
+  tile::product<T, true, false, S>(w, p.ldw, m0, dim, grad, ldg, n0, rows,
+                                   kbeg, kend, piece, smem, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;
-  float* out = slabs + split * slab;
+  float* out = p.slabs + split * p.slab;
 #pragma unroll
   for (int mi = 0; mi < S::MI; ++mi) {
     const int d = m0 + (wave / S::WN) * (S::MI * 16) + mi * 16 + g * 4;
@@ -766,40 +781,36 @@ __global__ __launch_bounds__(S::THREADS) void dx_kernel(
     for (int ni = 0; ni < S::NI; ++ni) {
       const int n = n0 + (wave % S::WN) * (S::NI * 16) + ni * 16 + i;
       if (n >= rows) continue;
-      f32x4* p = reinterpret_cast<f32x4*>(out + (long)n * dim + d);
-      *p = first ? acc[mi][ni] : *p + acc[mi][ni];
+      f32x4* at = reinterpret_cast<f32x4*>(out + (long)n * dim + d);
+      *at = p.first ? acc[mi][ni] : *at + acc[mi][ni];
     }
   }
 }
 
-// ------------------------------------------------------------- dw = g^T x
-// Rows of the tile are hidden units, columns vocabulary entries, k tokens.
 template <class T, class S>
-__global__ __launch_bounds__(S::THREADS) void dw_kernel(
-    const T* __restrict__ x, long ldx, const T* __restrict__ grad, long ldg,
-    int piece, int dim, int ldim, const int* count, int mt, int nt, int run,
-    const Factor factor, T* __restrict__ out, float* __restrict__ slabs,
-    long slab) {
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int split = blockIdx.x / (mt * nt);
+__device__ __forceinline__ void dw_body(const T* x, const T* grad, long ldg,
+                                        int piece, int dim, int ldim,
+                                        int rows, const Factor& factor,
+                                        const Dw& p, int block, char* smem) {
+  const int split = block / (p.mt * p.nt);
   int tm, tn;
-  tile::pick(blockIdx.x - split * mt * nt, mt, nt, &tm, &tn);
-  const int rows = *count;
+  tile::pick(block - split * p.mt * p.nt, p.mt, p.nt, &tm, &tn);
   const int m0 = tm * S::BM, n0 = tn * S::BN;
-  const int kbeg = split * run;
-  const int kend = rows - kbeg < run ? rows : kbeg + run;
+  const int kbeg = split * p.run;
+  const int kend = rows - kbeg < p.run ? rows : kbeg + p.run;
   f32x4 acc[S::MI][S::NI] = {};
-  tile::product<T, true, true, S>(x, ldx, m0, ldim, grad, ldg, n0,
+  tile::product<T, true, true, S>(x, p.ldx, m0, ldim, grad, ldg, n0,
                                   (int)ldg, kbeg, kend, kend, smem, acc);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;
   const float inv = factor.inverse();
   const int d0 = m0 + (wave / S::WN) * (S::MI * 16);
+  T* out = (T*)p.out;
   char* stage = smem + wave * (2 * S::MI * 256 * sizeof(T));
 #pragma unroll
   for (int ni = 0; ni < S::NI; ++ni) {
     const int v0 = n0 + (wave % S::WN) * (S::NI * 16) + ni * 16;
-    if (!slabs && dim % (16 / (int)sizeof(T)) == 0) {
+    if (!p.slabs && dim % (16 / (int)sizeof(T)) == 0) {
       T o[S::MI][4];
 #pragma unroll
       for (int mi = 0; mi < S::MI; ++mi) {
@@ -817,9 +828,9 @@ __global__ __launch_bounds__(S::THREADS) void dw_kernel(
     for (int mi = 0; mi < S::MI; ++mi) {
       const int d = d0 + mi * 16 + g * 4;
       if (d >= dim) continue;
-      if (slabs) {
-        *reinterpret_cast<f32x4*>(slabs + split * slab + (long)v * ldim + d) =
-            acc[mi][ni];
+      if (p.slabs) {
+        *reinterpret_cast<f32x4*>(p.slabs + split * p.slab + (long)v * ldim +
+                                  d) = acc[mi][ni];
       } else {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -829,6 +840,28 @@ __global__ __launch_bounds__(S::THREADS) void dw_kernel(
         }
       }
     }
+  }
+}
+
+// Both in one launch, the one with the longer runs first: alone, either leaves
+// part of the card idle at its end (us, with the adding up after them: bf16,
+// 700 x 33278 x 256: 43, 62 in two launches; 2976 kept of 3968 x 9521 x 512:
+// 80, 104; fp32, 700 x 33278 x 256: 202, 217).
+template <class T, class S>
+__global__ __launch_bounds__(S::THREADS) void products_kernel(
+    const T* __restrict__ w, const T* __restrict__ x,
+    const T* __restrict__ grad, long ldg, int piece, int dim, int ldim,
+    const Factor factor, const Dx dx, const Dw dw, int dw_first) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int rows = *factor.count;
+  const int lead = dw_first ? dw.blocks : dx.blocks;
+  const bool front = (int)blockIdx.x < lead;
+  const int block = front ? blockIdx.x : blockIdx.x - lead;
+  if (front == (dw_first != 0)) {
+    dw_body<T, S>(x, grad, ldg, piece, dim, ldim, rows, factor, dw, block,
+                  smem);
+  } else {
+    dx_body<T, S>(w, grad, ldg, piece, ldim, rows, dx, block, smem);
   }
 }
 
@@ -965,16 +998,20 @@ using Small = Shape<128, 64, 2, 2>;
 using Deep = Shape<64, 64, 2, 2, 3>;
 using Thin = Shape<64, 32, 2, 2, 4>;
 
-// calls f with a value of the tile's shape
-template <class F>
+// Calls f with a value of the tile's shape; those that a type never takes are
+// not built (SMALL: whether 16-bit types take that one).
+template <class T, bool SMALL, class F>
 void by_shape(Tile t, F f) {
-  switch (t) {
-    case Tile::wide: f(Wide()); break;
-    case Tile::mid: f(Mid()); break;
-    case Tile::small: f(Small()); break;
-    case Tile::deep: f(Deep()); break;
-    case Tile::thin: f(Thin()); break;
+  constexpr bool HALF = sizeof(T) == 2;
+  if constexpr (HALF) {
+    if (t == Tile::wide) return f(Wide());
+    if (t == Tile::mid) return f(Mid());
   }
+  if constexpr (SMALL || !HALF) {
+    if (t == Tile::small) return f(Small());
+  }
+  if (t == Tile::deep) return f(Deep());
+  f(Thin());
 }
 
 // Allows a kernel its LDS, once on each device.
@@ -1017,7 +1054,7 @@ struct Run {
     p.ztgt = f.ztgt;
     p.bands = o.plan.bands;
     p.ldg = padded(o.vocab);
-    by_shape(o.plan.logits, [&](auto shape) {
+    by_shape<T, true>(o.plan.logits, [&](auto shape) {
       using S = decltype(shape);
       if (grad) {
         logits<S, KEEP>(o, p, grad, s);
@@ -1061,52 +1098,52 @@ struct Run {
     p.share = o.eps / (float)o.vocab;
     p.pbias = b.pbias;
     p.all = o.vocab;
-    by_shape(o.plan.logits, [&](auto shape) {
+    by_shape<T, true>(o.plan.logits, [&](auto shape) {
       logits<decltype(shape), AGAIN>(o, p, (T*)b.grad, s);
     });
   }
 
   template <class S>
-  static void dx_product(const Operands& o, const Grads& b, long v0,
-                         int piece, hipStream_t s) {
-    const int md = ceil_div(o.ldx, S::BM), nt = ceil_div(o.rows, S::BN);
-    const int splits = o.plan.dx_splits;
-    const long ldg = padded(piece);
-    const int run = ceil_div(ceil_div(ldg, splits), 64) * 64;
-    with_lds<dx_kernel<T, S>>(S::LDS);
-    dx_kernel<T, S><<<md * nt * splits, S::THREADS, S::LDS, s>>>(
-        (const T*)o.w + v0 * o.ldw, o.ldw, (const T*)b.grad, ldg, piece,
-        o.ldx, o.count, md, splits, run, v0 == 0, b.dx_slabs,
-        o.rows * o.ldx);
-    check(hipGetLastError());
-  }
-
-  template <class S>
-  static void dw_product(const Operands& o, const Grads& b, long v0,
-                         int piece, hipStream_t s) {
-    const int md = ceil_div(o.ldx, S::BM), vt = ceil_div(piece, S::BN);
-    const int splits = o.plan.dw_splits;
-    const int run = ceil_div(ceil_div(o.rows, splits), 64) * 64;
-    with_lds<dw_kernel<T, S>>(S::LDS);
-    dw_kernel<T, S><<<md * vt * splits, S::THREADS, S::LDS, s>>>(
-        (const T*)o.x, o.ldx, (const T*)b.grad, padded(piece), piece, o.dim,
-        o.ldx, o.count, md, vt, run, factor(o, b), (T*)b.dw + v0 * o.dim,
-        b.dw_slabs, (long)piece * o.ldx);
+  static void products_as(const Operands& o, const Grads& b, long v0,
+                          int piece, hipStream_t s) {
+    const int md = ceil_div(o.ldx, S::BM);
+    Dx dx{};
+    Dw dw{};
+    if (b.dx_slabs) {
+      dx.ldw = o.ldw;
+      dx.mt = md;
+      dx.splits = o.plan.dx_splits;
+      dx.run = ceil_div(ceil_div(padded(piece), dx.splits), 64) * 64;
+      dx.first = v0 == 0;
+      dx.slabs = b.dx_slabs;
+      dx.slab = o.rows * o.ldx;
+      dx.blocks = md * ceil_div(o.rows, S::BN) * dx.splits;
+    }
+    if (b.dw || b.dw_slabs) {
+      dw.ldx = o.ldx;
+      dw.mt = md;
+      dw.nt = ceil_div(piece, S::BN);
+      dw.splits = o.plan.dw_splits;
+      dw.run = ceil_div(ceil_div(o.rows, dw.splits), 64) * 64;
+      dw.out = (T*)b.dw + v0 * o.dim;
+      dw.slabs = b.dw_slabs;
+      dw.slab = (long)piece * o.ldx;
+      dw.blocks = md * dw.nt * dw.splits;
+    }
+    if (dx.blocks + dw.blocks == 0) return;
+    with_lds<products_kernel<T, S>>(S::LDS);
+    products_kernel<T, S><<<dx.blocks + dw.blocks, S::THREADS, S::LDS, s>>>(
+        (const T*)o.w + v0 * o.ldw, (const T*)o.x, (const T*)b.grad,
+        padded(piece), piece, o.dim, o.ldx, factor(o, b), dx, dw,
+        dw.run > dx.run);
     check(hipGetLastError());
   }
 
   static void products(const Operands& o, const Grads& b, long v0, int piece,
                        hipStream_t s) {
-    if (b.dx_slabs) {
-      by_shape(o.plan.dx, [&](auto shape) {
-        dx_product<decltype(shape)>(o, b, v0, piece, s);
-      });
-    }
-    if (b.dw || b.dw_slabs) {
-      by_shape(o.plan.dw, [&](auto shape) {
-        dw_product<decltype(shape)>(o, b, v0, piece, s);
-      });
-    }
+    by_shape<T, false>(o.plan.grads, [&](auto shape) {
+      products_as<decltype(shape)>(o, b, v0, piece, s);
+    });
   }
 
   // What is left of rows [v0, v0 + piece) of dw, and of dx and db where they
@@ -1152,39 +1189,115 @@ void by_type(Type t, F f) {
 constexpr int EDGE_M[] = {256, 128, 128, 64, 64};
 constexpr int EDGE_N[] = {256, 128, 64, 64, 32};
 constexpr int BAND[] = {128, 64, 64, 32, 32};
-// workgroups that dx, with few tiles and a long k, is cut up for: enough to
-// fill the card once, no more, since each writes and reads fp32 partial sums
-constexpr int WANT[] = {256, 256, 1536, 256, 512};
-
 long tiles(Tile t, long m, long n) {
   return (long)ceil_div(m, EDGE_M[(int)t]) * ceil_div(n, EDGE_N[(int)t]);
 }
 
-// The tile of an m x n result of k products, by what was measured (us, of the
-// logits where not said):
+// The tile of the logits, m entries x n rows of k products, by what was measured
+// (us, for an m x n x k):
 // wide: twice the work per byte that goes through LDS, but one workgroup fills
-//   a CU: pays once there are enough for most CUs (bf16, 8192 x 16384 x 768:
-//   217, mid 251; 1024 x 9521 x 512: 18, mid 17).
+//   a CU: pays once there are enough for most CUs (bf16, 16384 x 8192 x 768:
+//   217, mid 251; 9521 x 1024 x 512: 18, mid 17).
 // small: fp32 products are 16 times slower for the same loads, so more
-//   workgroups to a CU lose nothing (4096 x 9521 x 1024: 590, deep 611; mid,
-//   16 waves, 610); also up to 64 rows (bf16, 35 x 33278 x 256: 6.2, wide 12.2,
+//   workgroups to a CU lose nothing (9521 x 4096 x 1024: 590, deep 611; mid,
+//   16 waves, 610); also up to 64 rows (bf16, 33278 x 35 x 256: 6.2, wide 12.2,
 //   mid 7.7).
 // deep: few tiles, or a short k, leave little work to a workgroup: smaller ones,
-//   with 2 slices on their way (bf16, 276 x 967 x 3264: 15.5, mid 26.7; fp32,
-//   700 x 33278 x 256: 110, small 124; its dw 103, small 112; but bf16, 512 x
-//   5000 x 512: 8.5, mid 8.0).
-// thin: up to 32 rows (fp32, 8 x 30522 x 768: 18.5, small 29).
-Tile tile_for(long m, long n, long k, int size, bool rows) {
-  if (rows && n <= 32) return Tile::thin;
+//   with 2 slices on their way (fp32, 33278 x 700 x 256: 110, small 124; but
+//   bf16, 5000 x 512 x 512: 8.5, mid 8.0).
+// thin: up to 32 rows (fp32, 30522 x 8 x 768: 18.5, small 29).
+Tile logits_tile(long m, long n, long k, int size) {
+  if (n <= 32) return Tile::thin;
   if (size == 4) {
     return tiles(Tile::small, m, n) * (k / 512) >= 1280 ? Tile::small
                                                         : Tile::deep;
   }
-  if (rows && n <= 64) {
+  if (n <= 64) {
     return tiles(Tile::small, m, n) < 160 ? Tile::deep : Tile::small;
   }
   if (tiles(Tile::wide, m, n) >= 192) return Tile::wide;
-  return rows && tiles(Tile::mid, m, n) < 128 ? Tile::deep : Tile::mid;
+  return tiles(Tile::mid, m, n) < 128 ? Tile::deep : Tile::mid;
+}
+
+// ------------------------------------------------ the tiles of the gradients
+// dw has the vocabulary's many tiles and a k of the rows; dx has few tiles and
+// a k of the vocabulary, so that is cut up into runs, each of which writes
+// fp32 partial sums that are read once more.  The tile and the number of runs
+// are those whose time comes out least by a simple count: the workgroups of
+// both products, the longer ones first, go to the first free place, of which a
+// CU has as many as workgroups fit into its LDS; one takes `start` us and per
+// slice of k `alone` us, or `shared` us for each of those that share its CU if
+// that is more; partial sums cost 0.3 us a MB.  The figures are fitted to 900
+// measured times of 19 shapes (1 to 8192 rows, 880 to 37397 entries, 32 to 1056
+// values): what it takes is 3% slower than the best of each on the mean (fp32:
+// 2%), at worst 13%; one rule for each product by itself was 25% slower.
+struct Speed {
+  float shared, alone, start;
+  int places;
+};
+constexpr float SLAB = 0.3e-6f;  // us a byte
+
+constexpr Speed HALF_SPEED[] = {{1.02f, 1.13f, 3.2f, 1},
+                                {0.485f, 0.725f, 3.2f, 2},
+                                {},
+                                {0.144f, 0.142f, 4.1f, 3},
+                                {0.155f, 0.131f, 3.6f, 3}};
+constexpr Speed FULL_SPEED[] = {{},
+                                {},
+                                {0.743f, 0.989f, 4.2f, 3},
+                                {0.36f, 0.494f, 4.9f, 3},
+                                {0.222f, 0.331f, 2.6f, 3}};
+constexpr int RUNS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
+
+// The end of n1 jobs of length a and then n2 of length b <= a on `places`.
+float ending(long n1, float a, long n2, float b, long places) {
+  const long late = n1 % places;  // places that are free one job later
+  const float lo = n1 / places * a, hi = late ? lo + a : lo;
+  if (n2 == 0) return hi;
+  const long behind = late ? (long)std::ceil(a / b) : 0;
+  long k = (n2 + places - late - 1) / (places - late);
+  if (k > behind) k = (n2 + late * behind + places - 1) / places;
+  float end = lo + k * b;
+  const long m = k - behind;  // does it end with the late ones' last job?
+  if (late && m >= 0 &&
+      (places - late) * (m + (long)(a / b)) + late * m >= n2) {
+    end = hi + m * b;
+  }
+  return std::max(end, hi);
+}
+
+void plan_grads(Plan* p, long rows, long ldim, int size) {
+  const long unit = 128 / size, piece = p->piece;
+  float best = INFINITY;
+  for (int t = 0; t < 5; ++t) {
+    const Speed& speed = (size == 2 ? HALF_SPEED : FULL_SPEED)[t];
+    if (speed.places == 0) continue;
+    const long nx = tiles((Tile)t, ldim, rows), nw = tiles((Tile)t, ldim, piece);
+    const long cuts =
+        std::max<long>(1, std::min<long>({256 / nw, rows / 512, 16}));
+    const float b = (float)ceil_div(ceil_div(rows, cuts), unit);
+    for (int runs : RUNS) {
+      if (runs > 1 && runs * 128 > piece) break;
+      const float a = (float)ceil_div(ceil_div(piece, runs), unit);
+      const long all = nx * runs + nw * cuts;
+      const float share = std::min(std::max(all / 256.f, 1.f),
+                                   (float)speed.places);
+      const float slice = std::max(speed.alone, speed.shared * share);
+      const long places = all > 256 ? 256 * speed.places : 256;
+      const float ta = speed.start + a * slice, tb = speed.start + b * slice;
+      const float cost =
+          (a >= b ? ending(nx * runs, ta, nw * cuts, tb, places)
+                  : ending(nw * cuts, tb, nx * runs, ta, places)) +
+          SLAB * 4 * ldim * ((float)runs * rows +
+                             (cuts > 1 ? (float)cuts * piece : 0.f));
+      if (cost < best) {
+        best = cost;
+        p->grads = (Tile)t;
+        p->dx_splits = runs;
+        p->dw_splits = (int)cuts;
+      }
+    }
+  }
 }
 
 }  // namespace
@@ -1193,7 +1306,7 @@ long padded(long n) { return (n + 7) / 8 * 8; }
 
 Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   Plan p;
-  p.logits = tile_for(vocab, rows, ldim, size, true);
+  p.logits = logits_tile(vocab, rows, ldim, size);
   p.band = BAND[(int)p.logits];
   const int edge_m = EDGE_M[(int)p.logits], edge_n = EDGE_N[(int)p.logits];
   p.bands = ceil_div(vocab, edge_m) * (edge_m / p.band);
@@ -1210,18 +1323,7 @@ Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
     while (p.part > 4 && columns * ceil_div(rows, p.part) < 512) p.part /= 2;
   }
   p.parts = ceil_div(rows, p.part);
-  // dx: a tile that fits the call's size, its k cut up
-  p.dx = size == 4 && p.logits != Tile::thin
-             ? tile_for(ldim, rows, p.piece, size, true)
-             : p.logits;
-  p.dx_splits = (int)std::max<long>(
-      1, std::min<long>({WANT[(int)p.dx] / tiles(p.dx, ldim, rows),
-                         p.piece / 256, 64}));
-  // dw has many tiles and its k are the rows
-  p.dw = tile_for(ldim, p.piece, rows, size, false);
-  const long dw_tiles = tiles(p.dw, ldim, p.piece);
-  p.dw_splits = (int)std::max<long>(
-      1, std::min<long>({256 / dw_tiles, rows / 512, 16}));
+  plan_grads(&p, rows, ldim, size);
   return p;
 }
 
