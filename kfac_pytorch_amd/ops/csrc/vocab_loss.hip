@@ -1300,11 +1300,7 @@ void plan_grads(Plan* p, long rows, long ldim, int size) {
   }
 }
 
-}  // namespace
-
-long padded(long n) { return (n + 7) / 8 * 8; }
-
-Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
+Plan make_plan(long rows, long vocab, int ldim, int size, bool keep) {
   Plan p;
   p.logits = logits_tile(vocab, rows, ldim, size);
   p.band = BAND[(int)p.logits];
@@ -1325,6 +1321,32 @@ Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   p.parts = ceil_div(rows, p.part);
   plan_grads(&p, rows, ldim, size);
   return p;
+}
+
+}  // namespace
+
+long padded(long n) { return (n + 7) / 8 * 8; }
+
+// The last sizes' plan is kept: the steps of a loop have the same, and the
+// count over tiles and runs takes a launch's time.
+Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
+  struct Last {
+    long rows = -1, vocab = 0;
+    int ldim = 0, size = 0;
+    bool keep = false;
+    Plan plan;
+  };
+  thread_local Last last;
+  if (last.rows != rows || last.vocab != vocab || last.ldim != ldim ||
+      last.size != size || last.keep != keep) {
+    last.plan = make_plan(rows, vocab, ldim, size, keep);
+    last.rows = rows;
+    last.vocab = vocab;
+    last.ldim = ldim;
+    last.size = size;
+    last.keep = keep;
+  }
+  return last.plan;
 }
 
 void scan(const void* target, bool wide_ints, long rows, long ignore,
