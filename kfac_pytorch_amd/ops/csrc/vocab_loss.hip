@@ -71,9 +71,9 @@ __device__ __forceinline__ float power(float z, float m) {
 }
 
 // The type that powers are kept in: 16 bits are best used as fp16, also for
-// bf16 (gradients off by 2.1e-3 of their norm instead of 2.6e-3).  A power is
-// at most 1; times 2^15, those down to 2^-29 of a band's largest keep all 11
-// bits.
+// bf16 (without the lift below, gradients off by 2.1e-3 of their norm instead
+// of 2.6e-3).  A power is at most 1; times 2^15, those down to 2^-29 of a
+// band's largest keep all 11 bits.
 template <class T>
 using Power = std::conditional_t<sizeof(T) == 2, _Float16, float>;
 template <class T>
@@ -565,28 +565,29 @@ __global__ __launch_bounds__(1024) void total_kernel(
 
 // ------------------------------------------------------ factors and scales
 // d(total)/d(loss) of a row is one (mean: 1 / count) times the upstream
-// factor.  fp16 holds g to 6e-8 only, and 1 / count times a small probability
-// is soon below that: there g is made with the factor brought to [2^14, 2^15)
-// by a power of two (|g| is at most the factor, and the type ends at 65504),
-// and the products are scaled back in fp32.
+// factor.  In 16 bits g is made with another factor, `lift`, and the products
+// are scaled in fp32, for two reasons.  Where p is small, most of a row's g is
+// its target's entry, -(1 - eps) factor: with factor = 1 / (1 - eps), times a
+// power of two, that is -1 and rounds to itself, where one / count or 0.9 would
+// be off by up to 2^-9 in every row alike (bf16, 2976 rows, eps 0.1: gradients
+// off by 2.9e-3 of their norm instead of 1.9e-3).  And fp16 holds g to 6e-8
+// only, so there the power of two is 2^14: |g| stays within 2^15, the type ends
+// at 65504.
 struct Factor {
-  const float* scale;  // [1]: the inverse of that power, or null: from count
+  const float* scale;  // [1]: the inverse of the rows' own lift, or null
   const int* count;
-  bool mean, lift;
+  bool mean;
+  float lift;  // 0: g is made with the factor itself
 
-  __device__ __forceinline__ int exponent(float one) const {
-    return lift ? 14 - (((int)__float_as_uint(one) >> 23) - 127) : 0;
-  }
   __device__ __forceinline__ float one() const {
     return mean ? 1.f / (float)*count : 1.f;
   }
-  // with the power of two
   __device__ __forceinline__ float lifted() const {
-    return ldexpf(one(), exponent(one()));
+    return lift != 0.f ? lift : one();
   }
   __device__ __forceinline__ float inverse() const {
     if (scale) return scale[1];
-    return *count > 0 ? ldexpf(1.f, -exponent(one())) : 1.f;
+    return lift != 0.f && *count > 0 ? one() / lift : 1.f;
   }
 };
 
@@ -690,19 +691,19 @@ __global__ __launch_bounds__(256) void probs_kernel(
 }
 
 // ---------------------------------------------------------- row coefficients
-// coef[i] = the factor of kept row i times the power of two, scale[0];
-// scale[1] is its inverse.
+// coef[i] = the factor of kept row i times scale[0], which brings the largest to
+// `lift`; scale[1] is its inverse.
 __global__ __launch_bounds__(1024) void coef_kernel(
     const float* __restrict__ up, int each, int mean,
     const int* __restrict__ idx, const int* __restrict__ tgt,
-    const int* __restrict__ count, int lift, float* __restrict__ coef,
+    const int* __restrict__ count, float lift, float* __restrict__ coef,
     float* __restrict__ scale) {
   __shared__ float part[16];
   __shared__ float shared_scale;
   const int rows = *count;
   const float one = each ? 1.f : (mean ? *up / (float)rows : *up);
   float top = 0.f;
-  if (lift) {
+  if (lift != 0.f) {
     if (each) {
       for (int i = threadIdx.x; i < rows; i += 1024) {
         const float a = fabsf(up[idx[i]]);
@@ -718,14 +719,12 @@ __global__ __launch_bounds__(1024) void coef_kernel(
   if (threadIdx.x == 0) {
     float m = 0.f;
     for (int k = 0; k < 16; ++k) m = fmaxf(m, part[k]);
-    int e = 0;
-    if (m > 0.f) {
-      e = 14 - (int)floorf(__builtin_amdgcn_logf(m));
-      e = e > 100 ? 100 : (e < -100 ? -100 : e);
-    }
-    shared_scale = ldexpf(1.f, e);
-    scale[0] = shared_scale;
-    scale[1] = ldexpf(1.f, -e);
+    // clamped: neither it nor its inverse leaves fp32
+    const float s =
+        m > 0.f ? fminf(fmaxf(lift / m, 0x1p-100f), 0x1p100f) : 1.f;
+    shared_scale = s;
+    scale[0] = s;
+    scale[1] = 1.f / s;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < rows; i += 1024) {
@@ -1028,6 +1027,14 @@ void with_lds(int bytes) {
   done.fetch_or(bit, std::memory_order_relaxed);
 }
 
+// what g's factor is brought to, see Factor; 0 leaves it
+template <class T>
+float lift(float eps) {
+  if (sizeof(T) == 4) return 0.f;
+  const float top = std::is_same_v<T, _Float16> ? 0x1p14f : 1.f;
+  return eps <= 0.5f ? top / (1.f - eps) : top;
+}
+
 template <class T>
 struct Run {
   template <class S, int MODE>
@@ -1069,8 +1076,7 @@ struct Run {
   }
 
   static Factor factor(const Operands& o, const Grads& b) {
-    return Factor{b.scale, o.count, b.mean, sizeof(T) == 2 &&
-                  std::is_same_v<T, _Float16>};
+    return Factor{b.scale, o.count, b.mean, lift<T>(o.eps)};
   }
 
   static void probs(const Operands& o, const Sums& f, const Grads& b,
@@ -1423,9 +1429,12 @@ void total(const float* loss, long rows, const int* count, bool mean,
 
 void coefficients(Type t, const Operands& o, const float* up, bool each,
                   const Grads& b, hipStream_t s) {
-  coef_kernel<<<1, 1024, 0, s>>>(up, each, b.mean, o.idx, o.tgt, o.count,
-                                 t == Type::fp16, b.coef, b.scale);
-  check(hipGetLastError());
+  by_type(t, [&](auto* q) {
+    using T = std::remove_pointer_t<decltype(q)>;
+    coef_kernel<<<1, 1024, 0, s>>>(up, each, b.mean, o.idx, o.tgt, o.count,
+                                   lift<T>(o.eps), b.coef, b.scale);
+    check(hipGetLastError());
+  });
 }
 
 void gradients_kept(Type t, const Operands& o, const Sums& f, const Grads& b,

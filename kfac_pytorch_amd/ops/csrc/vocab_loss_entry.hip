@@ -224,12 +224,12 @@ struct Gradients {
 
 // What vocab_forward kept, times up; uses it up.
 Gradients vocab_finish(const Tensor& up, const Tensor& hidden,
-                       const Tensor& weight, const Tensor& state_t, bool mean,
-                       const Kept& k) {
+                       const Tensor& weight, const Tensor& state_t,
+                       double eps, bool mean, const Kept& k) {
   const c10::OptionalDeviceGuard guard(hidden.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   const State state(state_t, hidden.size(0));
-  Call c = make_call(hidden, weight, state, 0.0, true);
+  Call c = make_call(hidden, weight, state, eps, true);
   Gradients g;
   if (k.dx_slabs.defined()) {
     g.dx = at::empty({c.o.rows, (long)c.o.dim}, hidden.options());
@@ -369,7 +369,8 @@ class VocabLoss : public torch::autograd::Function<VocabLoss> {
         for (int i = 0, j = 0; i < 4; ++i) {
           if (which >> i & 1) all[i] = kept[j++];
         }
-        g = vocab_finish(up, hidden, weight, state, reduction == MEAN,
+        g = vocab_finish(up, hidden, weight, state,
+                         saved["eps"].toDouble(), reduction == MEAN,
                          Kept{all[0], all[1], all[2], all[3]});
       } else {
         const int64_t bits = saved["need"].toInt();

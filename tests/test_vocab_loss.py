@@ -202,6 +202,31 @@ def test_many_rows(rows, ignored):
 
 @pytest.mark.gpu
 @needs_gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_the_targets_factor_is_not_rounded(dtype, reduction):
+    """1 - eps lies between two values of the type, u of itself from either;
+    with logits of zero and rows of w that add up to zero, dx is
+    -(1 - eps) w_t up, here -w_t.  2 - 2 u and 2 are neighbours: with that
+    factor rounded, dx would be 2 or less than w_t by as much."""
+    u = torch.finfo(dtype).eps / 2
+    left = 0.5 + u / 2 * 1.02
+    vocab = 65536
+    half = (2 - 2 * u) * (torch.randint(0, 2, (vocab // 2, 8), device="cuda")
+                          * 2 - 1)
+    w = torch.cat([half, -half]).to(dtype)
+    x = torch.zeros(64, 8, dtype=dtype, device="cuda")
+    t = torch.randint(0, vocab, (64,), device="cuda")
+    up = torch.full((64,) if reduction == "none" else (), 1 / left,
+                    device="cuda")
+    _, grads = run(x, w, None, t, 1 - left, reduction, up)
+    # the target's entry is -1 + 1 / vocab of the factor, the others' sum
+    # - w_t / vocab: 2^-16 each, together an 8th of fp16's half step below 1
+    assert torch.equal(grads[0], -w[t])
+
+
+@pytest.mark.gpu
+@needs_gpu
 def test_pieces_of_the_vocabulary():
     """Single rows' losses beyond 256 MB of g: two pieces, against the whole
     call with the same factors kept."""
