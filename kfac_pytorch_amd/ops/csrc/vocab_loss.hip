@@ -1228,8 +1228,9 @@ Tile logits_tile(long m, long n, long k, int size) {
 // ------------------------------------------------ the tiles of the gradients
 // dw has the vocabulary's many tiles and a k of the rows; dx has few tiles and
 // a k of the vocabulary, so that is cut up into runs, each of which writes
-// fp32 partial sums that are read once more.  The tile and the number of runs
-// are those whose time comes out least by a simple count: the workgroups of
+// fp32 partial sums that are read once more; so is the k of dw where its tiles
+// do not fill the card.  The tile and the number of runs are those whose time
+// comes out least by a simple count: the workgroups of
 // both products, the longer ones first, go to the first free place, of which a
 // CU has as many as workgroups fit into its LDS; one takes `start` us and per
 // slice of k `alone` us, or `shared` us for each of those that share its CU if
@@ -1279,29 +1280,32 @@ void plan_grads(Plan* p, long rows, long ldim, int size) {
     const Speed& speed = (size == 2 ? HALF_SPEED : FULL_SPEED)[t];
     if (speed.places == 0) continue;
     const long nx = tiles((Tile)t, ldim, rows), nw = tiles((Tile)t, ldim, piece);
-    const long cuts =
+    const long most =
         std::max<long>(1, std::min<long>({256 / nw, rows / 512, 16}));
-    const float b = (float)ceil_div(ceil_div(rows, cuts), unit);
-    for (int runs : RUNS) {
-      if (runs > 1 && runs * 128 > piece) break;
-      const float a = (float)ceil_div(ceil_div(piece, runs), unit);
-      const long all = nx * runs + nw * cuts;
-      const float share = std::min(std::max(all / 256.f, 1.f),
-                                   (float)speed.places);
-      const float slice = std::max(speed.alone, speed.shared * share);
-      const long places = all > 256 ? 256 * speed.places : 256;
-      const float ta = speed.start + a * slice, tb = speed.start + b * slice;
-      const float cost =
-          (a >= b ? ending(nx * runs, ta, nw * cuts, tb, places)
-                  : ending(nw * cuts, tb, nx * runs, ta, places)) +
-          SLAB * 4 * ldim * ((float)runs * rows +
-                             (cuts > 1 ? (float)cuts * piece : 0.f));
-      if (cost < best) {
-        best = cost;
-        p->grads = (Tile)t;
-        p->dx_splits = runs;
-        p->dw_splits = (int)cuts;
+    for (long cuts = 1;; cuts = most) {
+      const float b = (float)ceil_div(ceil_div(rows, cuts), unit);
+      for (int runs : RUNS) {
+        if (runs > 1 && runs * 128 > piece) break;
+        const float a = (float)ceil_div(ceil_div(piece, runs), unit);
+        const long all = nx * runs + nw * cuts;
+        const float share = std::min(std::max(all / 256.f, 1.f),
+                                     (float)speed.places);
+        const float slice = std::max(speed.alone, speed.shared * share);
+        const long places = all > 256 ? 256 * speed.places : 256;
+        const float ta = speed.start + a * slice, tb = speed.start + b * slice;
+        const float cost =
+            (a >= b ? ending(nx * runs, ta, nw * cuts, tb, places)
+                    : ending(nw * cuts, tb, nx * runs, ta, places)) +
+            SLAB * 4 * ldim * ((float)runs * rows +
+                               (cuts > 1 ? (float)cuts * piece : 0.f));
+        if (cost < best) {
+          best = cost;
+          p->grads = (Tile)t;
+          p->dx_splits = runs;
+          p->dw_splits = (int)cuts;
+        }
       }
+      if (cuts == most) break;
     }
   }
 }
