@@ -1230,30 +1230,31 @@ Tile logits_tile(long m, long n, long k, int size) {
 // a k of the vocabulary, so that is cut up into runs, each of which writes
 // fp32 partial sums that are read once more; so is the k of dw where its tiles
 // do not fill the card.  The tile and the number of runs are those whose time
-// comes out least by a simple count: the workgroups of
-// both products, the longer ones first, go to the first free place, of which a
-// CU has as many as workgroups fit into its LDS; one takes `start` us and per
-// slice of k `alone` us, or `shared` us for each of those that share its CU if
-// that is more; partial sums cost 0.3 us a MB.  The figures are fitted to 900
-// measured times of 19 shapes (1 to 8192 rows, 880 to 37397 entries, 32 to 1056
-// values): what it takes is 3% slower than the best of each on the mean (fp32:
-// 2%), at worst 13%; one rule for each product by itself was 25% slower.
+// comes out least by a simple count: the workgroups of both products, the
+// longer ones first, go to the first free place, of which a CU has as many as
+// workgroups fit into its LDS; one takes `start` us and per slice of k `alone`
+// us, or `shared` us for each of those that share its CU if that is more;
+// partial sums cost 0.3 us a MB.  The figures are fitted to 1319 measured times
+// of 30 shapes (1 to 8192 rows, 600 to 100000 entries, 32 to 2048 values): what
+// it takes is 2% slower than the best of each on the mean, at worst 15% (102 x
+// 11354 x 32: 11.2 us, 9.7).  A rule for each product by itself, that filled the
+// card with it, was 25% slower on the mean.
 struct Speed {
   float shared, alone, start;
   int places;
 };
 constexpr float SLAB = 0.3e-6f;  // us a byte
 
-constexpr Speed HALF_SPEED[] = {{1.02f, 1.13f, 3.2f, 1},
-                                {0.485f, 0.725f, 3.2f, 2},
+constexpr Speed HALF_SPEED[] = {{1.1f, 0.8f, 8.3f, 1},
+                                {0.44f, 0.74f, 3.5f, 2},
                                 {},
-                                {0.144f, 0.142f, 4.1f, 3},
-                                {0.155f, 0.131f, 3.6f, 3}};
+                                {0.194f, 0.28f, 3.8f, 3},
+                                {0.14f, 0.2f, 3.8f, 3}};
 constexpr Speed FULL_SPEED[] = {{},
                                 {},
-                                {0.743f, 0.989f, 4.2f, 3},
-                                {0.36f, 0.494f, 4.9f, 3},
-                                {0.222f, 0.331f, 2.6f, 3}};
+                                {0.78f, 0.97f, 4.8f, 3},
+                                {0.343f, 0.5f, 4.6f, 3},
+                                {0.216f, 0.33f, 3.0f, 3}};
 constexpr int RUNS[] = {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64};
 
 // The end of n1 jobs of length a and then n2 of length b <= a on `places`.
