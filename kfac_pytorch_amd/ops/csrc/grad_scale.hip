@@ -376,7 +376,8 @@ struct Batch {
 
   // sizes: bytes of a value of each operand
   void add(const Item<NP>& item, const std::array<long, NP>& sizes) {
-    if (!items.empty() && item.e.rows == 1 && items.back().e.rows == 1) {
+    if (!items.empty() && item.e.rows == 1 && items.back().e.rows == 1 &&
+        items.back().cols + item.cols < (1l << 33)) {
       Item<NP>& last = items.back();
       bool joins = true;
       for (int i = 0; i < NP; ++i) {
@@ -465,19 +466,47 @@ void check_lists(const char* name,
   }
 }
 
-void check_outputs(const char* name, const std::vector<Tensor>& out) {
-  std::vector<const void*> seen;
-  seen.reserve(out.size());
+// What is written: no place twice, and none of an input but its own, as it
+// lies (in place).  Of tensors with gaps, which may be woven into each other,
+// only the first value is looked at.
+void check_outputs(const char* name, const std::vector<Tensor>& in,
+                   const std::vector<Tensor>& out) {
+  struct Range {
+    const char *begin, *end;
+  };
+  const auto range = [](const Tensor& t) {
+    const char* begin = (const char*)t.const_data_ptr();
+    const bool dense = t.is_contiguous() || t.is_non_overlapping_and_dense();
+    return Range{begin, begin + (dense ? t.numel() : 1) * t.element_size()};
+  };
+  std::vector<Range> written;
+  written.reserve(out.size());
   for (const Tensor& t : out) {
     TORCH_CHECK_VALUE(t.is_contiguous() || at::has_internal_overlap(t) !=
                                                at::MemOverlap::Yes,
                       name, ": an output's values share memory");
-    if (t.numel()) seen.push_back(t.const_data_ptr());
+    if (t.numel()) written.push_back(range(t));
   }
-  std::sort(seen.begin(), seen.end());
-  TORCH_CHECK_VALUE(std::adjacent_find(seen.begin(), seen.end()) ==
-                        seen.end(),
-                    name, ": the same tensor is to be written twice");
+  std::sort(written.begin(), written.end(),
+            [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  for (size_t i = 1; i < written.size(); ++i) {
+    TORCH_CHECK_VALUE(written[i].begin >= written[i - 1].end, name,
+                      ": the same memory is to be written twice");
+  }
+  for (size_t i = 0; i < in.size(); ++i) {
+    if (in[i].numel() == 0 ||
+        (in[i].const_data_ptr() == out[i].const_data_ptr() &&
+         in[i].scalar_type() == out[i].scalar_type() &&
+         in[i].strides() == out[i].strides())) {
+      continue;
+    }
+    const Range r = range(in[i]);
+    const auto after = std::lower_bound(
+        written.begin(), written.end(), r.end,
+        [](const Range& w, const char* end) { return w.begin < end; });
+    TORCH_CHECK_VALUE(after == written.begin() || (after - 1)->end <= r.begin,
+                      name, ": an output shares memory with another input");
+  }
 }
 
 constexpr at::ScalarType TYPES[] = {at::kFloat, at::kBFloat16, at::kHalf};
@@ -544,7 +573,7 @@ Tensor grad_norm(std::vector<Tensor> tensors,
   TORCH_CHECK_VALUE(!tensors.empty(), "grad_norm: no tensors");
   if (out) {
     check_lists("clip_by_global_norm", {&tensors, &*out});
-    check_outputs("clip_by_global_norm", *out);
+    check_outputs("clip_by_global_norm", tensors, *out);
   } else {
     check_lists("global_norm", {&tensors});
   }
@@ -604,7 +633,7 @@ Tensor trust_region(std::vector<Tensor> updates, std::vector<Tensor> grads,
                     std::vector<Tensor> out, double lr, double kl) {
   TORCH_CHECK_VALUE(!updates.empty(), "kl_clip: no tensors");
   check_lists("kl_clip", {&updates, &grads, &out});
-  check_outputs("kl_clip", out);
+  check_outputs("kl_clip", updates, out);
   const c10::OptionalDeviceGuard guard(updates[0].device());
   const hipStream_t s = c10::hip::getCurrentHIPStream().stream();
   std::vector<Tensor> keep;

@@ -13,6 +13,7 @@ factors stay there.  On the CPU the plain expressions run.
 
 from __future__ import annotations
 
+import bisect
 import math
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
@@ -54,12 +55,33 @@ def _check_lists(name: str, *lists: Sequence[torch.Tensor]) -> None:
                                 f"got {t.dtype}, {t.layout}")
 
 
-def _check_outputs(name: str, out: Sequence[torch.Tensor]) -> None:
-    """Each output is written by its own workgroups: none may be there
-    twice."""
-    seen = [t.data_ptr() for t in out if t.numel()]
-    if len(set(seen)) != len(seen):
-        raise ValueError(f"{name}: the same tensor is to be written twice")
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """First byte and end; of a tensor with gaps its first value alone."""
+    n = 1 + sum((size - 1) * stride
+                for size, stride in zip(t.shape, t.stride()))
+    return (t.data_ptr(), t.data_ptr()
+            + (n if n == t.numel() else 1) * t.element_size())
+
+
+def _check_outputs(name: str, tensors: Sequence[torch.Tensor],
+                   out: Sequence[torch.Tensor]) -> None:
+    """Each output is written by workgroups of its own, while others read:
+    none may be there twice, or lie in another's input."""
+    written = sorted(_span(t) for t in out if t.numel())
+    for (_, end), (begin, _) in zip(written, written[1:]):
+        if begin < end:
+            raise ValueError(f"{name}: the same memory is to be written "
+                             "twice")
+    for t, o in zip(tensors, out):
+        if not t.numel() or (t.data_ptr() == o.data_ptr()
+                             and t.dtype == o.dtype
+                             and t.stride() == o.stride()):
+            continue
+        begin, end = _span(t)
+        at = bisect.bisect_left(written, (end, 0))
+        if at and written[at - 1][1] > begin:
+            raise ValueError(f"{name}: an output shares memory with another "
+                             "input")
 
 
 def _kind(name: str, norm_type: float) -> int:
@@ -105,7 +127,8 @@ def clip_by_global_norm(
 
     ``out``: tensors to write, of the same shapes (any of the types); the
     inputs themselves clip in place, and are then left untouched where the
-    factor is 1.  New tensors by default.  A norm that is not finite gives
+    factor is 1.  Otherwise an output must not share memory with an input or
+    another output.  New tensors by default.  A norm that is not finite gives
     what the expression gives (0 or NaN times the values).
     """
     tensors = _as_list(tensors)
@@ -124,7 +147,7 @@ def clip_by_global_norm(
         from kfac_pytorch_amd.ops import _ext
         return out, _ext.grad_norm(tensors, out, max_norm, kind)[0]
     _check_lists("clip_by_global_norm", tensors, out)
-    _check_outputs("clip_by_global_norm", out)
+    _check_outputs("clip_by_global_norm", tensors, out)
     norm = _cpu_norm(tensors, float(norm_type))
     factor = (max_norm / (norm.double() + 1e-6)).clamp(max=1.0).float()
     for t, o in zip(tensors, out):
@@ -163,8 +186,8 @@ def kl_clip(updates: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], *,
 
     ``<u, g>`` is the inner product over all tensors, summed in double.
     ``out``: tensors to write, of the same shapes (any of the types), which
-    may be the updates or the gradients themselves.  New tensors like the
-    gradients by default.  Returns them and nu (fp32, on the device).
+    may be the updates or the gradients themselves, but not share memory with
+    another's update.  New tensors like the gradients by default.  Returns them and nu (fp32, on the device).
     """
     updates, grads = _as_list(updates), _as_list(grads)
     lr, kl = float(lr), float(kl_clip)
@@ -181,7 +204,7 @@ def kl_clip(updates: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], *,
         from kfac_pytorch_amd.ops import _ext
         return out, _ext.trust_region(updates, grads, out, lr, kl)
     _check_lists("kl_clip", updates, grads, out)
-    _check_outputs("kl_clip", out)
+    _check_outputs("kl_clip", updates, out)
     total = sum((u.double() * g.double()).sum()
                 for u, g in zip(updates, grads)) * lr ** 2
     nu = (kl / total.abs().clamp_min(1e-30)).sqrt().clamp(max=1.0).float()

@@ -299,3 +299,39 @@ def test_refusals(device):
             ops.global_norm([a.double()])
         with pytest.raises(ValueError):
             ops.clip_by_global_norm([a], 1.0, out=[a[:1].expand(4, 3)])
+
+
+@devices
+def test_shared_memory(device):
+    """An output is its own input or lies apart from all of them."""
+    flat = torch.arange(1.0, 41.0, device=device)
+    a, b, c = flat[:10], flat[10:20], flat[20:30]
+    for out in ([b, a], [b, c], [flat[5:15], c], [c, flat[25:35]],
+                [a, flat[1:11]], [a.view(torch.bfloat16)[:10], c]):
+        before = flat.clone()
+        with pytest.raises(ValueError, match="memory"):
+            ops.clip_by_global_norm([a, b], 1.0, out=out)
+        with pytest.raises(ValueError, match="memory"):
+            ops.kl_clip([a, b], [c, c], lr=1.0, kl_clip=0.001, out=out)
+        assert torch.equal(flat, before)
+    with pytest.raises(ValueError, match="memory"):
+        ops.clip_by_global_norm([a, a], 1.0, out=[a, c])
+    # in place beside an output of its own, neighbours, gaps woven together
+    want = torch.linalg.vector_norm(flat[:20].double().cpu())
+    f = 1.0 / (float(want) + 1e-6)
+    wants = [a.double().cpu() * f, b.double().cpu() * f]
+    ops.clip_by_global_norm([a, b], 1.0, out=[a, c])
+    near_out([a, c], wants)
+    grid = torch.arange(1.0, 41.0, device=device).view(10, 4)
+    ins = [grid[:, :2], grid[:, 2:]]
+    wants = [t.double().cpu() / (float(torch.linalg.vector_norm(
+        grid.double())) + 1e-6) for t in ins]
+    ops.clip_by_global_norm(ins, 1.0, out=ins)
+    near_out(ins, wants)
+    # the gradients may be written: they are read before
+    us = [flat[:10].clone(), flat[10:20].clone()]
+    gs = [flat[20:30], flat[30:40]]
+    wants, nu = ops.kl_clip(us, gs, lr=1.0, kl_clip=0.001)
+    out, got = ops.kl_clip(us, gs, lr=1.0, kl_clip=0.001, out=gs[::-1])
+    assert torch.equal(nu, got)
+    assert all(torch.equal(x, y) for x, y in zip(out, wants))
