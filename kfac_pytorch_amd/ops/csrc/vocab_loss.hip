@@ -318,13 +318,13 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
 #pragma unroll
     for (int ni = 0; ni < S::NI; ++ni) {
       zs[ni] = 0.f;
-      if (t[ni] >= 0) {
+      if (t[ni] >= 0) {  // selects: a branch for each entry costs 4 us of 46
+        float z = 0.f;
 #pragma unroll
         for (int k = 0; k < S::MI * 4; ++k) {
-          if (t[ni] == (k >> 2) * 16 + (k & 3)) {
-            p.ztgt[nbase + ni * 16] = acc[k >> 2][ni][k & 3];
-          }
+          z = t[ni] == (k >> 2) * 16 + (k & 3) ? acc[k >> 2][ni][k & 3] : z;
         }
+        p.ztgt[nbase + ni * 16] = z;
       }
     }
     if (p.pz) {
@@ -420,11 +420,11 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
 #pragma unroll
     for (int ni = 0; ni < S::NI; ++ni) {
       if (t[ni] >= 0) {
+        const float less = (1.f - p.eps) * c[ni];
 #pragma unroll
         for (int q = 0; q < S::MI * 4; ++q) {
-          if (t[ni] == (q >> 2) * 16 + (q & 3)) {
-            acc[q >> 2][ni][q & 3] -= (1.f - p.eps) * c[ni];
-          }
+          acc[q >> 2][ni][q & 3] -=
+              t[ni] == (q >> 2) * 16 + (q & 3) ? less : 0.f;
         }
       }
     }
