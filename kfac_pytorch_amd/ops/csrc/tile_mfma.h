@@ -258,15 +258,17 @@ struct Operand {
   }
 };
 
-// acc (f32x4 [S::MI][S::NI]) += the product over k in [kbeg, kend); kbeg is a multiple of BK.  A
-// k-inner operand needs whole chunks up to kend; rows of a k-outer one from
-// `krows` on are taken for zeros.  `smem` is S::LDS bytes.  Every wave of the workgroup calls it with the same
-// arguments; on return all of them are done with smem.
-template <class T, bool KA, bool KB, class S, class Acc>
+// acc (f32x4 [S::MI][S::NI]) += the product over k in [kbeg, kend); kbeg is a
+// multiple of BK.  A k-inner operand needs whole chunks up to kend; rows of a
+// k-outer one from `krows` on are taken for zeros.  `smem` is S::LDS bytes.
+// begin() sets acc, while the first slices are on their way.  Every wave of the
+// workgroup calls it with the same arguments; on return all of them are done
+// with smem.
+template <class T, bool KA, bool KB, class S, class Acc, class Begin>
 __device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
                                         const T* B, long ldb, int n0, int N,
                                         int kbeg, int kend, int krows,
-                                        char* smem, Acc& acc) {
+                                        char* smem, Acc& acc, Begin begin) {
   using OA = Operand<T, KA, S::BM, S::NW>;
   using OB = Operand<T, KB, S::BN, S::NW>;
   constexpr int BK = OA::BK;
@@ -320,9 +322,9 @@ __device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
     issued += BK;
   };
 #pragma unroll
-  for (int t = 0; t < S::ST - 1; ++t) load_slice(smem + t * S::SLICE);
-  arrive<(S::ST - 2) * LOADS>();
-  load_slice(smem + (S::ST - 1) * S::SLICE);
+  for (int t = 0; t < S::ST; ++t) load_slice(smem + t * S::SLICE);
+  begin();
+  arrive<(S::ST - 1) * LOADS>();
   char* cur = smem;
 #pragma unroll
   for (int i = 0; i < FRAGS; ++i) read(cur, 0, 0, i);

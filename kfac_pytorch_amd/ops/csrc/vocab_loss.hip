@@ -273,37 +273,43 @@ __global__ __launch_bounds__(S::THREADS) void logits_kernel(
   const int vbase = m0 + wrow + g * 4;  // + 16 mi + r
   const int nbase = n0 + wcol + i;      // + 16 ni
 
-  f32x4 acc[S::MI][S::NI];
-#pragma unroll
-  for (int mi = 0; mi < S::MI; ++mi) {
-    f32x4 b = {};
-    if (bias) {
-      const int v = vbase + mi * 16;
-      T t[4] = {};
-      if (v + 4 <= p.vocab) {
-        __builtin_memcpy(t, bias + p.v0 + v, sizeof(t));
-      } else {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (v + r < p.vocab) t[r] = bias[p.v0 + v + r];
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) b[r] = (float)t[r];
-    }
-#pragma unroll
-    for (int ni = 0; ni < S::NI; ++ni) acc[mi][ni] = b;
-  }
-  tile::product<T, false, false, S>(w + (long)p.v0 * p.ldw, p.ldw, m0,
-                                    p.vocab, x, p.ldx, n0, rows, 0, p.ldx,
-                                    p.ldx, smem, acc);
-
-  // where a token's target is among this lane's entries: 16 mi + r, or none
   int t[S::NI];
 #pragma unroll
   for (int ni = 0; ni < S::NI; ++ni) {
     const int n = nbase + ni * 16;
-    t[ni] = n < rows ? p.tgt[n] - p.v0 - vbase : -1;
+    t[ni] = p.tgt[n < rows ? n : 0];
+  }
+  f32x4 acc[S::MI][S::NI];
+  const auto begin = [&] {
+#pragma unroll
+    for (int mi = 0; mi < S::MI; ++mi) {
+      f32x4 b = {};
+      if (bias) {
+        const int v = vbase + mi * 16;
+        T t[4] = {};
+        if (v + 4 <= p.vocab) {
+          __builtin_memcpy(t, bias + p.v0 + v, sizeof(t));
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if (v + r < p.vocab) t[r] = bias[p.v0 + v + r];
+          }
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) b[r] = (float)t[r];
+      }
+#pragma unroll
+      for (int ni = 0; ni < S::NI; ++ni) acc[mi][ni] = b;
+    }
+  };
+  tile::product<T, false, false, S>(w + (long)p.v0 * p.ldw, p.ldw, m0,
+                                    p.vocab, x, p.ldx, n0, rows, 0, p.ldx,
+                                    p.ldx, smem, acc, begin);
+
+  // where a token's target is among this lane's entries: 16 mi + r, or none
+#pragma unroll
+  for (int ni = 0; ni < S::NI; ++ni) {
+    t[ni] = nbase + ni * 16 < rows ? t[ni] - p.v0 - vbase : -1;
     if ((unsigned)t[ni] >= (unsigned)(S::MI * 16) || (t[ni] & 15) > 3 ||
         vbase + t[ni] >= p.vocab) {
       t[ni] = -1;
@@ -768,7 +774,7 @@ __device__ __forceinline__ void dx_body(const T* w, const T* grad, long ldg,
   const int kend = (int)ldg - kbeg < p.run ? (int)ldg : kbeg + p.run;
   f32x4 acc[S::MI][S::NI] = {};
   tile::product<T, true, false, S>(w, p.ldw, m0, dim, grad, ldg, n0, rows,
-                                   kbeg, kend, piece, smem, acc);
+                                   kbeg, kend, piece, smem, acc, [] {});
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;
   float* out = p.slabs + split * p.slab;
@@ -797,12 +803,13 @@ __device__ __forceinline__ void dw_body(const T* x, const T* grad, long ldg,
   const int m0 = tm * S::BM, n0 = tn * S::BN;
   const int kbeg = split * p.run;
   const int kend = rows - kbeg < p.run ? rows : kbeg + p.run;
+  const float inv = factor.inverse();
   f32x4 acc[S::MI][S::NI] = {};
   tile::product<T, true, true, S>(x, p.ldx, m0, ldim, grad, ldg, n0,
-                                  (int)ldg, kbeg, kend, kend, smem, acc);
+                                  (int)ldg, kbeg, kend, kend, smem, acc,
+                                  [] {});
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int i = lane & 15, g = lane >> 4;
-  const float inv = factor.inverse();
   const int d0 = m0 + (wave / S::WN) * (S::MI * 16);
   T* out = (T*)p.out;
   char* stage = smem + wave * (2 * S::MI * 256 * sizeof(T));
