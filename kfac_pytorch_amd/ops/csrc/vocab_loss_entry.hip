@@ -124,14 +124,36 @@ bool keeps(long rows, long vocab, int size) {
   return row < (1l << 22) && rows * row <= MOST_KEPT;
 }
 
-// What the forward pass leaves for vocab_finish; undefined where not needed.
-struct Kept {
-  Tensor dx_slabs, dw, dw_slabs, pbias;
-};
-
 struct Need {
   bool x, w, b;
   bool any() const { return x || w || b; }
+};
+
+// What the forward pass leaves for vocab_finish: dw, and the fp32 parts of the
+// others in one buffer; undefined where not needed.
+struct Kept {
+  Tensor parts, dw;
+};
+
+// Where what lies in Kept::parts, in floats.
+struct Parts {
+  long dx = 0, dw = 0, bias = 0;
+
+  Parts(const vocab_loss::Operands& o, Type type, Need need) {
+    if (need.x) dx = o.plan.dx_splits * o.rows * o.ldx;
+    // fp16 stays in fp32 until the upstream factor, a loss's scale, is known
+    if (need.w && (o.plan.dw_splits > 1 || type == Type::fp16)) {
+      dw = o.plan.dw_splits * o.vocab * o.ldx;
+    }
+    if (need.b) bias = o.plan.parts * o.vocab;
+  }
+  long all() const { return dx + dw + bias; }
+  void set(vocab_loss::Grads* b, const Tensor& parts) const {
+    float* at = parts.defined() ? parts.data_ptr<float>() : nullptr;
+    if (dx) b->dx_slabs = at;
+    if (dw) b->dw_slabs = at + dx;
+    if (bias) b->pbias = at + dx + dw;
+  }
 };
 
 struct Loss {
@@ -159,10 +181,14 @@ Loss vocab_forward(const Tensor& hidden, const Tensor& weight,
   Call c = make_call(hidden, weight, state, eps, r.keep);
   const auto& plan = c.o.plan;
 
-  // packed x, then the bands
-  const long xbytes = (rows * c.o.ldx * c.size + 255) / 256 * 256;
+  // packed x, the powers, the bands, and losses that are only added up
+  const long xs = (rows * c.o.ldx * c.size + 255) / 256 * 64;
+  const long row = vocab_loss::padded(vocab) * c.size;
+  const long powers = r.keep ? (rows * row + 255) / 256 * 64 : 0;
   const long bands = rows * plan.bands;
-  Tensor work = at::empty({xbytes / 4 + bands * (eps != 0.0 ? 3 : 2)}, f32);
+  Tensor work = at::empty(
+      {xs + powers + bands * (eps != 0.0 ? 3 : 2) +
+       (reduction == NONE ? 0 : rows)}, f32);
   c.o.x = work.data_ptr();
   vocab_loss::prepare(c.type, target.data_ptr(),
                       target.scalar_type() == at::kLong, rows, ignore_index,
@@ -171,22 +197,22 @@ Loss vocab_forward(const Tensor& hidden, const Tensor& weight,
                       c.o.dim, work.data_ptr(), c.o.ldx, stream);
   pack_weight(&c, weight, bias, stream);
 
-  Tensor each = at::empty({rows}, f32);
   vocab_loss::Sums f{};
-  f.pmax = work.data_ptr<float>() + xbytes / 4;
+  f.pmax = work.data_ptr<float>() + xs + powers;
   f.psum = f.pmax + bands;
   f.pz = f.psum + bands;
   f.rowm = state.rowm;
   f.rowi = state.rowi;
   f.ztgt = state.ztgt;
-  f.loss = each.data_ptr<float>();
-  Tensor grad;
-  if (r.keep) {
-    grad = at::empty({rows, vocab_loss::padded(vocab)}, hidden.options());
+  void* grad = r.keep ? work.data_ptr<float>() + xs : nullptr;
+  if (reduction == NONE) {
+    r.loss = at::empty({rows}, f32);
+    f.loss = r.loss.data_ptr<float>();
+  } else {
+    f.loss = f.pmax + bands * (eps != 0.0 ? 3 : 2);
   }
-  vocab_loss::forward(c.type, c.o, f, data(grad), stream);
+  vocab_loss::forward(c.type, c.o, f, grad, stream);
 
-  r.loss = each;
   if (reduction != NONE) {
     r.loss = at::empty({}, f32);
     f.total = r.loss.data_ptr<float>();
@@ -195,24 +221,16 @@ Loss vocab_forward(const Tensor& hidden, const Tensor& weight,
     }
   }
   if (r.keep) {
-    Kept& k = r.kept;
-    if (need.x) {
-      k.dx_slabs = at::empty({plan.dx_splits, rows, (long)c.o.ldx}, f32);
+    const Parts parts(c.o, c.type, need);
+    if (parts.all()) r.kept.parts = at::empty({parts.all()}, f32);
+    if (need.w && !parts.dw) {
+      r.kept.dw = at::empty({vocab, (long)c.o.dim}, weight.options());
     }
-    // fp16 stays in fp32 until the upstream factor, a loss's scale, is known
-    if (need.w && (plan.dw_splits > 1 || c.type == Type::fp16)) {
-      k.dw_slabs = at::empty({plan.dw_splits, vocab, (long)c.o.ldx}, f32);
-    } else if (need.w) {
-      k.dw = at::empty({vocab, (long)c.o.dim}, weight.options());
-    }
-    if (need.b) k.pbias = at::empty({plan.parts, vocab}, f32);
     vocab_loss::Grads b{};
     b.mean = mean;
-    b.pbias = floats(k.pbias);
-    b.dx_slabs = floats(k.dx_slabs);
-    b.dw_slabs = floats(k.dw_slabs);
-    b.grad = data(grad);
-    b.dw = data(k.dw);
+    b.grad = grad;
+    b.dw = data(r.kept.dw);
+    parts.set(&b, r.kept.parts);
     vocab_loss::gradients_kept(c.type, c.o, f, b, stream);
   }
   return r;
@@ -225,26 +243,22 @@ struct Gradients {
 // What vocab_forward kept, times up; uses it up.
 Gradients vocab_finish(const Tensor& up, const Tensor& hidden,
                        const Tensor& weight, const Tensor& state_t,
-                       double eps, bool mean, const Kept& k) {
+                       double eps, bool mean, Need need, const Kept& k) {
   const c10::OptionalDeviceGuard guard(hidden.device());
   const hipStream_t stream = c10::hip::getCurrentHIPStream().stream();
   const State state(state_t, hidden.size(0));
   Call c = make_call(hidden, weight, state, eps, true);
+  const Parts parts(c.o, c.type, need);
   Gradients g;
-  if (k.dx_slabs.defined()) {
-    g.dx = at::empty({c.o.rows, (long)c.o.dim}, hidden.options());
+  if (need.x) g.dx = at::empty({c.o.rows, (long)c.o.dim}, hidden.options());
+  if (need.w) {
+    g.dw = parts.dw ? at::empty({c.o.vocab, (long)c.o.dim}, weight.options())
+                    : k.dw;
   }
-  if (k.dw_slabs.defined()) {
-    g.dw = at::empty({c.o.vocab, (long)c.o.dim}, weight.options());
-  } else {
-    g.dw = k.dw;
-  }
-  if (k.pbias.defined()) g.db = at::empty({c.o.vocab}, weight.options());
+  if (need.b) g.db = at::empty({c.o.vocab}, weight.options());
   vocab_loss::Grads b{};
   b.mean = mean;
-  b.pbias = floats(k.pbias);
-  b.dx_slabs = floats(k.dx_slabs);
-  b.dw_slabs = floats(k.dw_slabs);
+  parts.set(&b, k.parts);
   b.dx = data(g.dx);
   b.dw = data(g.dw);
   b.db = data(g.db);
@@ -329,23 +343,10 @@ class VocabLoss : public torch::autograd::Function<VocabLoss> {
                                  (Reduction)reduction, need);
     ctx->save_for_backward({hidden, weight, b, r.state});
     auto& saved = ctx->saved_data;
-    saved["eps"] = eps;
-    saved["reduction"] = reduction;
-    saved["need"] = (int64_t)(need.x | need.w << 1 | need.b << 2);
-    if (r.keep) {
-      // those that are defined, and which they are
-      const Tensor all[] = {r.kept.dx_slabs, r.kept.dw, r.kept.dw_slabs,
-                            r.kept.pbias};
-      std::vector<Tensor> kept;
-      int64_t which = 0;
-      for (int i = 0; i < 4; ++i) {
-        if (!all[i].defined()) continue;
-        kept.push_back(all[i]);
-        which |= 1 << i;
-      }
-      saved["kept"] = kept;
-      saved["which"] = which;
-    }
+    saved["call"] = c10::ivalue::Tuple::create(
+        {eps, reduction, (int64_t)(need.x | need.w << 1 | need.b << 2)});
+    if (r.keep) saved["parts"] = r.kept.parts;
+    if (r.kept.dw.defined()) saved["dw"] = r.kept.dw;
     return r.loss;
   }
 
@@ -354,30 +355,31 @@ class VocabLoss : public torch::autograd::Function<VocabLoss> {
     const Tensor &hidden = tensors[0], &weight = tensors[1],
                  &bias = tensors[2], &state = tensors[3];
     auto& saved = ctx->saved_data;
-    const auto reduction = (Reduction)saved["reduction"].toInt();
+    const auto call = saved["call"].toTuple();
+    const double eps = call->elements()[0].toDouble();
+    const auto reduction = (Reduction)call->elements()[1].toInt();
+    const int64_t bits = call->elements()[2].toInt();
+    const Need need{(bits & 1) != 0, (bits & 2) != 0, (bits & 4) != 0};
     const bool differentiable = at::GradMode::is_enabled();
     Gradients g;
     {
       const at::NoGradGuard none;
       const Tensor up = grads[0].contiguous();
-      const auto at = saved.find("kept");
-      if (at != saved.end()) {
-        const std::vector<Tensor> kept = at->second.toTensorVector();
-        const int64_t which = saved["which"].toInt();
-        saved.erase(at);
-        Tensor all[4];
-        for (int i = 0, j = 0; i < 4; ++i) {
-          if (which >> i & 1) all[i] = kept[j++];
+      const auto parts = saved.find("parts");
+      if (parts != saved.end()) {
+        Kept kept;
+        if (!parts->second.isNone()) kept.parts = parts->second.toTensor();
+        saved.erase(parts);
+        const auto dw = saved.find("dw");
+        if (dw != saved.end()) {
+          kept.dw = dw->second.toTensor();
+          saved.erase(dw);
         }
-        g = vocab_finish(up, hidden, weight, state,
-                         saved["eps"].toDouble(), reduction == MEAN,
-                         Kept{all[0], all[1], all[2], all[3]});
+        g = vocab_finish(up, hidden, weight, state, eps, reduction == MEAN,
+                         need, kept);
       } else {
-        const int64_t bits = saved["need"].toInt();
-        g = vocab_backward(
-            up, hidden, weight, bias, state, saved["eps"].toDouble(),
-            reduction,
-            Need{(bits & 1) != 0, (bits & 2) != 0, (bits & 4) != 0});
+        g = vocab_backward(up, hidden, weight, bias, state, eps, reduction,
+                           need);
       }
     }
     variable_list out = {g.dx,     g.dw,     g.db,    Tensor(),
