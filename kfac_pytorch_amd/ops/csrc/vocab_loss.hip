@@ -1206,52 +1206,84 @@ long tiles(Tile t, long m, long n) {
   return (long)ceil_div(m, EDGE_M[(int)t]) * ceil_div(n, EDGE_N[(int)t]);
 }
 
-// The tile of the logits, m entries x n rows of k products, by what was measured
-// (us, for an m x n x k):
+// -------------------------------------------------------- choosing the tiles
+// A launch's time by a simple count.  A CU has as many places as workgroups fit
+// into its LDS; a workgroup takes `start` us and per slice of k `alone` us, or
+// `shared` us for each of those that share its CU if that is more.  The figures
+// are fitted to measured times.
+struct Speed {
+  float shared, alone, start;
+  int places;
+
+  float slice(long workgroups) const {
+    const float share =
+        std::min(std::max(workgroups / 256.f, 1.f), (float)places);
+    return std::max(alone, shared * share);
+  }
+  long all_places(long workgroups) const {
+    return workgroups > 256 ? 256 * places : 256;
+  }
+};
+constexpr float SLAB = 0.3e-6f;  // us a byte of fp32 that is written and read
+
+// Logits: 242 times of 48 shapes, with and without the powers.  What the count
+// takes is 0.4% slower than the best of each on the mean, at worst 5% (fp32:
+// 0.1%; a rule on the number of tiles, which took deep ones for 70 x 2246 x
+// 2080 in fp32, 37 us against 22 with thin ones, was 13% slower there).
 // wide: twice the work per byte that goes through LDS, but one workgroup fills
-//   a CU: pays once there are enough for most CUs (bf16, 16384 x 8192 x 768:
-//   217, mid 251; 9521 x 1024 x 512: 18, mid 17).
+//   a CU (bf16, 16384 x 8192 x 768: 217, mid 251; 5081 x 6852 x 32: 31, mid 27).
+// mid: a short k, some hundred rows (37215 x 88 x 416: 12.8, wide 18.6, small
+//   13.6).
 // small: fp32 products are 16 times slower for the same loads, so more
-//   workgroups to a CU lose nothing (9521 x 4096 x 1024: 590, deep 611; mid,
-//   16 waves, 610); also up to 64 rows (bf16, 33278 x 35 x 256: 6.2, wide 12.2,
-//   mid 7.7).
-// deep: few tiles, or a short k, leave little work to a workgroup: smaller ones,
-//   with 2 slices on their way (fp32, 33278 x 700 x 256: 110, small 124; but
-//   bf16, 5000 x 512 x 512: 8.5, mid 8.0).
-// thin: up to 32 rows (fp32, 30522 x 8 x 768: 18.5, small 29).
-Tile logits_tile(long m, long n, long k, int size) {
-  if (n <= 32) return Tile::thin;
-  if (size == 4) {
-    return tiles(Tile::small, m, n) * (k / 512) >= 1280 ? Tile::small
-                                                        : Tile::deep;
+//   workgroups to a CU lose nothing (9521 x 4096 x 1024: 590, deep 611); in 16
+//   bits up to 64 rows (33278 x 35 x 256: 7.6, wide 14.2, mid 9.0).
+// deep, thin: few tiles, or few rows (fp32, 30522 x 8 x 768: thin 18.5, small
+//   29; bf16, 2636 x 196 x 288: deep 5.8, mid 8.0).
+constexpr Speed HALF_LOGITS[] = {{1.13f, 1.19f, 9.3f, 1},
+                                 {0.48f, 0.57f, 4.4f, 2},
+                                 {0.36f, 0.37f, 4.1f, 3},
+                                 {0.23f, 0.25f, 4.1f, 3},
+                                 {0.09f, 0.2f, 3.4f, 3}};
+constexpr Speed FULL_LOGITS[] = {{},
+                                 {},
+                                 {1.0f, 0.91f, 5.1f, 3},
+                                 {0.55f, 0.52f, 4.3f, 3},
+                                 {0.24f, 0.285f, 3.7f, 3}};
+
+Tile logits_tile(long vocab, long rows, long k, int size) {
+  const float slices = (float)ceil_div(k * size, 128);
+  Tile taken = Tile::thin;
+  float best = INFINITY;
+  for (int t = 0; t < 5; ++t) {
+    const Speed& speed = (size == 2 ? HALF_LOGITS : FULL_LOGITS)[t];
+    if (speed.places == 0) continue;
+    const long all = tiles((Tile)t, vocab, rows);
+    const float one = speed.start + slices * speed.slice(all);
+    const float rounds = (float)all / speed.all_places(all);
+    // a last round that is filled in part takes half a round and half its part
+    const float whole = std::floor(rounds), part = rounds - whole;
+    const float cost =
+        one * (whole + (whole == 0.f ? 1.f
+                        : part > 0.f ? 0.5f + 0.5f * part : 0.f)) +
+        SLAB * 8 * rows * (float)(vocab / BAND[t]);
+    if (cost < best) {
+      best = cost;
+      taken = (Tile)t;
+    }
   }
-  if (n <= 64) {
-    return tiles(Tile::small, m, n) < 160 ? Tile::deep : Tile::small;
-  }
-  if (tiles(Tile::wide, m, n) >= 192) return Tile::wide;
-  return tiles(Tile::mid, m, n) < 128 ? Tile::deep : Tile::mid;
+  return taken;
 }
 
 // ------------------------------------------------ the tiles of the gradients
 // dw has the vocabulary's many tiles and a k of the rows; dx has few tiles and
 // a k of the vocabulary, so that is cut up into runs, each of which writes
 // fp32 partial sums that are read once more; so is the k of dw where its tiles
-// do not fill the card.  The tile and the number of runs are those whose time
-// comes out least by a simple count: the workgroups of both products, the
-// longer ones first, go to the first free place, of which a CU has as many as
-// workgroups fit into its LDS; one takes `start` us and per slice of k `alone`
-// us, or `shared` us for each of those that share its CU if that is more;
-// partial sums cost 0.3 us a MB.  The figures are fitted to 1319 measured times
-// of 30 shapes (1 to 8192 rows, 600 to 100000 entries, 32 to 2048 values): what
-// it takes is 2% slower than the best of each on the mean, at worst 15% (102 x
-// 11354 x 32: 11.2 us, 9.7).  A rule for each product by itself, that filled the
-// card with it, was 25% slower on the mean.
-struct Speed {
-  float shared, alone, start;
-  int places;
-};
-constexpr float SLAB = 0.3e-6f;  // us a byte
-
+// do not fill the card.  The workgroups of both products, the longer ones
+// first, go to the first free place.  1319 measured times of 30 shapes (1 to
+// 8192 rows, 600 to 100000 entries, 32 to 2048 values): what the count takes is
+// 2% slower than the best of each on the mean, at worst 15% (102 x 11354 x 32:
+// 11.2 us, 9.7).  A rule for each product by itself, that filled the card with
+// it, was 25% slower on the mean.
 constexpr Speed HALF_SPEED[] = {{1.1f, 0.8f, 8.3f, 1},
                                 {0.44f, 0.74f, 3.5f, 2},
                                 {},
@@ -1296,10 +1328,8 @@ void plan_grads(Plan* p, long rows, long ldim, int size) {
         if (runs > 1 && runs * 128 > piece) break;
         const float a = (float)ceil_div(ceil_div(piece, runs), unit);
         const long all = nx * runs + nw * cuts;
-        const float share = std::min(std::max(all / 256.f, 1.f),
-                                     (float)speed.places);
-        const float slice = std::max(speed.alone, speed.shared * share);
-        const long places = all > 256 ? 256 * speed.places : 256;
+        const float slice = speed.slice(all);
+        const long places = speed.all_places(all);
         const float ta = speed.start + a * slice, tb = speed.start + b * slice;
         const float cost =
             (a >= b ? ending(nx * runs, ta, nw * cuts, tb, places)
