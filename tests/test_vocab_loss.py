@@ -187,6 +187,38 @@ def test_wide_tiles(rows, dim, vocab, dtype):
               rows)
 
 
+HALVES = [torch.bfloat16, torch.float16]
+EACH_TILE = [(*shape, dtype) for shapes, dtypes in [
+    ([(660, 8, 21003), (700, 264, 16500),   # 256 x 256 of the logits
+      (360, 136, 23600),                    # and of the gradients
+      (970, 24, 5010), (2, 264, 6730),      # 128 x 128 of either
+      (33, 8, 30505),                       # 128 x 64 of the logits
+      (36, 72, 24603), (1, 200, 3372)],     # 64 x 64 of either
+     HALVES),
+    ([(68, 24, 24900), (2, 520, 8890),      # 128 x 64 of either
+      (34, 8, 30505), (1, 264, 11877)],     # 64 x 64 of either
+     [torch.float32]),
+] for shape in shapes for dtype in dtypes]
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("rows,dim,vocab,dtype", EACH_TILE)
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_each_tile(rows, dim, vocab, dtype, reduction):
+    x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.1, 31)
+    up = torch.rand(rows, device="cuda") + 0.5 if reduction == "none" \
+        else torch.ones(rows, device="cuda")
+    ref = formula(x, w, b, t, 0.05, up)
+    loss, grads = run(x, w, b, t, 0.05, reduction,
+                      up if reduction == "none" else None)
+    check_all(ref, loss if reduction == "none" else None, grads, x, w, b,
+              dtype, rows)
+    if reduction == "sum":
+        each, _ = run(x, w, b, t, 0.05, "none", up)
+        assert torch.equal(loss, each.double().sum().float())
+
+
 @pytest.mark.gpu
 @needs_gpu
 @pytest.mark.parametrize("rows", [16384, 16385, 20000])
