@@ -28,6 +28,8 @@ MI355X-first changes (not in the reference):
 
 from __future__ import annotations
 
+import contextlib
+import gc
 import logging
 from typing import Dict, List, Optional, Tuple
 
@@ -41,6 +43,47 @@ from kfac_pytorch_amd.parallel.comm import FlatBucket
 logger = logging.getLogger(__name__)
 
 SUPPORTED_MODULES = ("Linear", "Conv2d")
+
+
+class _CapturedGraph:
+    """A captured hipGraph that outlives every capture it is dropped in.
+
+    Destroying a graph waits for the device, which a stream that is being
+    captured does not allow: the destructor's exception ends the process.  A
+    preconditioner and its hooked layers refer to each other, so its graphs
+    go when the garbage collector runs, and that may be within a capture, its
+    successor's or a user's own.
+    """
+
+    _dropped: List = []  # graphs whose end is put off
+
+    def __init__(self, graph):
+        self.graph = graph
+
+    def replay(self):
+        self.graph.replay()
+
+    def __del__(self):
+        if torch.cuda.is_current_stream_capturing():
+            self._dropped.append(self.graph)
+
+    @classmethod
+    def sweep(cls):
+        if cls._dropped and not torch.cuda.is_current_stream_capturing():
+            cls._dropped.clear()
+
+
+@contextlib.contextmanager
+def _no_collection():
+    """The garbage collector does not run inside: what it would destroy may
+    need calls that a capture does not allow."""
+    was = gc.isenabled()
+    gc.disable()
+    try:
+        yield
+    finally:
+        if was:
+            gc.enable()
 
 
 class KFACBase(optim.Optimizer):
@@ -227,13 +270,15 @@ class KFACBase(optim.Optimizer):
             return
         try:
             import warnings
+            _CapturedGraph.sweep()
             side = torch.cuda.Stream()
             side.wait_stream(torch.cuda.current_stream())
             with torch.cuda.stream(side):
                 fn()  # warmup (allocator state, lazy inits)
             torch.cuda.current_stream().wait_stream(side)
             graph = torch.cuda.CUDAGraph()
-            with warnings.catch_warnings(record=True) as caught:
+            with warnings.catch_warnings(record=True) as caught, \
+                    _no_collection():
                 warnings.simplefilter("always")
                 with torch.cuda.graph(graph):
                     fn()
@@ -242,7 +287,7 @@ class KFACBase(optim.Optimizer):
             # as a capture failure and stay eager
             if any("empty" in str(w.message).lower() for w in caught):
                 raise RuntimeError("empty hipGraph capture")
-            self._graphs[key] = (graph, fingerprint)
+            self._graphs[key] = (_CapturedGraph(graph), fingerprint)
             graph.replay()
         except Exception:
             # capture-unfriendly op somewhere: stay eager for good
