@@ -46,6 +46,7 @@ def cuda(monkeypatch):
             ("is_current_stream_capturing", lambda: Graph.capturing)]:
         monkeypatch.setattr(torch.cuda, name, value)
     yield
+    gc.collect()
     base._CapturedGraph._dropped.clear()
 
 
