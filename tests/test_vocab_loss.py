@@ -187,6 +187,25 @@ def test_wide_tiles(rows, dim, vocab, dtype):
               rows)
 
 
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("rows,dim,vocab,dtype", [
+    (20000, 8, 40, torch.bfloat16),     # one band, many rows to number
+    (20000, 24, 130, torch.float32),
+    (70000, 8, 9, torch.float16),
+    (3, 8, 1200000, torch.bfloat16),    # a row of more than a million
+    (2, 8, 1100000, torch.float32),     # and one whose powers are not kept
+])
+def test_long_axes(rows, dim, vocab, dtype):
+    x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.3, 41)
+    loss, grads = run(x, w, b, t, 0.1, "sum")
+    ref = formula(x, w, b, t, 0.1, torch.ones(rows))
+    check_all(ref, None, grads, x, w, b, dtype, rows)
+    each, _ = run(x, w, b, t, 0.1, "none", torch.ones(rows, device="cuda"))
+    check_all(ref, each, None, x, w, b, dtype, rows)
+    assert torch.equal(loss, each.double().sum().float())
+
+
 HALVES = [torch.bfloat16, torch.float16]
 EACH_TILE = [(*shape, dtype) for shapes, dtypes in [
     ([(660, 8, 21003), (700, 264, 16500),   # 256 x 256 of the logits
