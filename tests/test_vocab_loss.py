@@ -206,6 +206,49 @@ def test_long_axes(rows, dim, vocab, dtype):
     assert torch.equal(loss, each.double().sum().float())
 
 
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_weight_beyond_32_bits(reduction):
+    """A weight and its gradient of 4.5 GB, against 64 bits in parts."""
+    rows, dim, vocab, part = 3, 12800, 176000, 12000
+    u = HALF[torch.bfloat16]
+    gen = torch.Generator(device="cuda").manual_seed(43)
+    w = torch.randn(vocab, dim, device="cuda", dtype=torch.bfloat16,
+                    generator=gen).mul_(2 / math.sqrt(dim))
+    assert w.numel() * 2 > 1 << 32
+    x = (torch.randn(rows, dim, device="cuda", generator=gen) / 8).bfloat16()
+    t = torch.tensor([vocab - 1, 5, vocab - 70001], device="cuda")
+    loss, (dx, dw) = run(x, w, None, t, 0.0, reduction,
+                         None if reduction == "sum"
+                         else torch.ones(rows, device="cuda"))
+    xd = x.double()
+    z = torch.cat([xd @ p.double().t() for p in w.split(part)], 1)
+    size = max(float((xd.abs() @ p.double().abs().t()).max())
+               for p in w.split(part))
+    each = torch.logsumexp(z, 1) - z.gather(1, t[:, None])[:, 0]
+    e = 2 * (dim + 8) * 2.0 ** -24 * size  # of a logit less another
+    want = each.sum() if reduction == "sum" else each
+    assert ((loss.double() - want).abs() <= rows * (e + 2.0 ** -18)).all()
+    g = z.softmax(1)
+    # an entry: its power and itself rounded, and the logits' errors
+    off = g * (e + 2 * u) + 1e-30
+    hit = torch.zeros_like(g).scatter_(1, t[:, None], 1.0)
+    g -= hit
+    off += hit * (e + u)
+    sx, ex = torch.zeros_like(xd), torch.zeros_like(xd)
+    for k, p in enumerate(w.split(part)):
+        cut = slice(k * part, (k + 1) * part)
+        p = p.double()
+        sx += g[:, cut] @ p
+        ex += (off[:, cut] + vocab * 2.0 ** -24 * g[:, cut].abs()) @ p.abs()
+        dw_want = g[:, cut].t() @ xd
+        bound = off[:, cut].t() @ xd.abs()
+        assert ((dw[cut].double() - dw_want).abs()
+                <= bound * (1 + u) + u * dw_want.abs()).all()
+    assert ((dx.double() - sx).abs() <= ex * (1 + u) + u * sx.abs()).all()
+
+
 HALVES = [torch.bfloat16, torch.float16]
 EACH_TILE = [(*shape, dtype) for shapes, dtypes in [
     ([(660, 8, 21003), (700, 264, 16500),   # 256 x 256 of the logits
