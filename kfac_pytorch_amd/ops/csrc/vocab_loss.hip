@@ -140,15 +140,31 @@ __global__ __launch_bounds__(SCAN) void scan_kernel(
 }
 
 // ------------------------------------------------------------------ packing
-// values c .. c + E of a row, zeros from `cols` on; wide: whole and aligned
+// How a row's values can be loaded: one by one; two 16-bit ones at a time, where
+// rows begin at multiples of 4 bytes; or 16 bytes of whole and aligned rows.
+enum Loads { SINGLE, PAIRS, WIDE };
+
+// values c .. c + E of a row, zeros from `cols` on
 template <class T>
 __device__ __forceinline__ void copy_chunk(const T* in, long step, int c,
-                                           int cols, int wide, T* out) {
+                                           int cols, int loads, T* out) {
   constexpr int E = 16 / sizeof(T);
   using V = __attribute__((ext_vector_type(4))) int;
   V v;
-  if (wide) {
+  if (loads == WIDE) {
     v = *reinterpret_cast<const V*>(in + c);
+  } else if (sizeof(T) == 2 && loads == PAIRS) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int k = c + 2 * j;
+      int pair = 0;
+      if (k + 2 <= cols) {
+        pair = *reinterpret_cast<const int*>(in + k);
+      } else if (k < cols) {
+        pair = *reinterpret_cast<const unsigned short*>(in + k);
+      }
+      v[j] = pair;
+    }
   } else {
     T e[E];
 #pragma unroll
@@ -160,22 +176,23 @@ __device__ __forceinline__ void copy_chunk(const T* in, long step, int c,
   *reinterpret_cast<V*>(out + c) = v;
 }
 
-// out[i, :] = in[idx ? idx[i] : i, :], zeros from `cols` to `ldo`
+// out[i, :] = in[idx ? idx[i] : i, :], zeros from `cols` to `ldo`; 2^lanes
+// lanes to a row.  Bound by memory.
 template <class T>
-__global__ void pack_kernel(const T* __restrict__ in, long ld, long step,
-                            long rows, int cols, const int* __restrict__ idx,
-                            const int* __restrict__ count,
-                            T* __restrict__ out, int ldo, int wide) {
+__global__ __launch_bounds__(256) void pack_kernel(
+    const T* __restrict__ in, long ld, long step, long rows, int cols,
+    const int* __restrict__ idx, const int* __restrict__ count,
+    T* __restrict__ out, int ldo, int loads, int lanes) {
   const long have = count ? *count : rows;
   constexpr int E = 16 / sizeof(T);
-  const int chunks = ldo / E;
-  const long total = have * chunks;
-  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < total;
-       i += (long)gridDim.x * blockDim.x) {
-    const long r = i / chunks;
-    const int c = (int)(i - r * chunks) * E;
-    copy_chunk(in + (idx ? idx[r] : r) * ld, step, c, cols, wide,
-               out + r * ldo);
+  const int chunks = ldo / E, each = 1 << lanes;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  const long all = (long)gridDim.x * 256 >> lanes;
+  for (long r = id >> lanes; r < have; r += all) {
+    const T* from = in + (idx ? idx[r] : r) * ld;
+    for (int c = (int)id & (each - 1); c < chunks; c += each) {
+      copy_chunk(from, step, c * E, cols, loads, out + r * ldo);
+    }
   }
 }
 
@@ -191,7 +208,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(
     const I* __restrict__ target, long rows, long ignore, long vocab,
     int* __restrict__ pos, int* __restrict__ idx, int* __restrict__ tgt,
     int* __restrict__ count, const T* __restrict__ in, long ld, long step,
-    int cols, T* __restrict__ out, int ldo, int wide, int prep) {
+    int cols, T* __restrict__ out, int ldo, int loads, int prep) {
   __shared__ int part[4], from[PREP], kept;
   const int t = threadIdx.x, lane = t & 63;
   const int first = blockIdx.x * prep;
@@ -225,7 +242,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(
   const int chunks = ldo / E;
   for (int k = t; k < kept * chunks; k += 256) {
     const int r = k / chunks, c = (k - r * chunks) * E;
-    copy_chunk(in + from[r] * ld, step, c, cols, wide,
+    copy_chunk(in + from[r] * ld, step, c, cols, loads,
                out + (long)(before + r) * ldo);
   }
 }
@@ -1286,8 +1303,9 @@ Tile logits_tile(long vocab, long rows, long k, int size) {
 // first, go to the first free place.  1319 measured times of 30 shapes (1 to
 // 8192 rows, 600 to 100000 entries, 32 to 2048 values): what the count takes is
 // 2% slower than the best of each on the mean, at worst 15% (102 x 11354 x 32:
-// 11.2 us, 9.7).  A rule for each product by itself, that filled the card with
-// it, was 25% slower on the mean.
+// 11.2 us, 9.7); on 8 others, of few rows and large weights, 4% on the mean, at
+// worst 7%.  A rule for each product by itself, that filled the card with it,
+// was 25% slower on the mean.
 constexpr Speed HALF_SPEED[] = {{1.1f, 0.8f, 8.3f, 1},
                                 {0.44f, 0.74f, 3.5f, 2},
                                 {},
@@ -1415,9 +1433,11 @@ void scan(const void* target, bool wide_ints, long rows, long ignore,
 }
 
 template <class T>
-bool wide_rows(const void* in, long ld, long step, int cols, int ldo) {
-  return step == 1 && ldo == cols && (uintptr_t)in % 16 == 0 &&
-         ld * sizeof(T) % 16 == 0;
+Loads loads_of(const void* in, long ld, long step, int cols, int ldo) {
+  const auto aligned = [&](long n) {
+    return step == 1 && (uintptr_t)in % n == 0 && ld * sizeof(T) % n == 0;
+  };
+  return ldo == cols && aligned(16) ? WIDE : aligned(4) ? PAIRS : SINGLE;
 }
 
 void pack(Type t, const void* in, long ld, long step, long rows, int cols,
@@ -1425,9 +1445,11 @@ void pack(Type t, const void* in, long ld, long step, long rows, int cols,
           hipStream_t s) {
   by_type(t, [&](auto* p) {
     using T = std::remove_pointer_t<decltype(p)>;
-    pack_kernel<T><<<blocks_for(rows * (ldo * sizeof(T) / 16)), 256, 0, s>>>(
+    int lanes = 0;
+    while (lanes < 6 && 16 << lanes < ldo * (int)sizeof(T)) ++lanes;
+    pack_kernel<T><<<blocks_for(rows << lanes), 256, 0, s>>>(
         (const T*)in, ld, step, rows, cols, idx, count, (T*)out, ldo,
-        wide_rows<T>(in, ld, step, cols, ldo));
+        loads_of<T>(in, ld, step, cols, ldo), lanes);
     check(hipGetLastError());
   });
 }
@@ -1448,7 +1470,7 @@ void prepare(Type t, const void* target, bool wide_ints, long rows,
       prepare_kernel<<<ceil_div(rows, prep), 256, 0, s>>>(
           targets, rows, ignore, vocab, pos, idx, tgt, count, (const T*)in,
           ld, step, cols, (T*)out, ldo,
-          (int)wide_rows<T>(in, ld, step, cols, ldo), prep);
+          (int)loads_of<T>(in, ld, step, cols, ldo), prep);
       check(hipGetLastError());
     };
     if (wide_ints) {
