@@ -357,18 +357,20 @@ __device__ __forceinline__ void product(const T* A, long lda, int m0, int M,
 // out[j * ld + c] for column j and row c.  A lane holds 4 neighbouring rows of
 // one column, v[ROWS / 16][4]; written from there, a store would be pieces of
 // 32 bytes.  They go through LDS (`lds`, the wave's own, ROWS * 16 values) and
-// leave as whole rows, 16 bytes a lane.  `cols` columns and `rows` rows exist
-// (rows a multiple of a chunk, out and ld aligned to 16 bytes).
-template <class T, int ROWS>
+// leave as whole rows, one Unit a lane.  `cols` columns and `rows` rows exist
+// (rows, out and ld in whole Units).
+struct alignas(16) Chunk16 {
+  int v[4];
+};
+
+template <class T, int ROWS, class Unit = Chunk16>
 __device__ __forceinline__ void store_columns(const T (&v)[ROWS / 16][4],
                                               char* lds, T* out, long ld,
                                               int cols, int rows, int lane) {
   constexpr int E = 16 / sizeof(T), CH = ROWS / E, LINE = ROWS * sizeof(T);
-  constexpr int EACH = 64 / CH > 0 ? 64 / CH : 1;  // columns at a time
-  static_assert(CH <= 64 && 16 % EACH == 0, "a column is at most one store");
-  struct alignas(16) Chunk {
-    T v[E];
-  };
+  constexpr int UNITS = LINE / sizeof(Unit);       // of a column
+  constexpr int SHARE = 16 / sizeof(Unit), EACH = sizeof(Unit) / sizeof(T);
+  static_assert(16 * UNITS % 64 == 0, "whole stores");
   const int i = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int m = 0; m < ROWS / 16; ++m) {
@@ -380,12 +382,13 @@ __device__ __forceinline__ void store_columns(const T (&v)[ROWS / 16][4],
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
-  for (int q = 0; q < 16 / EACH; ++q) {
-    const int j = q * EACH + lane / CH, c = lane % CH;
-    const Chunk t = *reinterpret_cast<const Chunk*>(
-        lds + j * LINE + ((c ^ (j & (CH - 1))) * 16));
-    if (j < cols && c * E < rows) {
-      *reinterpret_cast<Chunk*>(out + (long)j * ld + c * E) = t;
+  for (int q = 0; q < 16 * UNITS / 64; ++q) {
+    const int j = (q * 64 + lane) / UNITS, c = (q * 64 + lane) % UNITS;
+    const Unit t = *reinterpret_cast<const Unit*>(
+        lds + j * LINE + (((c / SHARE) ^ (j & (CH - 1))) * 16) +
+        (c % SHARE) * sizeof(Unit));
+    if (j < cols && c * EACH < rows) {
+      *reinterpret_cast<Unit*>(out + (long)j * ld + c * EACH) = t;
     }
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");

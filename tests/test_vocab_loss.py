@@ -255,10 +255,14 @@ EACH_TILE = [(*shape, dtype) for shapes, dtypes in [
       (360, 136, 23600),                    # and of the gradients
       (970, 24, 5010), (2, 264, 6730),      # 128 x 128 of either
       (33, 8, 30505),                       # 128 x 64 of the logits
-      (36, 72, 24603), (1, 200, 3372)],     # 64 x 64 of either
+      (36, 72, 24603), (1, 200, 3372),      # 64 x 64 of either
+      (360, 135, 23600), (2, 263, 6730),    # the same with odd rows
+      (1, 199, 3371), (360, 134, 23600),    # and rows of whole pairs
+      (3, 30, 700)],
      HALVES),
     ([(68, 24, 24900), (2, 520, 8890),      # 128 x 64 of either
-      (34, 8, 30505), (1, 264, 11877)],     # 64 x 64 of either
+      (34, 8, 30505), (1, 264, 11877),      # 64 x 64 of either
+      (2, 519, 8890)],
      [torch.float32]),
 ] for shape in shapes for dtype in dtypes]
 
