@@ -686,7 +686,9 @@ __global__ __launch_bounds__(256) void probs_kernel(
     for (int u = 0; u < U; ++u) {
       if (n + u >= n1) break;
       const int at = n + u - n0;
-      const float k = power(safe(b[u]), of(top, at)) * of(times, at);
+      // a band of nothing but -inf weighs nothing; taken for 0, it would be
+      // past fp32 in a row whose largest z is below -88
+      const float k = power(b[u], of(top, at)) * of(times, at);
       const int hit = __builtin_amdgcn_readlane(target, at) - v;
       const float h = of(there, at);
       float d[E];

@@ -468,6 +468,30 @@ def test_bands_masked_by_large_values(dtype, reduction):
 
 @pytest.mark.gpu
 @needs_gpu
+@pytest.mark.parametrize("dtype", list(HALF), ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("base", [-100.0, -200.0])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_masked_bands_beside_low_logits(dtype, base, reduction):
+    """Whole bands of -inf in rows whose largest logit is far below zero."""
+    x, w, b, t = inputs(50, 64, 900, dtype, True, 0.1, 4)
+    b += base
+    b[128:640] = float("-inf")
+    kept = torch.ones(900, dtype=torch.bool, device="cuda")
+    kept[128:640] = False
+    t = torch.where((t >= 128) & (t < 640), 3, t)
+    up = torch.ones(50, device="cuda") if reduction == "none" else None
+    loss, grads = run(x, w, b, t, 0.0, reduction, up)
+    each = 1 / int((t != IGNORE).sum()) if reduction == "mean" else 1.0
+    small = torch.where(t >= 640, t - 512, t)
+    ref = formula(x, w[kept], b[kept], small, 0.0, torch.full((50,), each))
+    check_all(ref, loss if up is not None else None,
+              [grads[0], grads[1][kept], grads[2][kept]], x, w[kept],
+              b[kept], dtype, 50)
+    assert not grads[1][~kept].any() and not grads[2][~kept].any()
+
+
+@pytest.mark.gpu
+@needs_gpu
 def test_all_entries_masked_alike():
     """A row of nothing but the lowest value is uniform, as in
     F.cross_entropy: the differences are zero."""
