@@ -124,10 +124,15 @@ def build_kfac(model, args, world: int):
 
 def train_loop(model, ddp_model, optimizer, preconditioner, criterion,
                batches, args, rank: int, use_cuda: bool,
-               lr_schedulers=()):
+               lr_schedulers=(), loss_of=None):
     """One epoch over `batches` (iterable of (data, target)), with the
-    reference's phase-timer breakdown in SPEED mode."""
+    reference's phase-timer breakdown in SPEED mode.  ``loss_of(data,
+    target)``: the loss, where it is not the criterion of the model's
+    output alone."""
     from kfac_pytorch_amd.utils import Metric, PhaseTimers
+    if loss_of is None:
+        def loss_of(data, target):
+            return criterion(ddp_model(data), target)
     model.train()
     timers = PhaseTimers(cuda=use_cuda)
     loss_metric = Metric("train_loss")
@@ -146,9 +151,9 @@ def train_loop(model, ddp_model, optimizer, preconditioner, criterion,
         optimizer.zero_grad(set_to_none=False)
         if autocast:
             with torch.autocast("cuda", dtype=torch.bfloat16):
-                loss = criterion(ddp_model(data), target)
+                loss = loss_of(data, target)
         else:
-            loss = criterion(ddp_model(data), target)
+            loss = loss_of(data, target)
         loss.backward()  # DDP allreduce overlaps here (COMM phase)
         if args.clip_grad:
             clip_grad_norm_(model.parameters(), args.clip_grad)

@@ -119,20 +119,17 @@ def main():
             logits = out[0] if isinstance(out, tuple) else out
             return self.ce(logits.reshape(-1, vocab), target.reshape(-1))
 
-    criterion = LMLoss()
-    forward = ddp
+    loss_of = None
     if args.fused_loss:
         # the model takes the targets and returns its loss
-        def forward(batch):
-            return ddp(batch[0], targets=batch[1])
-
-        def criterion(out, target):
-            return out[0]
+        def loss_of(data, target):
+            return ddp(data, targets=target)[0]
 
     for epoch in range(args.epochs):
         loss, iter_times = train_loop(
-            model, forward, optimizer, pre, criterion,
-            TokenBatches(args.iters_per_epoch), args, rank, use_cuda)
+            model, ddp, optimizer, pre, LMLoss(),
+            TokenBatches(args.iters_per_epoch), args, rank, use_cuda,
+            loss_of=loss_of)
         if rank == 0 and not args.speed:
             print(f"epoch {epoch}: loss={loss:.4f}")
     report_speed(iter_times, args.batch_size, world, rank)

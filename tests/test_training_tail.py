@@ -160,3 +160,41 @@ def test_trainers_run_fused():
             "--speed", "--display", "1", "--fused-loss", "--clip-grad",
             "0.25"])
         assert "images/s" in out
+
+
+def test_wikitext_trainer_takes_the_same_loss_fused(monkeypatch):
+    """Both ways of the trainer on the same batches, dropout and all: the
+    mean loss and the last step's gradients.  Sums of 32 products and losses
+    of 32 tokens, in fp32."""
+    import sys
+
+    import kfac_pytorch_amd.parallel.comm as comm_mod
+    from examples import train_wikitext_rnn as trainer
+    from tests.conftest import free_port
+    got = []
+
+    def loop(model, *args, **kw):
+        loss, times = real(model, *args, **kw)
+        got.append([torch.as_tensor(float(loss))]
+                   + [p.grad.clone() for p in model.parameters()])
+        return loss, times
+
+    real = trainer.train_loop
+    monkeypatch.setattr(trainer, "train_loop", loop)
+    for name, value in [("RANK", "0"), ("WORLD_SIZE", "1"),
+                        ("LOCAL_RANK", "0"), ("MASTER_ADDR", "127.0.0.1")]:
+        monkeypatch.setenv(name, value)
+    if torch.distributed.is_initialized():
+        torch.distributed.destroy_process_group()
+    for extra in ([], ["--fused-loss"]):
+        monkeypatch.setenv("MASTER_PORT", str(free_port()))
+        monkeypatch.setattr(sys, "argv", [
+            "train_wikitext_rnn.py", "--vocab-size", "90", "--bptt", "8",
+            "--emb", "32", "--hidden", "32", "--batch-size", "4",
+            "--iters-per-epoch", "3", "--epochs", "1", *extra])
+        comm_mod.reset()
+        trainer.main()
+        comm_mod.reset()
+    assert len(got) == 2
+    for a, b in zip(*got):
+        close(b, a, REL)
