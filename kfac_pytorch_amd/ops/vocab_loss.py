@@ -111,6 +111,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
         raise TypeError("linear_cross_entropy: hidden, weight and bias must "
                         f"have one dtype, got {hidden.dtype}, {weight.dtype}"
                         + (f", {bias.dtype}" if bias is not None else ""))
+    # what an ignored row holds must not meet its gradients' zeros
+    hidden = hidden.masked_fill((target == ignore_index).unsqueeze(-1), 0.0)
     wide = (lambda a: a if a is None or a.dtype == torch.float64
             else a.float())
     with torch.autocast(kind, enabled=False):

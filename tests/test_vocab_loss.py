@@ -722,3 +722,29 @@ def test_cpu(reduction, eps):
               torch.float32, 30)
     with pytest.raises(IndexError):
         ops.linear_cross_entropy(x, w, torch.full_like(t, 70))
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("eps", [0.0, 0.1])
+@pytest.mark.parametrize("dtype", list(HALF), ids=["bf16", "fp16", "fp32"])
+def test_ignored_rows_may_hold_anything_on_the_cpu(dtype, eps, reduction):
+    x, w, b, t = inputs(24, 16, 70, dtype, True, 0.4, 3, "cpu")
+    up = torch.rand(24) if reduction == "none" else None
+    want = run(x, w, b, t, eps, reduction, up)
+    gone = (t == IGNORE).nonzero().squeeze(1)
+    assert len(gone) >= 3
+    x[gone[0::3]] = float("nan")
+    x[gone[1::3]] = float("inf")
+    x[gone[2::3]] = torch.finfo(dtype).min
+    got = run(x, w, b, t, eps, reduction, up)
+    assert torch.equal(got[0], want[0])
+    for a, c in zip(got[1], want[1]):
+        assert torch.isfinite(a).all() and torch.equal(a, c)
+    assert not got[1][0][gone].any()
+    loss, grads = run(x, w, b, torch.full_like(t, IGNORE), eps, reduction, up)
+    if reduction == "mean":
+        assert torch.isnan(loss)
+    else:
+        assert not loss.any()
+    for g in grads:
+        assert not g.any()
