@@ -3,6 +3,7 @@
 #include <torch/extension.h>
 
 #include <ATen/autocast_mode.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -404,6 +405,12 @@ class VocabLoss : public torch::autograd::Function<VocabLoss> {
 Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
                             std::optional<Tensor> bias, int64_t ignore_index,
                             double eps, int64_t reduction) {
+  // a tangent would be lost without a word: nothing below carries it
+  const auto dual = [](const Tensor& t) { return t._fw_grad(0).defined(); };
+  TORCH_CHECK_NOT_IMPLEMENTED(
+      !c10::AutogradState::get_tls_state().get_fw_grad_mode() ||
+          !(dual(hidden) || dual(weight) || (bias && dual(*bias))),
+      "linear_cross_entropy has no forward-mode derivative on the GPU");
 #define CHECK_VALUE(cond, ...) \
   TORCH_CHECK_VALUE(cond, "linear_cross_entropy: ", __VA_ARGS__)
   CHECK_VALUE(eps >= 0.0 && eps <= 1.0,

@@ -81,7 +81,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
     floating arguments are cast as ``F.linear`` casts them.  A target outside
     the vocabulary raises on the CPU; on the GPU, where raising would mean to
     wait for the device, that row's loss and the gradients become NaN.
-    There is no double backward.
+    On the GPU there is no double backward and no forward-mode derivative;
+    both raise.
 
     On the GPU a reduced loss computes its gradients in the forward pass if
     any is asked for (evaluate under ``torch.no_grad()``).  Memory: the

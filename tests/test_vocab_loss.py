@@ -748,3 +748,47 @@ def test_ignored_rows_may_hold_anything_on_the_cpu(dtype, eps, reduction):
         assert not loss.any()
     for g in grads:
         assert not g.any()
+
+
+@pytest.mark.parametrize("which", [0, 1, 2])
+@pytest.mark.parametrize("also", [False, True])
+def test_forward_mode_is_refused(which, also):
+    """Before any check of devices, so that it can be seen without one; with
+    reverse-mode leaves among the inputs too."""
+    from torch.autograd import forward_ad
+    from kfac_pytorch_amd.ops import _ext
+    x, w, b, t = inputs(6, 16, 20, torch.float32, True, device="cpu")
+    args = [x, w, b]
+    if also:
+        args[(which + 1) % 3].requires_grad_()
+    with forward_ad.dual_level():
+        args[which] = forward_ad.make_dual(args[which],
+                                           torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            _ext.linear_cross_entropy(args[0], args[1], t, args[2], IGNORE,
+                                      0.0, 1)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(
+    "cuda", marks=[pytest.mark.gpu, needs_gpu])])
+def test_forward_mode(device):
+    """The CPU has the tangent, the GPU refuses; without tangents, or with
+    forward mode switched off, it answers."""
+    from torch.autograd import forward_ad
+    x, w, b, t = inputs(6, 16, 20, torch.float32, True, device=device)
+    want = ops.linear_cross_entropy(x, w, t, bias=b)
+    with forward_ad.dual_level():
+        got = ops.linear_cross_entropy(x, w, t, bias=b)
+        assert torch.equal(got, want)
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        if device == "cpu":
+            loss = ops.linear_cross_entropy(dual, w, t, bias=b)
+            slope = forward_ad.unpack_dual(loss).tangent
+            leaf = x.clone().requires_grad_()
+            dx, = torch.autograd.grad(
+                ops.linear_cross_entropy(leaf, w, t, bias=b), leaf)
+            # sums of 96 values and of 20 logits' terms, each below 8
+            assert abs(slope - dx.sum()) <= 256 * 2.0 ** -24 * 8
+        else:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                ops.linear_cross_entropy(dual, w, t, bias=b)
