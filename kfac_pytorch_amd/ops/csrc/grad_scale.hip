@@ -459,6 +459,8 @@ void check_lists(const char* name,
                             type == at::kHalf),
                        name, ": dense fp32, bf16 or fp16 expected on the "
                              "GPU, got ", type, ", ", t.layout());
+      TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), name,
+                                  " has no forward-mode derivative");
       TORCH_CHECK_VALUE(list == &first || t.sizes() == first[i].sizes(),
                         name, ": shapes ", first[i].sizes(), " and ",
                         t.sizes(), " differ");

@@ -8,7 +8,9 @@
 
 On the GPU two passes over the data, a few launches whatever the number of
 tensors (``csrc/grad_scale.hip``), and no wait for the device: norms and
-factors stay there.  On the CPU the plain expressions run.
+factors stay there.  On the CPU the plain expressions run.  None of them is
+differentiated: results require no gradient, and tensors with a forward-mode
+tangent raise.
 """
 
 from __future__ import annotations
@@ -18,6 +20,7 @@ import math
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
+from torch.autograd import forward_ad
 
 __all__ = ["global_norm", "clip_by_global_norm", "clip_grad_norm_",
            "kl_clip"]
@@ -53,6 +56,9 @@ def _check_lists(name: str, *lists: Sequence[torch.Tensor]) -> None:
             if not t.dtype.is_floating_point or t.layout != torch.strided:
                 raise TypeError(f"{name}: dense floating tensors expected, "
                                 f"got {t.dtype}, {t.layout}")
+            if forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} has no forward-mode "
+                                          "derivative")
 
 
 def _span(t: torch.Tensor) -> Tuple[int, int]:

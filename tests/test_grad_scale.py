@@ -335,3 +335,20 @@ def test_shared_memory(device):
     out, got = ops.kl_clip(us, gs, lr=1.0, kl_clip=0.001, out=gs[::-1])
     assert torch.equal(nu, got)
     assert all(torch.equal(x, y) for x, y in zip(out, wants))
+
+
+@devices
+def test_forward_mode_is_refused(device):
+    """A clipped tensor's tangent would lack the norm's part, or be lost."""
+    from torch.autograd import forward_ad
+    a, b = tensors([(5, 3), (5, 3)], torch.float32, device)
+    with forward_ad.dual_level():
+        ops.clip_by_global_norm([a], 1.0, out=[b.clone()])
+        d = forward_ad.make_dual(a, b)
+        for call in (lambda: ops.global_norm([a, d]),
+                     lambda: ops.clip_by_global_norm([d], 1.0),
+                     lambda: ops.clip_by_global_norm([a], 1.0, out=[d]),
+                     lambda: ops.kl_clip([d], [b], lr=1.0, kl_clip=0.001),
+                     lambda: ops.kl_clip([a], [d], lr=1.0, kl_clip=0.001)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
