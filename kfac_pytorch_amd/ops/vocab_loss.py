@@ -24,6 +24,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.nn.modules import module
 
 __all__ = ["linear_cross_entropy", "projection_loss"]
 
@@ -130,15 +131,29 @@ def projection_loss(layer: torch.nn.Linear, hidden: torch.Tensor,
     """``linear_cross_entropy`` with an output layer's weight and bias.
 
     The layer itself is not called, so nothing that hangs on its calls may
-    be left waiting: a layer with hooks (K-FAC's, of a preconditioner that
-    does not leave the vocabulary projection out) is refused.
+    be left waiting, and the call may be nothing else than ``F.linear``: a
+    layer with hooks (K-FAC's, of a preconditioner that does not leave the
+    vocabulary projection out; hooks on all modules too) or with a forward
+    pass of its own (an adapter, a scaled or quantised head) is refused.
     """
-    if (layer._forward_pre_hooks or layer._forward_hooks
-            or layer._backward_hooks or layer._backward_pre_hooks):
+    plain = getattr(layer, "_orig_mod", layer)  # of torch.compile(layer)
+    if any(getattr(m, name) for m in {layer, plain}
+           for name in ("_forward_pre_hooks", "_forward_hooks",
+                        "_backward_hooks", "_backward_pre_hooks")) or any(
+            getattr(module, "_global" + name, None)
+            for name in ("_forward_pre_hooks", "_forward_hooks",
+                         "_backward_hooks", "_backward_pre_hooks")):
         raise RuntimeError(
             "the vocabulary projection carries hooks, which a loss without "
             "logits does not run; leave the layer out of K-FAC "
-            f"(exclude_vocabulary_size={layer.out_features}) or take the "
+            f"(exclude_vocabulary_size={plain.weight.size(0)}) or take the "
             "loss from the logits")
-    return linear_cross_entropy(hidden, layer.weight, target,
-                                bias=layer.bias, **kw)
+    if (getattr(type(plain), "forward", None) is not torch.nn.Linear.forward
+            or type(plain).__call__ is not torch.nn.Module.__call__
+            or "forward" in vars(plain)):
+        raise RuntimeError(
+            f"the vocabulary projection, a {type(plain).__name__}, has a "
+            "forward pass of its own, which a loss without logits does not "
+            "run; take the loss from the logits")
+    return linear_cross_entropy(hidden, plain.weight, target,
+                                bias=plain.bias, **kw)

@@ -198,3 +198,79 @@ def test_wikitext_trainer_takes_the_same_loss_fused(monkeypatch):
     assert len(got) == 2
     for a, b in zip(*got):
         close(b, a, REL)
+
+
+class Adapted(torch.nn.Linear):
+    def forward(self, x):
+        return super().forward(x) * 0.5
+
+
+class Counted(torch.nn.Linear):
+    def __call__(self, x):
+        return super().__call__(x) + 1
+
+
+@pytest.mark.parametrize("kind", ["subclass", "call", "instance", "other",
+                                  "global pre", "global", "global backward"])
+def test_projection_that_is_more_than_linear_is_refused(kind):
+    """model(x, targets=y) must not be the loss of another model than
+    model(x) is."""
+    from torch.nn.modules import module as hooks
+    model, x, y = lstm("cpu")
+    d, handle = model.decoder, None
+    if kind in ("subclass", "call"):
+        d = (Adapted if kind == "subclass" else Counted)(32, VOCAB)
+        d.load_state_dict(model.decoder.state_dict())
+    elif kind == "instance":
+        d.forward = lambda x: F.linear(x, d.weight) * 2
+    elif kind == "other":
+        class Head(torch.nn.Module):
+            def __init__(self):
+                super().__init__()
+                self.weight, self.bias = model.decoder.weight, None
+                self.out_features = VOCAB
+
+            def forward(self, x):
+                return F.linear(x, self.weight).tanh()
+        d = Head()
+    elif kind == "global pre":
+        handle = hooks.register_module_forward_pre_hook(lambda m, a: None)
+    elif kind == "global":
+        handle = hooks.register_module_forward_hook(lambda m, a, o: None)
+    else:
+        handle = hooks.register_module_full_backward_hook(
+            lambda m, a, o: None)
+    model.decoder = d
+    try:
+        with pytest.raises(RuntimeError, match="loss without logits|loss "
+                                               "from the logits"):
+            ops.projection_loss(d, torch.randn(4, 32), y[0, :4])
+        with pytest.raises(RuntimeError, match="from the logits"):
+            model(x, targets=y)
+    finally:
+        if handle is not None:
+            handle.remove()
+
+
+def test_projections_that_are_linear_are_taken():
+    """Parametrised, subclassed without another forward pass, compiled: the
+    loss is that of the layer's own output."""
+    from torch.nn.utils import parametrize
+
+    class Named(torch.nn.Linear):
+        pass
+
+    class Half(torch.nn.Module):
+        def forward(self, w):
+            return w / 2
+
+    torch.manual_seed(0)
+    x, t = torch.randn(6, 16), torch.randint(20, (6,))
+    layers = [torch.nn.Linear(16, 20), Named(16, 20, bias=False),
+              torch.nn.Linear(16, 20)]
+    parametrize.register_parametrization(layers[2], "weight", Half())
+    layers.append(torch.compile(torch.nn.Linear(16, 20), backend="eager"))
+    for layer in layers:
+        plain = getattr(layer, "_orig_mod", layer)
+        want = F.cross_entropy(plain(x), t)
+        close(ops.projection_loss(layer, x, t), want, REL)
