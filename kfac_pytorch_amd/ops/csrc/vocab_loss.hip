@@ -928,7 +928,7 @@ __device__ __forceinline__ void add_body(const Adding& a, float f,
     }
     T o[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = (T)(s[r] * f);
+    for (int r = 0; r < 4; ++r) o[r] = (T)(p >= 0 ? s[r] * f : 0.f);
     T* out = (T*)a.out + n * a.dim + d;
     if (d + 4 <= a.dim) {
       __builtin_memcpy(out, o, sizeof(o));
@@ -1006,8 +1006,10 @@ template <class T>
 __global__ __launch_bounds__(256) void end_kernel(
     const Adding dx, const Adding dw, const Bias db, const Times dw_times,
     const Factor factor, const float* __restrict__ up) {
-  const float u = up ? *up : 1.f;
-  const float f = factor.inverse() * u;
+  // no rows, no gradient, whatever the factor: 0 times infinity is none
+  const bool any = *factor.count > 0;
+  const float u = up && any ? *up : 1.f;
+  const float f = any ? factor.inverse() * u : 0.f;
   int block = blockIdx.x;
   if (block < dx.blocks) return add_body<T>(dx, f, block);
   block -= dx.blocks;

@@ -792,3 +792,22 @@ def test_forward_mode(device):
         else:
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 ops.linear_cross_entropy(dual, w, t, bias=b)
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("dtype", list(HALF), ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_ignored_rows_beside_a_factor_that_is_not_finite(value, dtype,
+                                                         reduction):
+    """An overflowed loss scale reaches the rows that count; the ignored
+    ones, and all gradients of a call where no row counts, stay zero."""
+    x, w, b, t = inputs(70, 64, 300, dtype, True, 0.4, 3)
+    up = torch.full((70,) if reduction == "none" else (), value,
+                    device="cuda")
+    _, grads = run(x, w, b, t, 0.1, reduction, up)
+    assert not grads[0][t == IGNORE].any()
+    assert not torch.isfinite(grads[0][t != IGNORE]).all()
+    _, grads = run(x, w, b, torch.full_like(t, IGNORE), 0.1, reduction, up)
+    assert not any(g.any() for g in grads)
