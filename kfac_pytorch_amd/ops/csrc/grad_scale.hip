@@ -464,6 +464,9 @@ void check_lists(const char* name,
       TORCH_CHECK_VALUE(list == &first || t.sizes() == first[i].sizes(),
                         name, ": shapes ", first[i].sizes(), " and ",
                         t.sizes(), " differ");
+      // sharded or fake tensors name a device and have no memory there
+      TORCH_CHECK_TYPE(t.numel() == 0 || t.const_data_ptr() != nullptr, name,
+                       ": tensors with memory of their own expected");
     }
   }
 }

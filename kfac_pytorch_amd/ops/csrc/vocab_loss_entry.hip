@@ -434,6 +434,15 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
                   target.device() == hidden.device() &&
                   (!bias || bias->device() == hidden.device()),
               "all tensors must be on ", hidden.device());
+  // sharded or fake tensors name a device and have no memory there
+  const auto dense = [](const Tensor& t) {
+    return t.layout() == at::kStrided &&
+           (t.numel() == 0 || t.const_data_ptr() != nullptr);
+  };
+  TORCH_CHECK_TYPE(dense(hidden) && dense(weight) && dense(target) &&
+                       (!bias || dense(*bias)),
+                   "linear_cross_entropy: dense tensors with memory of their "
+                   "own expected");
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     const auto t = at::autocast::get_autocast_dtype(at::kCUDA);
     hidden = at::autocast::cached_cast(t, hidden, at::kCUDA);

@@ -352,3 +352,48 @@ def test_forward_mode_is_refused(device):
                      lambda: ops.kl_clip([a], [d], lr=1.0, kl_clip=0.001)):
             with pytest.raises(NotImplementedError, match="forward-mode"):
                 call()
+
+
+class Storageless(torch.Tensor):
+    """As a sharded or a fake tensor: a device's name without memory."""
+
+    @staticmethod
+    def __new__(cls, shape):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, shape, dtype=torch.float32, device="cuda")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        assert func is torch.ops.aten.detach.default, func
+        return cls(args[0].shape)
+
+
+class Parameter:
+    def __init__(self, grad):
+        self.grad = grad
+
+
+def test_tensors_without_memory_are_refused():
+    """On the host: a kernel would read from address zero."""
+    a, b, c = (Storageless((5, 3)) for _ in range(3))
+    assert a.is_cuda and a.data_ptr() == 0
+    for call in (lambda: ops.global_norm([a, b]),
+                 lambda: ops.clip_by_global_norm([a], 1.0, out=[a]),
+                 lambda: ops.clip_by_global_norm([a], 1.0, out=[b]),
+                 lambda: ops.kl_clip([a], [b], lr=1.0, kl_clip=0.001,
+                                     out=[c]),
+                 lambda: ops.clip_grad_norm_([Parameter(a)], 1.0)):
+        with pytest.raises(TypeError, match="memory of their own"):
+            call()
+
+
+@only_gpu
+def test_one_tensor_without_memory_is_refused(device):
+    a = Storageless((5, 3))
+    b = torch.ones(5, 3, device=device)
+    for call in (lambda: ops.global_norm([b, a]),
+                 lambda: ops.clip_by_global_norm([b], 1.0, out=[a]),
+                 lambda: ops.kl_clip([b], [a], lr=1.0, kl_clip=0.001,
+                                     out=[b])):
+        with pytest.raises((TypeError, ValueError)):
+            call()

@@ -811,3 +811,44 @@ def test_ignored_rows_beside_a_factor_that_is_not_finite(value, dtype,
     assert not torch.isfinite(grads[0][t != IGNORE]).all()
     _, grads = run(x, w, b, torch.full_like(t, IGNORE), 0.1, reduction, up)
     assert not any(g.any() for g in grads)
+
+
+class Storageless(torch.Tensor):
+    """As a sharded or a fake tensor: a device's name without memory."""
+
+    @staticmethod
+    def __new__(cls, like):
+        return torch.Tensor._make_wrapper_subclass(
+            cls, like.shape, dtype=like.dtype, device="cuda")
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise AssertionError(f"{func} is not for the test")
+
+
+def test_tensors_without_memory_are_refused():
+    """On the host: a kernel would read from address zero."""
+    x, w, b, t = inputs(6, 16, 20, torch.float32, True, device="cpu")
+    x, w, b, t = (Storageless(a) for a in (x, w, b, t))
+    assert x.is_cuda and x.data_ptr() == 0
+    for bias in (b, None):
+        with pytest.raises(TypeError, match="memory of their own"):
+            ops.linear_cross_entropy(x, w, t, bias=bias)
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("which", range(4))
+def test_one_tensor_without_memory_is_refused(which):
+    args = list(inputs(6, 16, 20, torch.float32, True))
+    args[which] = Storageless(args[which])
+    x, w, b, t = args
+    with pytest.raises((TypeError, ValueError)):
+        ops.linear_cross_entropy(x, w, t, bias=b)
+
+
+def test_sparse_tensors_are_refused():
+    x, w, b, t = inputs(6, 16, 20, torch.float32, True, device="cpu")
+    from kfac_pytorch_amd.ops import _ext
+    with pytest.raises((TypeError, ValueError)):
+        _ext.linear_cross_entropy(x.to_sparse(), w, t, b, IGNORE, 0.0, 1)
