@@ -516,6 +516,12 @@ void check_outputs(const char* name, const std::vector<Tensor>& in,
 
 constexpr at::ScalarType TYPES[] = {at::kFloat, at::kBFloat16, at::kHalf};
 
+// The imaginary part of a lazy conjugate is memory with a sign pending on it.
+// The kernels read and write memory, which is right where both operands have
+// the sign or neither has.
+bool other_sign(const Tensor& a, const Tensor& b) {
+  return a.is_neg() != b.is_neg();
+}
 
 template <int NP>
 Item<NP> must(const std::array<const Tensor*, NP>& t) {
@@ -536,8 +542,8 @@ void scale_pass(const std::vector<Tensor>& in, const std::vector<Tensor>& out,
           continue;
         }
         Item<2> e{};
-        if (!as_rows<2>({&in[i], &out[i]}, &e)) {
-          Tensor a = in[i].contiguous();
+        if (other_sign(in[i], out[i]) || !as_rows<2>({&in[i], &out[i]}, &e)) {
+          Tensor a = in[i].resolve_neg().contiguous();
           Tensor b = at::empty(out[i].sizes(), out[i].options());
           e = must<2>({&a, &b});
           copies.emplace_back(out[i], b);
@@ -652,9 +658,10 @@ Tensor trust_region(std::vector<Tensor> updates, std::vector<Tensor> grads,
         continue;
       }
       Item<2> e{};
-      if (!as_rows<2>({&updates[i], &grads[i]}, &e)) {
-        keep.push_back(updates[i].contiguous());
-        keep.push_back(grads[i].contiguous());
+      if (other_sign(updates[i], grads[i]) ||
+          !as_rows<2>({&updates[i], &grads[i]}, &e)) {
+        keep.push_back(updates[i].resolve_neg().contiguous());
+        keep.push_back(grads[i].resolve_neg().contiguous());
         e = must<2>({&keep[keep.size() - 2], &keep.back()});
       }
       batch[k].add(e, {(long)updates[i].element_size(),

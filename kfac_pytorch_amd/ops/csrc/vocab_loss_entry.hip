@@ -365,7 +365,7 @@ class VocabLoss : public torch::autograd::Function<VocabLoss> {
     Gradients g;
     {
       const at::NoGradGuard none;
-      const Tensor up = grads[0].contiguous();
+      const Tensor up = grads[0].resolve_neg().contiguous();
       const auto parts = saved.find("parts");
       if (parts != saved.end()) {
         Kept kept;
@@ -443,6 +443,10 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
                        (!bias || dense(*bias)),
                    "linear_cross_entropy: dense tensors with memory of their "
                    "own expected");
+  // the kernels read memory: no sign may be pending on it
+  hidden = hidden.resolve_neg();
+  weight = weight.resolve_neg();
+  if (bias) bias = bias->resolve_neg();
   if (at::autocast::is_autocast_enabled(at::kCUDA)) {
     const auto t = at::autocast::get_autocast_dtype(at::kCUDA);
     hidden = at::autocast::cached_cast(t, hidden, at::kCUDA);

@@ -397,3 +397,45 @@ def test_one_tensor_without_memory_is_refused(device):
                                      out=[b])):
         with pytest.raises((TypeError, ValueError)):
             call()
+
+
+@devices
+def test_tensors_with_a_pending_sign(device):
+    """The imaginary part of a lazy conjugate is memory to be negated."""
+    def lazy(a):
+        a = torch.complex(torch.zeros_like(a), -a).conj().imag
+        assert a.is_neg()
+        return a
+
+    us = tensors([(64, 33), (5,), (9000,)], torch.float32, device, 1)
+    gs = tensors([(64, 33), (5,), (9000,)], torch.float32, device, 2)
+    gs = [u + 0.1 * g for u, g in zip(us, gs)]
+    clipped, norm = ops.clip_by_global_norm(us, 1.0)
+    out, nu = ops.kl_clip(us, gs, lr=1.0, kl_clip=0.001)
+
+    def same(got, want, number, wanted):
+        near(number, wanted.double().cpu(), 2.0 ** -23)
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+    same(*[[lazy(u) for u in us], us], ops.global_norm(
+        [lazy(u) for u in us]), norm)
+    got, n = ops.clip_by_global_norm([lazy(u) for u in us], 1.0)
+    same(got, clipped, n, norm)
+    got, n = ops.clip_by_global_norm(us, 1.0, out=[lazy(u) for u in us])
+    same(got, clipped, n, norm)
+    both = [lazy(u) for u in us]
+    got, n = ops.clip_by_global_norm(both, 1.0, out=both)
+    same(both, clipped, n, norm)
+    for a, b in (([lazy(u) for u in us], gs), (us, [lazy(g) for g in gs]),
+                 ([lazy(u) for u in us], [lazy(g) for g in gs])):
+        written = [torch.zeros(g.shape, device=device) for g in gs]
+        got, n = ops.kl_clip(a, b, lr=1.0, kl_clip=0.001, out=written)
+        same(written, out, n, nu)
+    got, n = ops.kl_clip([lazy(u) for u in us], [lazy(g) for g in gs], lr=1.0,
+                         kl_clip=0.001)
+    same(got, out, n, nu)
+    # the sign is pending on one of the two only: written over the gradients
+    both = [lazy(g) for g in gs]
+    got, n = ops.kl_clip(us, both, lr=1.0, kl_clip=0.001, out=both)
+    same(both, out, n, nu)

@@ -852,3 +852,26 @@ def test_sparse_tensors_are_refused():
     from kfac_pytorch_amd.ops import _ext
     with pytest.raises((TypeError, ValueError)):
         _ext.linear_cross_entropy(x.to_sparse(), w, t, b, IGNORE, 0.0, 1)
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param(
+    "cuda", marks=[pytest.mark.gpu, needs_gpu])])
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_operands_with_a_pending_sign(device, reduction):
+    """The imaginary part of a lazy conjugate is memory to be negated."""
+    args = inputs(20, 16, 70, torch.float32, True, 0.1, 3, device)
+    t = args[3]
+
+    def lazy(a):
+        a = torch.complex(torch.zeros_like(a), -a).conj().imag
+        assert a.is_neg()
+        return a
+
+    up = torch.rand(20, device=device) if reduction == "none" else \
+        torch.tensor(2.0, device=device)
+    want = run(*args, reduction=reduction, up=up)
+    got = run(*(lazy(a) for a in args[:3]), t, reduction=reduction,
+              up=lazy(up))
+    assert torch.equal(got[0], want[0])
+    for a, c in zip(got[1], want[1]):
+        assert torch.equal(a, c)
