@@ -178,6 +178,17 @@ def linear_cross_entropy(hidden, weight, target, bias, ignore_index: int,
                                         ignore_index, eps, reduction)
 
 
+def linear_cross_entropy_plan(rows: int, vocab: int, dim: int, size: int,
+                              keep: bool) -> dict:
+    """How a call of these sizes (values of ``size`` bytes) is cut up; keep:
+    with the powers kept for the gradients.  Needs no GPU."""
+    tiles = ("wide", "mid", "small", "deep", "thin")
+    logits, grads, piece, dx, dw, items = _load().linear_cross_entropy_plan(
+        rows, vocab, dim, size, keep)
+    return {"logits": tiles[logits], "grads": tiles[grads], "piece": piece,
+            "dx_splits": dx, "dw_splits": dw, "work_items": items}
+
+
 # -- one norm or inner product over many tensors ------------------------------
 def grad_norm(tensors, out, max_norm: float, kind: int) -> torch.Tensor:
     """[norm, factor], fp32 on the GPU; ``out`` (a list, or None) gets the

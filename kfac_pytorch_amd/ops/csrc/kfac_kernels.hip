@@ -431,6 +431,10 @@ torch::Tensor linear_cross_entropy(torch::Tensor hidden, torch::Tensor weight,
                                    int64_t ignore_index, double eps,
                                    int64_t reduction);
 
+std::vector<int64_t> linear_cross_entropy_plan(int64_t rows, int64_t vocab,
+                                               int64_t dim, int64_t size,
+                                               bool keep);
+
 // defined in grad_scale.hip
 torch::Tensor grad_norm(std::vector<torch::Tensor> tensors,
                         std::optional<std::vector<torch::Tensor>> out,
@@ -455,6 +459,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "largest dim the Jacobi kernel handles");
   m.def("linear_cross_entropy", &linear_cross_entropy,
         "cross entropy of a vocabulary projection, no logits in memory");
+  m.def("linear_cross_entropy_plan", &linear_cross_entropy_plan,
+        "how a call of given sizes is cut up");
   m.def("grad_norm", &grad_norm,
         "norm over many tensors, and their rescale by it");
   m.def("trust_region", &trust_region,

@@ -35,6 +35,9 @@ struct Plan {
 
 // keep: the whole vocabulary's powers are kept for the gradients
 Plan plan(long rows, long vocab, int ldim, int size, bool keep);
+// Work items of a plan's largest launch.  The runtime launches fewer than 2^32.
+long work_items(const Plan& p, long rows, long vocab, int ldim, int size,
+                bool keep);
 
 long padded(long n);  // to whole 16-byte chunks of every type
 

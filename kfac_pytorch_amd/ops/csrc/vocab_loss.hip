@@ -1425,6 +1425,28 @@ Plan plan(long rows, long vocab, int ldim, int size, bool keep) {
   return last.plan;
 }
 
+long work_items(const Plan& p, long rows, long vocab, int ldim, int size,
+                bool keep) {
+  static_assert(Wide::THREADS == 512 && Mid::THREADS == 512 &&
+                    Small::THREADS == 256 && Deep::THREADS == 256 &&
+                    Thin::THREADS == 256, "as below");
+  const auto threads = [](Tile t) {
+    return t == Tile::wide || t == Tile::mid ? 512l : 256l;
+  };
+  const auto blocks = [](long a, long b) { return (a + b - 1) / b; };
+  const long logits = tiles(p.logits, vocab, rows) * threads(p.logits);
+  const long grads = (tiles(p.grads, ldim, rows) * p.dx_splits +
+                      tiles(p.grads, ldim, p.piece) * p.dw_splits) *
+                     threads(p.grads);
+  const long join = blocks(rows, 4) * 256;
+  const long probs =
+      keep ? (blocks(rows, p.part) * blocks(padded(vocab) * size, 4096) + 1) *
+                 256
+           : 0;
+  const long end = (3 * 8192 + blocks(vocab, 64)) * 256;
+  return std::max({logits, grads, join, probs, end});
+}
+
 void scan(const void* target, bool wide_ints, long rows, long ignore,
           long vocab, int* pos, int* idx, int* tgt, int* count,
           hipStream_t s) {

@@ -125,6 +125,27 @@ bool keeps(long rows, long vocab, int size) {
   return row < (1l << 22) && rows * row <= MOST_KEPT;
 }
 
+// Whether every launch of a call of these sizes is possible.
+bool launches(long rows, long vocab, int ldim, int size) {
+  constexpr long MOST = 1l << 32;
+  // the smallest tiles and the most cuts: fewer, and no plan need be made
+  const long dx = (ldim / 64 + 1) * (rows / 32 + 1) * 64,
+             dw = (ldim / 64 + 1) * (vocab / 32 + 1) * 16;
+  if (rows < (1l << 25) && vocab < (1l << 25) &&
+      (vocab / 64 + 1) * (rows / 32 + 1) * 256 < MOST &&
+      (dx + dw) * 256 < MOST) {
+    return true;
+  }
+  for (bool keep : {false, true}) {
+    if (keep && !keeps(rows, vocab, size)) continue;
+    const auto plan = vocab_loss::plan(rows, vocab, ldim, size, keep);
+    if (vocab_loss::work_items(plan, rows, vocab, ldim, size, keep) >= MOST) {
+      return false;
+    }
+  }
+  return true;
+}
+
 struct Need {
   bool x, w, b;
   bool any() const { return x || w || b; }
@@ -434,6 +455,16 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
                   target.device() == hidden.device() &&
                   (!bias || bias->device() == hidden.device()),
               "all tensors must be on ", hidden.device());
+  const bool casts = at::autocast::is_autocast_enabled(at::kCUDA);
+  const auto cast = at::autocast::get_autocast_dtype(at::kCUDA);
+  const int64_t d = hidden.size(-1), n = hidden.numel() / d,
+                size = c10::elementSize(casts ? cast : hidden.scalar_type());
+  CHECK_VALUE(n > 0 && n < (1l << 30) && weight.size(0) < (1l << 30) &&
+                  d * size < (1l << 22) &&
+                  launches(n, weight.size(0), (int)vocab_loss::padded(d),
+                           (int)size),
+              "sizes out of range: ", hidden.sizes(), " and ",
+              weight.sizes());
   // sharded or fake tensors name a device and have no memory there
   const auto dense = [](const Tensor& t) {
     return t.layout() == at::kStrided &&
@@ -447,11 +478,10 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
   hidden = hidden.resolve_neg();
   weight = weight.resolve_neg();
   if (bias) bias = bias->resolve_neg();
-  if (at::autocast::is_autocast_enabled(at::kCUDA)) {
-    const auto t = at::autocast::get_autocast_dtype(at::kCUDA);
-    hidden = at::autocast::cached_cast(t, hidden, at::kCUDA);
-    weight = at::autocast::cached_cast(t, weight, at::kCUDA);
-    if (bias) bias = at::autocast::cached_cast(t, *bias, at::kCUDA);
+  if (casts) {
+    hidden = at::autocast::cached_cast(cast, hidden, at::kCUDA);
+    weight = at::autocast::cached_cast(cast, weight, at::kCUDA);
+    if (bias) bias = at::autocast::cached_cast(cast, *bias, at::kCUDA);
   }
   TORCH_CHECK_TYPE(hidden.scalar_type() == weight.scalar_type() &&
                        (!bias || bias->scalar_type() == weight.scalar_type()),
@@ -463,13 +493,6 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
   const Tensor rows =
       hidden.dim() == 2 ? hidden : hidden.reshape({-1, hidden.size(-1)});
   const Tensor flat = target.reshape({-1}).contiguous();
-  CHECK_VALUE(rows.size(0) > 0 && rows.size(0) < (1l << 30) &&
-                  weight.size(0) < (1l << 30) &&
-                  rows.size(1) * rows.element_size() < (1l << 22) &&
-                  // a launch has at most 2^31 tiles
-                  (rows.size(0) / 32 + 1) * (weight.size(0) / 64 + 1) <
-                      (1l << 31),
-              "sizes out of range: ", rows.sizes(), " and ", weight.sizes());
 #undef CHECK_VALUE
   const bool grads =
       at::GradMode::is_enabled() &&
@@ -482,4 +505,20 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
                             ignore_index, eps, (Reduction)reduction, Need{})
                   .loss;
   return reduction == NONE ? loss.view(target.sizes()) : loss;
+}
+
+// What a call of these sizes is cut into, for tests: logits' and gradients'
+// tile, pieces' length, dx's and dw's cuts, work items of the largest launch.
+std::vector<int64_t> linear_cross_entropy_plan(int64_t rows, int64_t vocab,
+                                               int64_t dim, int64_t size,
+                                               bool keep) {
+  TORCH_CHECK_VALUE(rows > 0 && vocab > 0 && dim > 0 &&
+                        (size == 2 || size == 4) && rows < (1l << 30) &&
+                        vocab < (1l << 30) && dim * size < (1l << 22),
+                    "linear_cross_entropy_plan: sizes out of range");
+  const int ldim = (int)vocab_loss::padded(dim);
+  const auto p = vocab_loss::plan(rows, vocab, ldim, (int)size, keep);
+  return {(int64_t)p.logits, (int64_t)p.grads, p.piece, p.dx_splits,
+          p.dw_splits,
+          vocab_loss::work_items(p, rows, vocab, ldim, (int)size, keep)};
 }

@@ -875,3 +875,66 @@ def test_operands_with_a_pending_sign(device, reduction):
     assert torch.equal(got[0], want[0])
     for a, c in zip(got[1], want[1]):
         assert torch.equal(a, c)
+
+
+EDGES = {"wide": (256, 256, 512), "mid": (128, 128, 512),
+         "small": (128, 64, 256), "deep": (64, 64, 256),
+         "thin": (64, 32, 256)}
+
+
+def launched(p, rows, vocab, dim, size, keep):
+    """Work items of the largest launch, counted from the plan's tiles."""
+    up = lambda a, b: -(-a // b)
+    tiles = lambda t, m, n: up(m, EDGES[t][0]) * up(n, EDGES[t][1])
+    dim = up(dim, 8) * 8
+    logits = tiles(p["logits"], vocab, rows) * EDGES[p["logits"]][2]
+    grads = (tiles(p["grads"], dim, rows) * p["dx_splits"]
+             + tiles(p["grads"], dim, p["piece"]) * p["dw_splits"]) \
+        * EDGES[p["grads"]][2]
+    return max(logits, grads, up(rows, 4) * 256)
+
+
+def test_sizes_that_no_launch_takes_are_refused():
+    """The runtime launches fewer than 2^32 work items.  On the host: sizes
+    that fit go on to the check of memory, which stands behind it."""
+    from kfac_pytorch_amd.ops import _ext
+    seen = set()
+    for rows, vocab, dim, dtype in [
+            (1, 1, 1, torch.bfloat16), (8192, 128000, 4096, torch.bfloat16),
+            (1 << 21, 1 << 17, 8, torch.bfloat16),
+            (1 << 22, 1 << 17, 8, torch.bfloat16),
+            (1 << 23, 1 << 17, 8, torch.bfloat16),
+            (1 << 17, 1 << 21, 8, torch.float16),
+            (1 << 20, 1 << 20, 64, torch.float16),
+            (1 << 19, 1 << 16, 64, torch.float32),
+            (1 << 19, 1 << 17, 64, torch.float32),
+            ((1 << 26) - 4, 2, 8, torch.bfloat16), (1 << 26, 2, 8,
+                                                    torch.bfloat16),
+            (2, 1 << 28, 8, torch.bfloat16)]:
+        size = dtype.itemsize
+        p = _ext.linear_cross_entropy_plan(rows, vocab, dim, size, False)
+        count = launched(p, rows, vocab, dim, size, False)
+        fits = count < 1 << 32
+        assert (p["work_items"] < 1 << 32) == fits and \
+            p["work_items"] >= count
+        x = Storageless(torch.empty(rows, dim, dtype=dtype, device="meta"))
+        w = Storageless(torch.empty(vocab, dim, dtype=dtype, device="meta"))
+        t = Storageless(torch.empty(rows, dtype=torch.int64, device="meta"))
+        with pytest.raises(TypeError if fits else ValueError,
+                           match="memory" if fits else "out of range"):
+            ops.linear_cross_entropy(x, w, t)
+        seen.add(fits)
+    assert seen == {True, False}
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("rows,vocab", [(1 << 23, 1 << 17), (1 << 26, 2)])
+def test_large_calls_are_refused_before_anything_is_launched(rows, vocab):
+    x = torch.zeros(rows, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(vocab, 8, dtype=torch.bfloat16, device="cuda")
+    t = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    before = torch.cuda.memory_allocated()
+    with pytest.raises(ValueError, match="out of range"):
+        ops.linear_cross_entropy(x, w, t)
+    assert torch.cuda.memory_allocated() == before
