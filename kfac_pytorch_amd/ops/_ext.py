@@ -183,10 +183,11 @@ def linear_cross_entropy_plan(rows: int, vocab: int, dim: int, size: int,
     """How a call of these sizes (values of ``size`` bytes) is cut up; keep:
     with the powers kept for the gradients.  Needs no GPU."""
     tiles = ("wide", "mid", "small", "deep", "thin")
-    logits, grads, piece, dx, dw, items = _load().linear_cross_entropy_plan(
-        rows, vocab, dim, size, keep)
+    logits, grads, piece, dx, dw, part, items = \
+        _load().linear_cross_entropy_plan(rows, vocab, dim, size, keep)
     return {"logits": tiles[logits], "grads": tiles[grads], "piece": piece,
-            "dx_splits": dx, "dw_splits": dw, "work_items": items}
+            "dx_splits": dx, "dw_splits": dw, "part": part,
+            "work_items": items}
 
 
 # -- one norm or inner product over many tensors ------------------------------

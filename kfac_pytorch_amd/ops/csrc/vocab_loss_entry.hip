@@ -508,7 +508,8 @@ Tensor linear_cross_entropy(Tensor hidden, Tensor weight, Tensor target,
 }
 
 // What a call of these sizes is cut into, for tests: logits' and gradients'
-// tile, pieces' length, dx's and dw's cuts, work items of the largest launch.
+// tile, pieces' length, dx's and dw's cuts, tokens to a part of the bias's
+// gradient, work items of the largest launch.
 std::vector<int64_t> linear_cross_entropy_plan(int64_t rows, int64_t vocab,
                                                int64_t dim, int64_t size,
                                                bool keep) {
@@ -519,6 +520,6 @@ std::vector<int64_t> linear_cross_entropy_plan(int64_t rows, int64_t vocab,
   const int ldim = (int)vocab_loss::padded(dim);
   const auto p = vocab_loss::plan(rows, vocab, ldim, (int)size, keep);
   return {(int64_t)p.logits, (int64_t)p.grads, p.piece, p.dx_splits,
-          p.dw_splits,
+          p.dw_splits, p.part,
           vocab_loss::work_items(p, rows, vocab, ldim, (int)size, keep)};
 }

@@ -86,10 +86,22 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
     both raise.
 
     On the GPU a reduced loss computes its gradients in the forward pass if
-    any is asked for (evaluate under ``torch.no_grad()``).  Memory: the
-    gradients, and while the call lasts rows x V values of the inputs' type
-    if that is 4 GiB at most; else, and for ``"none"``, 256 MB pieces of it
-    during the backward pass.
+    any is asked for (evaluate under ``torch.no_grad()``), and scales them
+    by the upstream factor in the first backward pass.
+
+    Memory on the GPU.  While a call lasts: a packed copy of ``hidden``, one
+    of ``weight`` unless its rows are whole 16-byte chunks, 8 or 12 bytes
+    for each row and 32 to 128 entries of the vocabulary, and, for gradients
+    of a reduced loss, rows x V values of the inputs' type if that is 4 GiB
+    at most.  From there to the first backward pass, which allocates the
+    gradients beside it: the weight's gradient, in fp32 for fp16; the fp32
+    partial sums of the hidden states' gradient, one to 64 times rows x d (1
+    to 3 times from some 50 MB on); of the bias's, V for each 4 to 64 rows;
+    and, where the weight's gradient has too few tiles for the GPU, up to 16
+    of its partial sums instead (some 60 MB at most).  Beyond 4 GiB, for
+    ``"none"`` and for a second backward pass nothing is kept: the backward
+    pass makes the logits again, 256 MB of them at a time (64 to 256 entries
+    of the vocabulary at least).
     """
     if reduction not in _REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of "

@@ -938,3 +938,34 @@ def test_large_calls_are_refused_before_anything_is_launched(rows, vocab):
     with pytest.raises(ValueError, match="out of range"):
         ops.linear_cross_entropy(x, w, t)
     assert torch.cuda.memory_allocated() == before
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("rows,dim,vocab,dtype", [
+    (700, 256, 33278, torch.bfloat16), (700, 256, 33278, torch.float16),
+    (700, 256, 33278, torch.float32), (8192, 256, 9521, torch.bfloat16),
+    (4000, 512, 9521, torch.float16), (13, 1000, 20001, torch.bfloat16),
+])
+def test_memory_until_the_backward_pass(rows, dim, vocab, dtype):
+    """What the documentation says: the weight's gradient (fp32 for fp16, or
+    partial sums), partial sums of the others, seven numbers for each row."""
+    from kfac_pytorch_amd.ops import _ext
+    x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.1, 5)
+    leaves = [a.requires_grad_() for a in (x, w, b)]
+    size = dtype.itemsize
+    p = _ext.linear_cross_entropy_plan(rows, vocab, dim, size, True)
+    wide = -(-dim // 8) * 8
+    parts = p["dw_splits"] > 1 or dtype == torch.float16
+    held = 4 * p["dx_splits"] * rows * wide + 4 * vocab * -(-rows // p["part"])
+    held += 4 * p["dw_splits"] * vocab * wide if parts else size * vocab * dim
+    assert 1 <= p["dx_splits"] <= 64 and 1 <= p["dw_splits"] <= 16
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    loss = ops.linear_cross_entropy(x, w, t, bias=b)
+    # the allocator's blocks are whole 512 bytes, large ones whole 2 MB
+    assert torch.cuda.memory_allocated() - before <= held + 28 * rows + (
+        4 << 20)
+    torch.autograd.grad(loss, leaves)
+    del loss
+    assert torch.cuda.memory_allocated() - before <= 512
