@@ -163,7 +163,14 @@ struct Parts {
 
   Parts(const vocab_loss::Operands& o, Type type, Need need) {
     if (need.x) dx = o.plan.dx_splits * o.rows * o.ldx;
-    // fp16 stays in fp32 until the upstream factor, a loss's scale, is known
+    // fp16 stays in fp32 until the upstream factor, a loss's scale, is known:
+    // the type's range is too small to be scaled afterwards.  bf16 that is not
+    // cut up is rounded here and once more where the factor is no power of two
+    // (relative to the norm, off by 2.4e-3 to 2.6e-3 then and 1.9e-3 else; a
+    // layer in bf16 with its loss: 2.4e-3 to 3.6e-3).  In fp32 until the end it
+    // would be 1.9e-3 always and cost the usual factor of 1 a second pass: 700
+    // x 33278 x 256 takes 109.8 us instead of 101.3, 8192 x 128000 x 4096 21.18
+    // ms instead of 20.19, and twice the memory until the backward pass.
     if (need.w && (o.plan.dw_splits > 1 || type == Type::fp16)) {
       dw = o.plan.dw_splits * o.vocab * o.ldx;
     }

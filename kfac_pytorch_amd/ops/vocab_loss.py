@@ -87,7 +87,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
 
     On the GPU a reduced loss computes its gradients in the forward pass if
     any is asked for (evaluate under ``torch.no_grad()``), and scales them
-    by the upstream factor in the first backward pass.
+    by the upstream factor in the first backward pass.  A bf16 gradient of
+    the weight may be rounded twice then, to bf16 before and after a factor
+    that is no power of two.
 
     Memory on the GPU.  While a call lasts: a packed copy of ``hidden``, one
     of ``weight`` unless its rows are whole 16-byte chunks, 8 or 12 bytes

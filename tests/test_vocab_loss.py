@@ -942,6 +942,33 @@ def test_large_calls_are_refused_before_anything_is_launched(rows, vocab):
 
 @pytest.mark.gpu
 @needs_gpu
+@pytest.mark.parametrize("dtype", list(HALF), ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_a_power_of_two_as_upstream_factor_rounds_nothing(dtype, reduction):
+    """It scales the gradients' bits; of a factor that is none, bf16 rounds
+    the weight's gradient once before it and once after."""
+    from kfac_pytorch_amd.ops import _ext
+    rows, dim, vocab = 90, 64, 3000
+    x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.2, 31)
+    assert _ext.linear_cross_entropy_plan(rows, vocab, dim, dtype.itemsize,
+                                          True)["dw_splits"] == 1
+    grads = {}
+    for up in (1.0, 4.0, 0.25, 3.0):
+        grads[up] = run(x, w, b, t, 0.1, reduction,
+                        torch.tensor(up, device="cuda"))[1]
+    # fp16's smallest steps are lost below 2^-14
+    low = 2.0 ** -12 if dtype == torch.float16 else 0.0
+    for up in (4.0, 0.25):
+        for a, c in zip(grads[up], grads[1.0]):
+            assert torch.equal(torch.where(c.abs() >= low, a, 0),
+                               torch.where(c.abs() >= low, c * up, 0))
+    if dtype == torch.bfloat16:
+        assert torch.equal(grads[3.0][1],
+                           (grads[1.0][1].float() * 3).bfloat16())
+
+
+@pytest.mark.gpu
+@needs_gpu
 @pytest.mark.parametrize("rows,dim,vocab,dtype", [
     (700, 256, 33278, torch.bfloat16), (700, 256, 33278, torch.float16),
     (700, 256, 33278, torch.float32), (8192, 256, 9521, torch.bfloat16),
