@@ -120,8 +120,10 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
     kind = hidden.device.type
     if torch.is_autocast_enabled(kind):
         t = torch.get_autocast_dtype(kind)
-        hidden, weight = hidden.to(t), weight.to(t)
-        bias = bias.to(t) if bias is not None else None
+        # autocast leaves float64 alone
+        cast = (lambda a: a if a is None or a.dtype == torch.float64
+                else a.to(t))
+        hidden, weight, bias = cast(hidden), cast(weight), cast(bias)
     if hidden.dtype != weight.dtype or (
             bias is not None and bias.dtype != weight.dtype):
         raise TypeError("linear_cross_entropy: hidden, weight and bias must "

@@ -996,3 +996,14 @@ def test_memory_until_the_backward_pass(rows, dim, vocab, dtype):
     torch.autograd.grad(loss, leaves)
     del loss
     assert torch.cuda.memory_allocated() - before <= 512
+
+
+def test_cpu_autocast_casts_as_a_linear_layer():
+    """To the autocast type, but for float64."""
+    for dtype in (torch.float64, torch.float32, torch.float16):
+        x, w, b, t = inputs(9, 16, 20, dtype, True, 0.2, 3, "cpu")
+        with torch.autocast("cpu", dtype=torch.bfloat16):
+            to = F.linear(x, w, b).dtype
+            got = ops.linear_cross_entropy(x, w, t, bias=b)
+        want = ops.linear_cross_entropy(x.to(to), w.to(to), t, bias=b.to(to))
+        assert torch.equal(got, want) and got.dtype == want.dtype
