@@ -566,7 +566,10 @@ class KFACBase(optim.Optimizer):
             grads += [p.grad.data for p in params]
             updates += self._reshape_preconditioned_grad(
                 module, self.m_precon_grad[module])
+        # (a learning rate on the device would be waited for by that one)
         if (use_clip and grads and not self.exclude_communicate_inverse
+                and not torch.is_tensor(self.lr)
+                and not torch.is_tensor(self.kl_clip)
                 and self._one_pass_update(grads, updates)):
             from kfac_pytorch_amd.ops.grad_scale import kl_clip
             kl_clip(updates, grads, lr=self.lr, kl_clip=self.kl_clip,

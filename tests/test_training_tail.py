@@ -274,3 +274,28 @@ def test_projections_that_are_linear_are_taken():
         plain = getattr(layer, "_orig_mod", layer)
         want = F.cross_entropy(plain(x), t)
         close(ops.projection_loss(layer, x, t), want, REL)
+
+
+@devices
+def test_learning_rate_in_a_tensor_is_not_waited_for(device, monkeypatch,
+                                                     single_process_comm):
+    """It goes the layer-by-layer way, which leaves it on the device; the
+    result is the same."""
+    from kfac_pytorch_amd.ops import grad_scale
+    calls = []
+    real = grad_scale.kl_clip
+    monkeypatch.setattr(grad_scale, "kl_clip",
+                        lambda *a, **kw: calls.append(1) or real(*a, **kw))
+    got = []
+    for lr in (0.5, torch.tensor(0.5, device=device)):
+        torch.manual_seed(1)
+        model = torch.nn.Linear(16, 5).to(device)
+        pre = kfac.KFAC_EIGEN_DP(model, lr=0.5, damping=0.01, kl_clip=1e-3)
+        pre._one_pass_update = lambda grads, updates: True
+        pre.param_groups[0]["lr"] = lr
+        model(torch.randn(4, 16, device=device)).square().sum().backward()
+        pre.step()
+        got.append([p.grad.clone() for p in model.parameters()])
+        assert len(calls) == 1
+    for a, b in zip(*got):
+        close(b, a, 2.0 ** -19)
