@@ -31,6 +31,7 @@ from __future__ import annotations
 import contextlib
 import gc
 import logging
+import threading
 from typing import Dict, List, Optional, Tuple
 
 import torch
@@ -46,16 +47,22 @@ SUPPORTED_MODULES = ("Linear", "Conv2d")
 
 
 class _CapturedGraph:
-    """A captured hipGraph that outlives every capture it is dropped in.
+    """A captured hipGraph that outlives the captures it is dropped in.
 
     Destroying a graph waits for the device, which a stream that is being
     captured does not allow: the destructor's exception ends the process.  A
     preconditioner and its hooked layers refer to each other, so its graphs
     go when the garbage collector runs, and that may be within a capture, its
-    successor's or a user's own.
+    successor's or a user's own.  Seen are captures of the thread's current
+    stream and those of this class in any thread; a user's own capture in
+    another thread is not (drop preconditioners outside of it, or set
+    KFAC_PRED_GRAPH=0).  What was put off goes with the first garbage
+    collection, or the first capture of this class, outside of a capture.
     """
 
     _dropped: List = []  # graphs whose end is put off
+    _captures = 0        # of this class, under way
+    _lock = threading.Lock()
 
     def __init__(self, graph):
         self.graph = graph
@@ -63,14 +70,39 @@ class _CapturedGraph:
     def replay(self):
         self.graph.replay()
 
+    @classmethod
+    def _wait(cls) -> bool:
+        return (cls._captures > 0
+                or torch.cuda.is_current_stream_capturing())
+
     def __del__(self):
-        if torch.cuda.is_current_stream_capturing():
+        if self._wait():
             self._dropped.append(self.graph)
 
     @classmethod
     def sweep(cls):
-        if cls._dropped and not torch.cuda.is_current_stream_capturing():
+        if cls._dropped and not cls._wait():
             cls._dropped.clear()
+
+    @classmethod
+    @contextlib.contextmanager
+    def capture(cls, graph):
+        with cls._lock:
+            cls._captures += 1
+        try:
+            with torch.cuda.graph(graph):
+                yield
+        finally:
+            with cls._lock:
+                cls._captures -= 1
+
+
+def _after_collection(phase, info, graphs=_CapturedGraph):
+    if phase == "stop":
+        graphs.sweep()
+
+
+gc.callbacks.append(_after_collection)
 
 
 @contextlib.contextmanager
@@ -280,7 +312,7 @@ class KFACBase(optim.Optimizer):
             with warnings.catch_warnings(record=True) as caught, \
                     _no_collection():
                 warnings.simplefilter("always")
-                with torch.cuda.graph(graph):
+                with _CapturedGraph.capture(graph):
                     fn()
             # torch only WARNS when a capture lands empty; an empty
             # graph would replay as a silent no-op forever -- treat it

@@ -5,6 +5,7 @@ end the process on a GPU.
 """
 import contextlib
 import gc
+import threading
 
 import pytest
 import torch
@@ -107,3 +108,61 @@ def test_a_graph_dropped_within_a_capture_is_kept_until_after_it(cuda):
     del owner
     gc.collect()  # outside a capture nothing is kept
     assert not dropped
+
+
+def test_what_was_put_off_goes_with_the_next_collection(cuda):
+    """Without another preconditioner that captures."""
+    dropped = base._CapturedGraph._dropped
+    owner = Owner()
+    owner.run("pred", lambda: None, 1)
+    with capture(None):
+        del owner
+        gc.collect()
+        gc.collect()
+        assert len(dropped) == 1
+    gc.collect()
+    assert not dropped
+
+
+def test_a_graph_dropped_while_another_thread_captures(cuda, monkeypatch):
+    """The thread that drops it does not capture itself."""
+    here = threading.current_thread()
+    monkeypatch.setattr(
+        torch.cuda, "is_current_stream_capturing",
+        lambda: Graph.capturing and threading.current_thread() is not here)
+    dropped = base._CapturedGraph._dropped
+    owner = Owner()
+    owner.run("pred", lambda: None, 1)
+    captures, goes_on = threading.Event(), threading.Event()
+
+    def work():
+        if Graph.capturing:
+            captures.set()
+            assert goes_on.wait(30)
+
+    other = Owner()
+    thread = threading.Thread(target=other.run, args=("pred", work, 1))
+    thread.start()
+    try:
+        assert captures.wait(30)
+        owner.me = None  # no cycle: it goes at once
+        del owner
+        assert len(dropped) == 1
+        base._CapturedGraph.sweep()
+        assert len(dropped) == 1
+    finally:
+        goes_on.set()
+        thread.join()
+    assert base._CapturedGraph._captures == 0
+    gc.collect()
+    assert not dropped
+    assert not getattr(other, "_graph_disabled", False)
+
+
+def test_captures_are_counted_when_they_fail(cuda):
+    def fails_in_capture():
+        if Graph.capturing:
+            raise RuntimeError("not capturable")
+
+    Owner().run("pred", fails_in_capture, 1)
+    assert base._CapturedGraph._captures == 0
