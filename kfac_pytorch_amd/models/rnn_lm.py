@@ -31,13 +31,15 @@ class LSTMLanguageModel(nn.Module):
             self.decoder.weight = self.embed.weight
         self.vocab_size = vocab_size
 
-    def forward(self, x, hidden=None, targets=None):
+    def forward(self, x, hidden=None, targets=None, ignore_index=-100):
         """Logits and the LSTM's state; with ``targets`` (token numbers, the
         shape of ``x``) the mean cross entropy instead of the logits, which
-        are then never in memory (``ops.linear_cross_entropy``)."""
+        are then never in memory (``ops.linear_cross_entropy``).  Targets of
+        ``ignore_index`` are left out."""
         emb = self.drop(self.embed(x))
         out, hidden = self.lstm(emb, hidden)
         out = self.drop(out)
         if targets is not None:
-            return projection_loss(self.decoder, out, targets), hidden
+            return projection_loss(self.decoder, out, targets,
+                                   ignore_index=ignore_index), hidden
         return self.decoder(out), hidden

@@ -299,3 +299,15 @@ def test_learning_rate_in_a_tensor_is_not_waited_for(device, monkeypatch,
         assert len(calls) == 1
     for a, b in zip(*got):
         close(b, a, 2.0 ** -19)
+
+
+@devices
+def test_lstm_leaves_out_any_padding_number(device):
+    model, x, y = lstm(device)
+    pad = VOCAB - 1
+    y[y == pad] = 0
+    want, _ = model(x, targets=y)
+    y[y == -100] = pad
+    got, _ = model(x, targets=y, ignore_index=pad)
+    assert torch.equal(got, want)
+    assert not torch.equal(got, model(x, targets=y)[0])
