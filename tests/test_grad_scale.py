@@ -439,3 +439,27 @@ def test_tensors_with_a_pending_sign(device):
     both = [lazy(g) for g in gs]
     got, n = ops.kl_clip(us, both, lr=1.0, kl_clip=0.001, out=both)
     same(both, out, n, nu)
+
+
+@devices
+@pytest.mark.parametrize("update_order,grad_order", [
+    (torch.contiguous_format, torch.channels_last),
+    (torch.channels_last, torch.contiguous_format),
+    (torch.channels_last, torch.channels_last)])
+def test_kl_clip_of_channels_last(update_order, grad_order, device):
+    """Convolutions' gradients in one order, the updates in another; written
+    apart and over the gradients."""
+    shapes = [(6, 5, 3, 3), (16, 16, 1, 1), (33, 7, 5, 5), (4, 1, 3, 3)]
+    us = [u.contiguous(memory_format=update_order)
+          for u in tensors(shapes, torch.float32, device, 1)]
+    gs = [(u * 0.2 + n).contiguous(memory_format=grad_order)
+          for u, n in zip(us, tensors(shapes, torch.float32, device, 2, 0.1))]
+    nu_want = trust(us, gs, 0.5, 0.001)
+    want = [u.double().cpu() * nu_want for u in us]
+    strides = [g.stride() for g in gs]
+    out, nu = ops.kl_clip(us, gs, lr=0.5, kl_clip=0.001)
+    near(nu, torch.tensor(nu_want).double(), 2.0 ** -23)
+    near_out(out, want)
+    ops.kl_clip(us, gs, lr=0.5, kl_clip=0.001, out=gs)
+    near_out(gs, want)
+    assert [g.stride() for g in gs] == strides
