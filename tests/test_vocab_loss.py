@@ -1007,3 +1007,88 @@ def test_cpu_autocast_casts_as_a_linear_layer():
             got = ops.linear_cross_entropy(x, w, t, bias=b)
         want = ops.linear_cross_entropy(x.to(to), w.to(to), t, bias=b.to(to))
         assert torch.equal(got, want) and got.dtype == want.dtype
+
+
+# tokens enough for dw's k to be cut up, by each of the gradients' tiles
+CUT_TOKENS = [(*shape, dtype) for shapes, dtypes in [
+    ([(9420, 149, 1919), (9887, 1744, 74),  # 256 x 256, dx cut up and not
+      (1697, 8, 8474), (5888, 867, 8),      # 128 x 128
+      (6517, 8, 673), (16674, 8, 8),        # 64 x 64
+      (1024, 10, 603), (1142, 8, 9)],       # 64 x 32
+     HALVES),
+    ([(1716, 69, 4269), (9119, 2005, 9),    # 128 x 64
+      (5968, 8, 870), (25825, 8, 8),        # 64 x 64
+      (1122, 8, 664), (1157, 9, 8)],        # 64 x 32
+     [torch.float32]),
+] for shape in shapes for dtype in dtypes]
+
+
+def test_the_lists_reach_every_tile():
+    """Which tile a size takes comes of fitted figures: were they fitted
+    again, a list here might no longer reach every kernel."""
+    from kfac_pytorch_amd.ops import _ext
+    for size, logits, grads in [
+            (2, {"wide", "mid", "small", "deep", "thin"},
+             {"wide", "mid", "deep", "thin"}),
+            (4, {"small", "deep", "thin"}, {"small", "deep", "thin"})]:
+        shapes = {s[:3] for s in EACH_TILE + CUT_TOKENS
+                  if s[3].itemsize == size}
+        for keep in (False, True):
+            plans = [_ext.linear_cross_entropy_plan(rows, vocab, dim, size,
+                                                    keep)
+                     for rows, dim, vocab in shapes]
+            assert {p["logits"] for p in plans} == logits
+            for cut in (False, True):
+                assert {p["grads"] for p in plans
+                        if (p["dw_splits"] > 1) == cut} == grads
+            for tile in grads:
+                assert {p["dx_splits"] > 1 for p in plans
+                        if p["grads"] == tile} == {False, True}
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("rows,dim,vocab,dtype", CUT_TOKENS)
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+def test_cut_tokens(rows, dim, vocab, dtype, reduction):
+    test_each_tile(rows, dim, vocab, dtype, reduction)
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("dtype", HALVES)
+def test_pieces_of_the_vocabulary_in_16_bits(dtype):
+    """As in fp32 above: two pieces, against the whole call.  Either way an
+    entry of g is off by u of itself, the kept one's power by fp16's too."""
+    from kfac_pytorch_amd.ops import _ext
+    rows, dim, vocab = 9000, 16, 17000
+    piece = _ext.linear_cross_entropy_plan(rows, vocab, dim, 2,
+                                           False)["piece"]
+    assert piece < vocab
+    x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.1, 21)
+    up = torch.ones(rows, device="cuda")
+    loss, grads = run(x, w, b, t, 0.1, "none", up)
+    total, kept = run(x, w, b, t, 0.1, "sum")
+    u = HALF[dtype]
+    xd, wd = x.double(), w.double()
+    xd[t == IGNORE] = 0
+    z = xd @ wd.t()
+    z += b.double()
+    z -= torch.logsumexp(z, 1, keepdim=True)
+    z.exp_()
+    z += 0.1 / vocab       # of each entry, |g| at most this, and the target's
+    z[t == IGNORE] = 0
+    at = t.clamp(min=0)
+    # fp16 holds g as g / 2^14 in steps of 2^-24: 2^-39, far below
+    off = 2 * u + 2.0 ** -10 + (vocab + rows) * 2.0 ** -24
+    size = z @ wd.abs() + wd.abs()[at]
+    assert ((grads[0].double() - kept[0].double()).abs()
+            <= (off + 2 * u) * size).all()
+    size = z.t() @ xd.abs()
+    size.index_add_(0, at, xd.abs())
+    assert ((grads[1].double() - kept[1].double()).abs()
+            <= (off + 2 * u) * size + 2.0 ** -24).all()
+    size = z.sum(0) + torch.bincount(t[t >= 0], minlength=vocab)
+    assert ((grads[2].double() - kept[2].double()).abs()
+            <= (off + 2 * u) * size).all()
+    assert abs(float(loss.double().sum() - total)) <= 2e-6 * float(total)
