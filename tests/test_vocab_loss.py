@@ -1092,3 +1092,66 @@ def test_pieces_of_the_vocabulary_in_16_bits(dtype):
     assert ((grads[2].double() - kept[2].double()).abs()
             <= (off + 2 * u) * size).all()
     assert abs(float(loss.double().sum() - total)) <= 2e-6 * float(total)
+
+
+def rounded(v, dtype):
+    return torch.tensor(v, dtype=torch.float64).to(dtype).double().item()
+
+
+def band_of_one_power(bad, ok):
+    """(low, vocab): entries of bias 0 at every 32nd place (so in each band),
+    `low` elsewhere.  exp(low) as `bad` holds it is off by more than 0.8 2^-8,
+    as `ok` by less than 2^-12; its share of the sum lies within a sixth of
+    half a step of a bf16 value, and the bad one's is another value."""
+    for k in range(1, 2000):
+        low = -k / 128.0
+        if rounded(low, torch.bfloat16) != low:
+            continue
+        e = math.exp(low)
+        off = bad(e) / e - 1
+        if abs(off) < 0.8 * 2.0 ** -8 or abs(ok(e) / e - 1) > 2.0 ** -12:
+            continue
+        for vocab in range(64, 4096, 32):
+            p = e / (vocab // 32 * (1 + 31 * e))
+            near = rounded(p, torch.bfloat16)
+            step = 2.0 ** (math.floor(math.log2(near)) - 8)  # half of one
+            if abs(p - near) <= step / 6 and near > 2 ** -100 and rounded(
+                    p * (1 + off), torch.bfloat16) != near:
+                return low, vocab, near
+    raise AssertionError("no such numbers")
+
+
+POWERS = {
+    "not bf16": lambda e: rounded(e, torch.bfloat16),
+    "not fp16 without the lift": lambda e: rounded(e, torch.float16),
+}
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("kind", sorted(POWERS))
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+def test_powers_are_kept_as_lifted_fp16_for_bf16(kind, reduction):
+    """The bias's gradient is summed before g is rounded: of one row of equal
+    powers it shows how these were rounded."""
+    low, vocab, want = band_of_one_power(
+        POWERS[kind], lambda e: rounded(e * 32768, torch.float16) / 32768)
+    b = torch.full((vocab,), low, dtype=torch.bfloat16, device="cuda")
+    b[::32] = 0
+    x = torch.zeros(1, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.ones(vocab, 8, dtype=torch.bfloat16, device="cuda")
+    t = torch.zeros(1, dtype=torch.int64, device="cuda")
+    _, grads = run(x, w, b, t, 0.0, reduction)
+    db = grads[2].double().cpu()
+    db = db[torch.arange(vocab) % 32 != 0]
+    assert (db == want).all()
+
+
+def test_numbers_that_tell_the_powers_types_apart():
+    for bad in POWERS.values():
+        low, vocab, want = band_of_one_power(
+            bad, lambda e: rounded(e * 32768, torch.float16) / 32768)
+        e = math.exp(low)
+        share = lambda v: rounded(v / (vocab // 32 * (1 + 31 * e)),
+                                  torch.bfloat16)
+        assert share(e) == want != share(bad(e))
