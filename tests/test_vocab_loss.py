@@ -872,9 +872,13 @@ def test_operands_with_a_pending_sign(device, reduction):
     want = run(*args, reduction=reduction, up=up)
     got = run(*(lazy(a) for a in args[:3]), t, reduction=reduction,
               up=lazy(up))
-    assert torch.equal(got[0], want[0])
-    for a, c in zip(got[1], want[1]):
-        assert torch.equal(a, c)
+    for a, c in zip((got[0], *got[1]), (want[0], *want[1])):
+        if device == "cuda":
+            assert torch.equal(a, c)
+        else:
+            # a product's order may go by its operands' layout: sums of up to
+            # 70 terms, twice, of at most 16 each
+            assert (a - c).abs().max() <= 2 * 78 * 2.0 ** -24 * 70 * 16
 
 
 EDGES = {"wide": (256, 256, 512), "mid": (128, 128, 512),
