@@ -1159,3 +1159,115 @@ def test_numbers_that_tell_the_powers_types_apart():
         share = lambda v: rounded(v / (vocab // 32 * (1 + 31 * e)),
                                   torch.bfloat16)
         assert share(e) == want != share(bad(e))
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_calls_of_several_threads():
+    """Each on a stream of its own, with sizes in turn: the bits of calls one
+    after the other."""
+    import threading
+    data = [inputs(rows, dim, vocab, dtype, True, 0.2, 7)
+            for rows, dim, vocab, dtype in [
+                (300, 64, 1100, torch.bfloat16),
+                (40, 256, 9000, torch.float16),
+                (129, 72, 700, torch.float32),
+                (1000, 128, 5000, torch.bfloat16)]]
+    want = [run(*a, 0.1) for a in data]
+    torch.cuda.synchronize()
+    done, errors = [], []
+
+    def work(k):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for i in range(12):
+                    j = (k + i) % 4
+                    got = run(*data[j], 0.1)
+                    stream.synchronize()
+                    for a, c in zip((got[0], *got[1]),
+                                    (want[j][0], *want[j][1])):
+                        assert torch.equal(a, c), j
+            done.append(k)
+        except BaseException as e:
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and len(done) == 4
+
+
+@pytest.mark.gpu
+@needs_gpu
+@pytest.mark.parametrize("reduction", ["sum", "none"])
+@pytest.mark.parametrize("rows,dim,vocab,dtype", [
+    (2, 2000000, 3, torch.bfloat16), (2, 1999999, 3, torch.float16),
+    (3, 1000000, 40, torch.float32), (1, 1, 1, torch.bfloat16),
+    (5, 8, 1, torch.float16), (1, 1, 1, torch.float32)])
+def test_ends_of_the_sizes(rows, dim, vocab, dtype, reduction):
+    x, w, b, t = inputs(rows, dim, vocab, dtype, True, 0.0, 3)
+    x = (x / 8).to(dtype)
+    up = torch.ones(rows, device="cuda") if reduction == "none" else None
+    loss, grads = run(x, w, b, t, 0.05, reduction, up)
+    check_all(formula(x, w, b, t, 0.05, torch.ones(rows)),
+              loss if up is not None else None, grads, x, w, b, dtype, rows)
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_saved_on_the_cpu_and_checkpointed():
+    from torch.utils.checkpoint import checkpoint
+    x, w, b, t = inputs(40, 64, 300, torch.bfloat16, True, 0.2, 5)
+    want = run(x, w, b, t)
+    leaves = [a.clone().requires_grad_() for a in (x, w, b)]
+    with torch.autograd.graph.save_on_cpu():
+        loss = ops.linear_cross_entropy(leaves[0], leaves[1], t,
+                                        bias=leaves[2])
+    for a, c in zip(torch.autograd.grad(loss, leaves), want[1]):
+        assert torch.equal(a, c)
+    loss = checkpoint(
+        lambda a, c, d: ops.linear_cross_entropy(a, c, t, bias=d), *leaves,
+        use_reentrant=False)
+    for a, c in zip(torch.autograd.grad(loss, leaves), want[1]):
+        assert torch.equal(a, c)
+    with torch.inference_mode():
+        assert torch.equal(ops.linear_cross_entropy(x, w, t, bias=b), want[0])
+
+
+@pytest.mark.gpu
+@needs_gpu
+def test_step_into_grad_is_captured_and_replayed():
+    """projection_loss and its backward pass into .grad, as a user captures
+    a step."""
+    x, _, _, t = inputs(300, 64, 1100, torch.bfloat16, True, 0.2, 11)
+    layer = torch.nn.Linear(64, 1100, device="cuda", dtype=torch.bfloat16)
+    x.requires_grad_()
+    params = [x, *layer.parameters()]
+
+    def step():
+        for p in params:
+            p.grad = None
+        loss = ops.projection_loss(layer, x, t)
+        loss.backward()
+        return loss.detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step()
+    for seed in range(3):
+        with torch.no_grad():
+            x.copy_(inputs(300, 64, 1100, torch.bfloat16, False, seed=seed)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(x.detach(), layer.weight.detach(), layer.bias.detach(), t)
+        assert torch.equal(loss, want[0])
+        for p, c in zip(params, want[1]):
+            assert torch.equal(p.grad, c)
