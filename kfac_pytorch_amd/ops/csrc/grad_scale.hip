@@ -304,8 +304,9 @@ struct Item {
   long cols;
 };
 
-// Several operands of one shape as rows x cols with unit column stride;
-// false where they are not so.
+// Several operands of one shape as rows x cols with unit column stride; false
+// where they are not so, and the caller copies them: a few launches a tensor
+// (ResNet-50's updates and channels-last gradients: 301 us; of one order: 90).
 template <int NP>
 bool as_rows(const std::array<const Tensor*, NP>& t, Item<NP>* item) {
   Entry<NP>* e = &item->e;

@@ -116,7 +116,7 @@ void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 
 // The powers of a whole call are kept up to this many bytes (while the call
 // lasts); beyond, the backward pass makes the logits again.  Kept, 8192 x
-// 128000 x 4096 in bf16 takes 2 GiB and a fifth less time (25.1 against 20.1
+// 128000 x 4096 in bf16 takes 2 GiB and a fifth less time (25.2 against 20.3
 // ms).
 constexpr long MOST_KEPT = 4l << 30;
 
