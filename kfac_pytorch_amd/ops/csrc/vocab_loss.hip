@@ -252,9 +252,10 @@ __global__ __launch_bounds__(256) void prepare_kernel(
 // holds 4 neighbouring entries of one token, which it can write at once, and
 // a token's sums stay within a column.  A wave's rows are one band.
 // Long k: bound by the matrix cores (8192 x 30522 x 768 in fp16: 415 us at best,
-// 925 TFLOP/s, 470 on the median; the library's product alone 433).  Short k: a tile of 256 x 256 takes
-// 8 us besides its slices of 1.1 us, half of them the 65536 exponentials (8192 x
-// 32768 x 64: one slice, 74 us for 8 rounds; with the powers stored 87).
+// 925 TFLOP/s, 470 on the median; the library's product alone 433).  Short k: a
+// tile of 256 x 256 takes 8 us besides its slices of 1.1 us, half of them the
+// 65536 exponentials (8192 x 32768 x 64: one slice, 74 us for 8 rounds; with the
+// powers stored 87).
 struct Logits {
   long ldw;
   int ldx, v0, vocab;  // the piece [v0, v0 + vocab) of the entries

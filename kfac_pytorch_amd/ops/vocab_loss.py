@@ -97,8 +97,8 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor,
     of a reduced loss, rows x V values of the inputs' type if that is 4 GiB
     at most.  From there to the first backward pass, which allocates the
     gradients beside it: the weight's gradient, in fp32 for fp16; the fp32
-    partial sums of the hidden states' gradient, one to 64 times rows x d (1
-    to 3 times from some 50 MB on); of the bias's, V for each 4 to 64 rows;
+    partial sums of the hidden states' gradient, one to 64 times rows x d (4
+    at most where that is over 70 MB); of the bias's, V for each 4 to 64 rows;
     and, where the weight's gradient has too few tiles for the GPU, up to 16
     of its partial sums instead (some 60 MB at most).  Beyond 4 GiB, for
     ``"none"`` and for a second backward pass nothing is kept: the backward
