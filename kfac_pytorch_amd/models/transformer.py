@@ -67,7 +67,8 @@ class Seq2SeqTransformer(nn.Module):
                 smoothing: float = 0.0, ignore_index: int = -100):
         """Logits; with ``targets`` (token numbers, the shape of ``trg``)
         the mean loss instead, without the logits in memory.  ``smoothing``
-        is ``utils.LabelSmoothLoss``'s (spread over the other tokens)."""
+        is ``utils.LabelSmoothLoss``'s (spread over the other tokens; more
+        than 1 - 1 / V raises)."""
         causal = nn.Transformer.generate_square_subsequent_mask(
             trg.size(1), device=trg.device)
         h = self.transformer(

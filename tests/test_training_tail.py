@@ -311,3 +311,18 @@ def test_lstm_leaves_out_any_padding_number(device):
     got, _ = model(x, targets=y, ignore_index=pad)
     assert torch.equal(got, want)
     assert not torch.equal(got, model(x, targets=y)[0])
+
+
+def test_transformer_smoothing_up_to_uniform():
+    """1 - 1 / V makes all tokens alike; more raises, as a label smoothing
+    past 1 does."""
+    torch.manual_seed(0)
+    model = make_transformer(vocab=20, d_model=16, nhead=2, num_layers=1,
+                             dim_ff=16, max_len=8, dropout=0.0)
+    src, trg = torch.randint(20, (2, 5)), torch.randint(20, (2, 5))
+    loss = model(src, trg[:, :-1], targets=trg[:, 1:], smoothing=0.95)
+    want = LabelSmoothLoss(0.95)(model(src, trg[:, :-1]).reshape(-1, 20),
+                                 trg[:, 1:].reshape(-1))
+    close(loss, want, REL)
+    with pytest.raises(ValueError):
+        model(src, trg[:, :-1], targets=trg[:, 1:], smoothing=0.97)
